@@ -545,6 +545,108 @@ tcx_status tcx_kv_gather(const void* d_pool, uint32_t planes, uint64_t pool_page
                          const uint32_t* d_seq_tokens, const uint64_t* d_out_offsets, uint64_t n_seq,
                          uint64_t total_pages, void* d_out, uint64_t out_bytes, uint32_t* d_status, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Attention over the paged KV pool, and eviction from it (no reference
+ * counterpart). The pool and its tables are tcx_kv_gather's; a page's token row
+ * is kv_heads rows of head_dim 16-bit values.
+ * ------------------------------------------------------------------------ */
+
+#define TCX_KV_BF16 0
+#define TCX_KV_FP16 1
+
+/* One attention call. Sequence s has len = d_seq_tokens[s] tokens in its pages
+ * and nq = d_q_offsets[s+1] - d_q_offsets[s] query tokens, its newest ones: query
+ * i stands at position p = prefix + len - nq + i, token j of the sequence at
+ * prefix + j, where prefix is the length of the shared prefix (0 without one). A
+ * query sees the positions j <= p with window == 0, or j > p - window, or
+ * j < sinks. Its heads are grouped: q head h reads kv head h / (q_heads /
+ * kv_heads).
+ *   out = sum_j exp(scale q.k_j - lse) v_j,  lse = ln sum_j exp(scale q.k_j)
+ * A query that sees nothing has out 0 and lse -inf. */
+typedef struct tcx_kv_attention_args {
+  const void* d_pool;             /* 16-byte aligned */
+  uint64_t planes, pool_pages, page_tokens; /* page_tokens a multiple of 8 */
+  uint64_t kv_heads, q_heads;     /* q_heads a multiple of kv_heads */
+  uint64_t head_dim;              /* 64 or 128 */
+  uint64_t dtype;                 /* TCX_KV_BF16 or TCX_KV_FP16: pool, q and out */
+  uint64_t k_plane, v_plane;
+  const uint32_t* d_page_table;
+  const uint64_t* d_page_offsets; /* [n_seq + 1] */
+  const uint32_t* d_seq_tokens;   /* [n_seq], read on the device by every call */
+  uint64_t n_seq;
+  const uint32_t* d_q_offsets;    /* [n_seq + 1] */
+  uint64_t q_tokens;              /* d_q_offsets[n_seq] (host copy) */
+  uint64_t max_q;                 /* at least every sequence's nq (host bound) */
+  uint64_t total_pages;           /* d_page_offsets[n_seq] (host copy) */
+  uint64_t max_pages;             /* at least every sequence's pages (host bound) */
+  const uint32_t* d_prefix_table; /* pages of the shared prefix; NULL without one */
+  uint64_t prefix_pages;
+  const uint32_t* d_prefix_tokens; /* one value */
+  uint64_t window, sinks;
+  double scale;                   /* > 0 */
+  const void* d_q;                /* element (t, h, e) at t * q_token_stride + h * q_head_stride + e */
+  uint64_t q_token_stride, q_head_stride; /* in elements, multiples of 8; d_q 16-byte aligned */
+  void* d_out;                    /* the same form; overlaps neither q nor the pool */
+  uint64_t out_token_stride, out_head_stride;
+  float* d_lse;                   /* [q_tokens][q_heads] */
+  float* d_weights;               /* NULL, or accumulators: see below */
+  uint64_t weights_head_stride;   /* in elements */
+  uint32_t* d_status;             /* zero before the first call */
+} tcx_kv_attention_args;
+
+/* Scratch of a call with these sizes (pointers are not looked at). */
+uint64_t tcx_kv_attention_scratch_bytes(const tcx_kv_attention_args* args);
+
+/* Runs the call, stream-ordered, on the current device. With d_weights, every
+ * token's softmax weights are added to it: element kv_head * weights_head_stride
+ * + d_page_offsets[s] * page_tokens + j gains the sum over the sequence's queries
+ * and the kv head's q heads of exp(scale q.k_j - lse) (not with a shared prefix).
+ * d_seq_tokens may change between calls (also between replays of a captured
+ * one), up to the pages' capacity. Rows of out and lse from q_tokens on are not
+ * touched. Table entries are checked on the device: a bad one leaves a non-zero
+ * code in *d_status (1 slot out of the pool, 2 more tokens than the pages hold)
+ * and nothing outside the pool is read; the rows of that sequence are then not
+ * meaningful. A call with the same scratch must have ended. Values of tokens that
+ * none of a sequence's queries sees are never used, whatever they hold; a
+ * non-finite value of a token that some of them see may reach the others. */
+tcx_status tcx_kv_attention(const tcx_kv_attention_args* args, void* d_scratch, uint64_t scratch_bytes, void* stream);
+
+/* Eviction: sequence s of n = d_seq_tokens[s] tokens keeps min(n, d_budgets[s])
+ * of them for every layer and kv head: its first `sinks`, its newest `recent`
+ * (both within the budget, sinks first), and of the rest those with the highest
+ * weight (equal ones by lower index; NaN ranks lowest). Plane 2 l holds layer l's
+ * keys, 2 l + 1 its values. The kept rows are copied in their old order to the
+ * destination pages, which must be distinct and none of the source pages; the
+ * source pages are only read. */
+typedef struct tcx_kv_evict_args {
+  void* d_pool;                   /* 16-byte aligned */
+  uint64_t planes;                /* 2 x layers */
+  uint64_t pool_pages, page_tokens, kv_heads;
+  uint64_t head_bytes;            /* bytes of one head's row, a multiple of 16 */
+  const uint32_t* d_page_table;
+  const uint64_t* d_page_offsets; /* [n_seq + 1] */
+  const uint32_t* d_seq_tokens;   /* [n_seq] */
+  const uint32_t* d_dst_page_table;
+  const uint64_t* d_dst_page_offsets; /* [n_seq + 1] */
+  const uint32_t* d_budgets;      /* [n_seq], each within its destination pages */
+  uint64_t n_seq;
+  uint64_t dst_total_pages;       /* d_dst_page_offsets[n_seq] (host copy) */
+  uint64_t sinks, recent;
+  const float* d_weights;         /* (layer, head, page_offsets[s] * page_tokens + j) */
+  uint64_t weights_layer_stride, weights_head_stride; /* in elements */
+  int32_t* d_keep;                /* [layers][kv_heads][dst capacity]: the kept tokens' old indices, -1 behind them */
+  float* d_dst_weights;           /* the same form: their weights, 0 behind them */
+  uint32_t* d_dst_tokens;         /* [n_seq]: min(n, budget) */
+  uint32_t* d_status;
+} tcx_kv_evict_args;
+
+/* Runs the eviction, stream-ordered, on the current device. dst capacity is
+ * dst_total_pages * page_tokens; token r of sequence s stands at
+ * d_dst_page_offsets[s] * page_tokens + r. *d_status as in tcx_kv_gather: 1 a
+ * slot out of the pool (its rows are skipped), 2 more tokens than the pages hold
+ * (the pages' capacity counts), 3 a budget past its destination pages (likewise). */
+tcx_status tcx_kv_evict(const tcx_kv_evict_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

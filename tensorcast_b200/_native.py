@@ -99,6 +99,23 @@ class FileStage(ctypes.Structure):
                 ("ring_slots", _c.c_int), ("slot_bytes", _c.c_uint64)]
 
 
+class KvAttentionArgs(ctypes.Structure):
+    _fields_ = [(n, _c.c_double if n == "scale" else _c.c_void_p if n.startswith("d_") else _c.c_uint64) for n in (
+        "d_pool", "planes", "pool_pages", "page_tokens", "kv_heads", "q_heads", "head_dim", "dtype", "k_plane",
+        "v_plane", "d_page_table", "d_page_offsets", "d_seq_tokens", "n_seq", "d_q_offsets", "q_tokens", "max_q",
+        "total_pages", "max_pages", "d_prefix_table", "prefix_pages", "d_prefix_tokens", "window", "sinks", "scale",
+        "d_q", "q_token_stride", "q_head_stride", "d_out", "out_token_stride", "out_head_stride", "d_lse",
+        "d_weights", "weights_head_stride", "d_status")]
+
+
+class KvEvictArgs(ctypes.Structure):
+    _fields_ = [(n, _c.c_void_p if n.startswith("d_") else _c.c_uint64) for n in (
+        "d_pool", "planes", "pool_pages", "page_tokens", "kv_heads", "head_bytes", "d_page_table", "d_page_offsets",
+        "d_seq_tokens", "d_dst_page_table", "d_dst_page_offsets", "d_budgets", "n_seq", "dst_total_pages", "sinks",
+        "recent", "d_weights", "weights_layer_stride", "weights_head_stride", "d_keep", "d_dst_weights",
+        "d_dst_tokens", "d_status")]
+
+
 # Every function exported by include/tcx.h with (restype, argtypes).
 _SIGNATURES = {
     "tcx_last_error": (_c.c_char_p, []),
@@ -118,6 +135,9 @@ _SIGNATURES = {
     "tcx_kv_gather": (_c.c_int, [_c.c_void_p, _c.c_uint32, _c.c_uint64, _c.c_uint32, _c.c_uint64, _c.c_void_p,
                                  _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_uint64, _c.c_uint64, _c.c_void_p,
                                  _c.c_uint64, _c.c_void_p, _c.c_void_p]),
+    "tcx_kv_attention_scratch_bytes": (_c.c_uint64, [_c.POINTER(KvAttentionArgs)]),
+    "tcx_kv_attention": (_c.c_int, [_c.POINTER(KvAttentionArgs), _c.c_void_p, _c.c_uint64, _c.c_void_p]),
+    "tcx_kv_evict": (_c.c_int, [_c.POINTER(KvEvictArgs), _c.c_void_p]),
     "tcx_merkle_root": (_c.c_int, [_c.c_void_p, _c.c_uint64, _c.c_void_p, _c.c_uint64, _c.c_void_p, _c.c_void_p]),
     "tcx_multihash_encode": (_c.c_int, [_c.c_void_p, _c.c_char_p, _c.c_size_t]),
     "tcx_multihash_from_gpu": (_c.c_int, [_c.c_void_p, _c.c_uint64, _c.c_int, _c.c_uint64, _c.c_char_p, _c.c_size_t]),

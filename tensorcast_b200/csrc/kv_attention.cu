@@ -1,0 +1,288 @@
+// Attention of each sequence's newest tokens over its pages of the KV pool.
+//
+// Query i of a sequence stands at position p and sees the tokens of
+//   [0, min(sinks, p + 1))  and  (p - window, p]        (all of [0, p] without a window),
+// counted from the start of the shared prefix where there is one. A row of the
+// computation is one query token of one q head.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "tcx_internal.h"
+
+namespace tcx {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr uint32_t kBadSlot = 1, kBadLength = 2;
+
+struct AttnArgs {
+  const uint8_t* pool;
+  uint64_t pool_pages, page_bytes, token_bytes, row_bytes;  // row: one head of one token
+  uint32_t page_tokens, kv_heads, group;
+  uint64_t k_plane, v_plane;
+  const uint32_t* page_table;
+  const uint64_t* page_offsets;
+  const uint32_t* seq_tokens;
+  const uint32_t* q_offsets;
+  uint32_t n_seq, q_tokens;
+  const uint32_t* prefix_table;
+  const uint32_t* prefix_tokens;
+  uint64_t prefix_pages;
+  int64_t window, sinks;
+  float scale_log2;  // scale * log2(e): exponents are powers of two
+  const uint8_t* q;
+  uint8_t* out;
+  uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;  // bytes
+  float* lse;
+  float* weights;
+  uint64_t weights_head_stride;
+  uint32_t* status;
+};
+
+// Tokens of sequence s, cut at its pages' capacity.
+__device__ __forceinline__ uint32_t seq_length(const AttnArgs& a, uint32_t s) {
+  const uint64_t cap = (a.page_offsets[s + 1] - a.page_offsets[s]) * a.page_tokens;
+  const uint32_t n = a.seq_tokens[s];
+  if (n > cap) {
+    atomicCAS(a.status, 0u, kBadLength);
+    return static_cast<uint32_t>(cap);
+  }
+  return n;
+}
+
+__device__ __forceinline__ uint32_t prefix_length(const AttnArgs& a) {
+  if (a.prefix_table == nullptr) return 0;
+  const uint64_t cap = a.prefix_pages * a.page_tokens;
+  const uint32_t n = *a.prefix_tokens;
+  if (n > cap) {
+    atomicCAS(a.status, 0u, kBadLength);
+    return static_cast<uint32_t>(cap);
+  }
+  return n;
+}
+
+// The sequence of query token t: q_offsets[s] <= t < q_offsets[s + 1].
+__device__ __forceinline__ uint32_t seq_of(const AttnArgs& a, uint32_t t) {
+  uint32_t lo = 0, hi = a.n_seq;
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (a.q_offsets[mid] <= t) lo = mid; else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ uint64_t checked_slot(const AttnArgs& a, const uint32_t* table, uint64_t page) {
+  const uint32_t slot = table[page];
+  if (slot < a.pool_pages) return slot;
+  atomicCAS(a.status, 0u, kBadSlot);
+  return 0;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_float(T v) {
+  return static_cast<float>(v);
+}
+
+// One warp per row; a lane holds D / 32 dimensions. The running maximum and sum
+// of the softmax are kept in 32 bits over one pass of the visible tokens.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attention_row_kernel(AttnArgs a) {
+  constexpr int E = D / 32;
+  const uint32_t lane = threadIdx.x % 32;
+  const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
+  const uint32_t q_heads = a.kv_heads * a.group;
+  if (row >= static_cast<uint64_t>(a.q_tokens) * q_heads) return;
+  const uint32_t t = static_cast<uint32_t>(row / q_heads), h = static_cast<uint32_t>(row % q_heads);
+  const uint32_t kvh = h / a.group, s = seq_of(a, t);
+  const int64_t len = seq_length(a, s), prefix = prefix_length(a);
+  const int64_t nq = a.q_offsets[s + 1] - a.q_offsets[s];
+  const int64_t pos = prefix + len - nq + (t - a.q_offsets[s]);
+  float q[E], o[E] = {}, m = -INFINITY, l = 0.f;
+  const T* qp = reinterpret_cast<const T*>(a.q + t * a.q_token_stride + h * a.q_head_stride);
+  for (int e = 0; e < E; ++e) q[e] = to_float(qp[lane * E + e]);
+  const int64_t low = a.window ? max(int64_t{0}, pos - a.window + 1) : 0;
+  for (int64_t j = 0; j <= pos; ++j) {
+    if (j >= a.sinks && j < low) j = low;
+    const uint32_t* table = j < prefix ? a.prefix_table : a.page_table + a.page_offsets[s];
+    const int64_t k = j < prefix ? j : j - prefix;
+    const uint64_t off = checked_slot(a, table, k / a.page_tokens) * a.page_bytes +
+                         (k % a.page_tokens) * a.token_bytes + kvh * a.row_bytes;
+    const uint64_t plane = a.pool_pages * a.page_bytes;
+    const T* kp = reinterpret_cast<const T*>(a.pool + a.k_plane * plane + off);
+    const T* vp = reinterpret_cast<const T*>(a.pool + a.v_plane * plane + off);
+    float z = 0.f;
+    for (int e = 0; e < E; ++e) z += q[e] * to_float(kp[lane * E + e]);
+    for (int x = 16; x; x /= 2) z += __shfl_xor_sync(~0u, z, x);
+    z *= a.scale_log2;
+    const float top = fmaxf(m, z), old = m == -INFINITY ? 0.f : exp2f(m - top);
+    const float p = exp2f(z - top);
+    l = l * old + p;
+    for (int e = 0; e < E; ++e) o[e] = o[e] * old + p * to_float(vp[lane * E + e]);
+    m = top;
+  }
+  T* op = reinterpret_cast<T*>(a.out + t * a.out_token_stride + h * a.out_head_stride);
+  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // a NaN sum stays one
+  for (int e = 0; e < E; ++e) op[lane * E + e] = static_cast<T>(o[e] * inv);
+  if (lane == 0) a.lse[static_cast<uint64_t>(t) * q_heads + h] = kLn2 * (m + log2f(l));
+}
+
+// One warp per token and kv head: the token's weights of all rows, added in the
+// rows' order, so that the sum does not depend on the run.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) attention_weights_kernel(AttnArgs a) {
+  constexpr int E = D / 32;
+  const uint32_t lane = threadIdx.x % 32, kvh = blockIdx.y, s = blockIdx.z;
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
+  const int64_t len = seq_length(a, s);
+  if (j >= len) return;
+  const int64_t nq = a.q_offsets[s + 1] - a.q_offsets[s];
+  const uint32_t q_heads = a.kv_heads * a.group;
+  const uint64_t off = checked_slot(a, a.page_table + a.page_offsets[s], j / a.page_tokens) * a.page_bytes +
+                       (j % a.page_tokens) * a.token_bytes + kvh * a.row_bytes;
+  const T* kp = reinterpret_cast<const T*>(a.pool + a.k_plane * a.pool_pages * a.page_bytes + off);
+  float k[E], sum = 0.f;
+  for (int e = 0; e < E; ++e) k[e] = to_float(kp[lane * E + e]);
+  for (int64_t i = 0; i < nq; ++i) {
+    const int64_t pos = len - nq + i;
+    if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) continue;
+    const uint64_t t = a.q_offsets[s] + i;
+    for (uint32_t g = 0; g < a.group; ++g) {
+      const uint32_t h = kvh * a.group + g;
+      const T* qp = reinterpret_cast<const T*>(a.q + t * a.q_token_stride + h * a.q_head_stride);
+      float z = 0.f;
+      for (int e = 0; e < E; ++e) z += to_float(qp[lane * E + e]) * k[e];
+      for (int x = 16; x; x /= 2) z += __shfl_xor_sync(~0u, z, x);
+      sum += exp2f(z * a.scale_log2 - a.lse[t * q_heads + h] * kLog2e);
+    }
+  }
+  if (lane == 0) a.weights[kvh * a.weights_head_stride + a.page_offsets[s] * a.page_tokens + j] += sum;
+}
+
+template <typename T, int D>
+tcx_status launch(const AttnArgs& a, uint64_t max_tokens, cudaStream_t stream) {
+  const uint64_t rows = static_cast<uint64_t>(a.q_tokens) * a.kv_heads * a.group;
+  attention_row_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(a);
+  note_launches(1);
+  TCX_CUDA_TRY(cudaGetLastError());
+  if (a.weights != nullptr && max_tokens > 0) {
+    const dim3 grid(static_cast<unsigned>((max_tokens + 3) / 4), a.kv_heads, a.n_seq);
+    attention_weights_kernel<T, D><<<grid, 128, 0, stream>>>(a);
+    note_launches(1);
+    TCX_CUDA_TRY(cudaGetLastError());
+  }
+  return TCX_OK;
+}
+
+tcx_status check(const tcx_kv_attention_args& a) {
+  if (a.d_pool == nullptr || a.d_page_offsets == nullptr || a.d_seq_tokens == nullptr ||
+      a.d_q_offsets == nullptr || a.d_q == nullptr || a.d_out == nullptr || a.d_lse == nullptr || a.d_status == nullptr)
+    return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
+  if (a.d_page_table == nullptr && a.total_pages != 0) return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
+  if (a.planes == 0 || a.pool_pages == 0 || a.page_tokens == 0 || a.kv_heads == 0 || a.q_heads == 0)
+    return set_error(TCX_INVALID_ARGUMENT, "planes, pool_pages, page_tokens, kv_heads and q_heads must be > 0");
+  if (a.page_tokens % 8 != 0 || a.page_tokens > (1u << 20))
+    return set_errorf(TCX_INVALID_ARGUMENT, "page_tokens must be a multiple of 8 up to 2^20, got %llu",
+                      static_cast<unsigned long long>(a.page_tokens));
+  if (a.head_dim != 64 && a.head_dim != 128)
+    return set_errorf(TCX_INVALID_ARGUMENT, "head_dim must be 64 or 128, got %llu",
+                      static_cast<unsigned long long>(a.head_dim));
+  if (a.dtype != TCX_KV_BF16 && a.dtype != TCX_KV_FP16) return set_error(TCX_INVALID_ARGUMENT, "unknown dtype");
+  if (a.kv_heads > 1024 || a.q_heads > 65536 || a.q_heads % a.kv_heads != 0)
+    return set_errorf(TCX_INVALID_ARGUMENT, "q_heads (%llu) must be a multiple of kv_heads (%llu, at most 1024)",
+                      static_cast<unsigned long long>(a.q_heads), static_cast<unsigned long long>(a.kv_heads));
+  if (a.k_plane >= a.planes || a.v_plane >= a.planes)
+    return set_error(TCX_INVALID_ARGUMENT, "k_plane and v_plane must be planes of the pool");
+  if (a.pool_pages > 0x7fffffffull || a.planes > 0x7fffffffull ||
+      a.pool_pages * a.page_tokens > 0x7fffffffull / a.planes)
+    return set_error(TCX_INVALID_ARGUMENT, "the pool's planes hold 2^31 token rows or more");
+  if (a.n_seq > 65535) return set_error(TCX_INVALID_ARGUMENT, "more than 65535 sequences");
+  if (a.q_tokens > 0x7fffffffull / a.q_heads) return set_error(TCX_INVALID_ARGUMENT, "2^31 query rows or more");
+  if (a.max_q > a.q_tokens || a.total_pages > 0x7fffffffull || a.max_pages > a.total_pages ||
+      a.max_pages > 0x7fffffffull / a.page_tokens || a.prefix_pages > 0x3fffffffull / a.page_tokens)
+    return set_error(TCX_INVALID_ARGUMENT, "inconsistent size bounds");
+  if (a.window > 0x3fffffffull || a.sinks > 0x3fffffffull)
+    return set_error(TCX_INVALID_ARGUMENT, "window and sinks must be below 2^30");
+  if (!(a.scale > 0) || !(a.scale * 1.4426950408889634 <= 3e38) || !(static_cast<float>(a.scale * kLog2e) > 0))
+    return set_error(TCX_INVALID_ARGUMENT, "scale must be > 0 and finite");
+  if ((reinterpret_cast<uintptr_t>(a.d_pool) | reinterpret_cast<uintptr_t>(a.d_q) |
+       reinterpret_cast<uintptr_t>(a.d_out)) & 15u)
+    return set_error(TCX_INVALID_ARGUMENT, "pool, q and out must be 16-byte aligned");
+  if ((a.q_token_stride | a.q_head_stride | a.out_token_stride | a.out_head_stride) % 8 != 0)
+    return set_error(TCX_INVALID_ARGUMENT, "strides of q and out must be multiples of 8 elements");
+  if (a.d_prefix_table != nullptr) {
+    if (a.d_prefix_tokens == nullptr) return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
+    if (a.d_weights != nullptr)
+      return set_error(TCX_INVALID_ARGUMENT, "weights are not accumulated with a shared prefix");
+  }
+  return TCX_OK;
+}
+
+AttnArgs device_args(const tcx_kv_attention_args& x) {
+  AttnArgs a{};
+  a.pool = static_cast<const uint8_t*>(x.d_pool);
+  a.pool_pages = x.pool_pages;
+  a.row_bytes = x.head_dim * 2;
+  a.token_bytes = x.kv_heads * a.row_bytes;
+  a.page_bytes = x.page_tokens * a.token_bytes;
+  a.page_tokens = static_cast<uint32_t>(x.page_tokens);
+  a.kv_heads = static_cast<uint32_t>(x.kv_heads);
+  a.group = static_cast<uint32_t>(x.q_heads / x.kv_heads);
+  a.k_plane = x.k_plane;
+  a.v_plane = x.v_plane;
+  a.page_table = x.d_page_table;
+  a.page_offsets = x.d_page_offsets;
+  a.seq_tokens = x.d_seq_tokens;
+  a.q_offsets = x.d_q_offsets;
+  a.n_seq = static_cast<uint32_t>(x.n_seq);
+  a.q_tokens = static_cast<uint32_t>(x.q_tokens);
+  a.prefix_table = x.d_prefix_table;
+  a.prefix_tokens = x.d_prefix_tokens;
+  a.prefix_pages = x.prefix_pages;
+  a.window = static_cast<int64_t>(x.window);
+  a.sinks = static_cast<int64_t>(x.sinks);
+  a.scale_log2 = static_cast<float>(x.scale * 1.4426950408889634);
+  a.q = static_cast<const uint8_t*>(x.d_q);
+  a.out = static_cast<uint8_t*>(x.d_out);
+  a.q_token_stride = x.q_token_stride * 2;
+  a.q_head_stride = x.q_head_stride * 2;
+  a.out_token_stride = x.out_token_stride * 2;
+  a.out_head_stride = x.out_head_stride * 2;
+  a.lse = x.d_lse;
+  a.weights = x.d_weights;
+  a.weights_head_stride = x.weights_head_stride;
+  a.status = x.d_status;
+  return a;
+}
+
+}  // namespace
+}  // namespace tcx
+
+using namespace tcx;
+
+extern "C" uint64_t tcx_kv_attention_scratch_bytes(const tcx_kv_attention_args* args) {
+  (void)args;
+  return 0;
+}
+
+extern "C" tcx_status tcx_kv_attention(const tcx_kv_attention_args* args, void* d_scratch, uint64_t scratch_bytes,
+                                       void* stream) {
+  if (args == nullptr) return set_error(TCX_INVALID_ARGUMENT, "null arguments");
+  if (args->n_seq == 0 || args->q_tokens == 0) return TCX_OK;
+  if (const tcx_status st = check(*args); st != TCX_OK) return st;
+  const uint64_t need = tcx_kv_attention_scratch_bytes(args);
+  if (scratch_bytes < need || (need != 0 && d_scratch == nullptr))
+    return set_errorf(TCX_INVALID_ARGUMENT, "scratch too small: %llu bytes, %llu needed",
+                      static_cast<unsigned long long>(scratch_bytes), static_cast<unsigned long long>(need));
+  const AttnArgs a = device_args(*args);
+  const uint64_t max_tokens = args->max_pages * args->page_tokens;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (args->dtype == TCX_KV_BF16)
+    return args->head_dim == 128 ? launch<__nv_bfloat16, 128>(a, max_tokens, s)
+                                 : launch<__nv_bfloat16, 64>(a, max_tokens, s);
+  return args->head_dim == 128 ? launch<__half, 128>(a, max_tokens, s) : launch<__half, 64>(a, max_tokens, s);
+}

@@ -1,0 +1,266 @@
+// Eviction from the paged KV pool: the tokens with the highest accumulated
+// attention weight of every (sequence, layer, kv head) stay, and their rows are
+// copied in their old order to the sequence's destination pages.
+//
+// Two launches: select_kernel, one CTA per (layer, kv head, sequence), finds the
+// budget's weight by radix selection over the weights' order-preserving integer
+// images and writes the kept indices; copy_kernel moves the rows, bound by HBM
+// (each kept row is read and written once). The destination pages are not the
+// source's: a page may be shared with other sequences, and the copy needs no
+// order between its CTAs.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "tcx_internal.h"
+
+namespace tcx {
+namespace {
+
+constexpr int kSelectThreads = 512;
+constexpr int kCopyThreads = 256;
+constexpr int kBins = 256;
+
+struct EvictArgs {
+  uint8_t* pool;
+  uint64_t pool_pages, page_bytes, token_bytes, head_bytes;
+  uint32_t page_tokens, kv_heads, n_seq;
+  const uint32_t* page_table;
+  const uint64_t* page_offsets;
+  const uint32_t* seq_tokens;
+  const uint32_t* dst_page_table;
+  const uint64_t* dst_page_offsets;
+  const uint32_t* budgets;
+  uint64_t dst_capacity, sinks, recent;
+  const float* weights;
+  uint64_t weights_layer_stride, weights_head_stride;
+  int32_t* keep;
+  float* dst_weights;
+  uint32_t* dst_tokens;
+  uint32_t* status;
+};
+
+// Tokens of sequence s and how many of them it keeps, both cut at their pages.
+__device__ __forceinline__ void lengths(const EvictArgs& a, uint32_t s, uint32_t* n, uint32_t* kept) {
+  const uint64_t cap = (a.page_offsets[s + 1] - a.page_offsets[s]) * a.page_tokens;
+  const uint64_t dst_cap = (a.dst_page_offsets[s + 1] - a.dst_page_offsets[s]) * a.page_tokens;
+  uint64_t have = a.seq_tokens[s], budget = a.budgets[s];
+  if (have > cap) {
+    atomicCAS(a.status, 0u, 2u);
+    have = cap;
+  }
+  if (budget > dst_cap) {
+    atomicCAS(a.status, 0u, 3u);
+    budget = dst_cap;
+  }
+  *n = static_cast<uint32_t>(have);
+  *kept = static_cast<uint32_t>(min(have, budget));
+}
+
+// Larger weights have larger images; -0 and 0 have the same, NaN the lowest.
+__device__ __forceinline__ uint32_t image(float w) {
+  if (w != w) return 0;
+  const uint32_t b = __float_as_uint(w + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// Exclusive sum over the CTA of one value per thread; *total gets the sum.
+__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, uint32_t* total) {
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+  uint32_t inc = v;
+  for (int d = 1; d < 32; d *= 2) {
+    const uint32_t up = __shfl_up_sync(~0u, inc, d);
+    if (lane >= d) inc += up;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = inc;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+  for (uint32_t w = 0; w < warps; ++w) {
+    if (w < warp) before += warp_sums[w];
+    all += warp_sums[w];
+  }
+  *total = all;
+  return before + inc - v;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
+  __shared__ uint32_t bins[kBins], warp_sums[kSelectThreads / 32], s_pick[2];
+  const uint32_t head = blockIdx.x, layer = blockIdx.y, s = blockIdx.z;
+  uint32_t n, kept;
+  lengths(a, s, &n, &kept);
+  const uint64_t base = a.page_offsets[s] * a.page_tokens, dst_base = a.dst_page_offsets[s] * a.page_tokens;
+  const uint64_t dst_cap = a.dst_page_offsets[s + 1] * a.page_tokens - dst_base;
+  const float* w = a.weights + layer * a.weights_layer_stride + head * a.weights_head_stride + base;
+  const uint64_t plane = (static_cast<uint64_t>(layer) * a.kv_heads + head) * a.dst_capacity + dst_base;
+  int32_t* keep = a.keep + plane;
+  float* left = a.dst_weights + plane;
+  if (layer == 0 && head == 0 && threadIdx.x == 0) a.dst_tokens[s] = kept;
+  for (uint64_t r = kept + threadIdx.x; r < dst_cap; r += blockDim.x) {
+    keep[r] = -1;
+    left[r] = 0.f;
+  }
+  if (n == kept) {
+    for (uint32_t j = threadIdx.x; j < n; j += blockDim.x) {
+      keep[j] = static_cast<int32_t>(j);
+      left[j] = w[j];
+    }
+    return;
+  }
+  // The first `first` and the tokens from `last` on stay; `want` more of those between.
+  const uint32_t first = static_cast<uint32_t>(min(a.sinks, static_cast<uint64_t>(kept)));
+  const uint32_t newest = static_cast<uint32_t>(min(a.recent, static_cast<uint64_t>(kept - first)));
+  const uint32_t last = n - newest;
+  uint32_t want = kept - first - newest;
+  uint32_t prefix = 0, known = 0;  // the wanted image's upper bits, and their mask
+  if (want > 0) {
+    for (int shift = 24; shift >= 0; shift -= 8) {
+      for (uint32_t b = threadIdx.x; b < kBins; b += blockDim.x) bins[b] = 0;
+      __syncthreads();
+      for (uint32_t j = first + threadIdx.x; j < last; j += blockDim.x) {
+        const uint32_t x = image(w[j]);
+        if ((x & known) == prefix) atomicAdd(&bins[x >> shift & 255], 1u);
+      }
+      __syncthreads();
+      // thread b: how many lie in higher bins than 255 - b
+      uint32_t all;
+      const uint32_t mine = threadIdx.x < kBins ? bins[kBins - 1 - threadIdx.x] : 0;
+      const uint32_t above = block_scan(mine, warp_sums, &all);
+      if (threadIdx.x < kBins && above < want && above + mine >= want) {
+        s_pick[0] = kBins - 1 - threadIdx.x;
+        s_pick[1] = above;
+      }
+      __syncthreads();
+      prefix |= s_pick[0] << shift;
+      known |= 255u << shift;
+      want -= s_pick[1];
+      __syncthreads();
+    }
+  }
+  // `want` of the tokens with exactly this image stay, the lowest indices first.
+  const bool any = kept > first + newest;
+  uint32_t done = 0, equal_done = 0;
+  for (uint32_t j0 = 0; j0 < n; j0 += blockDim.x) {
+    const uint32_t j = j0 + threadIdx.x;
+    const float v = j < n ? w[j] : 0.f;
+    const bool middle = j >= first && j < last, safe = j < n && !middle;
+    const uint32_t x = image(v);
+    uint32_t total;
+    const uint32_t equal = any && middle && x == prefix;
+    const uint32_t equal_before = equal_done + block_scan(equal, warp_sums, &total);
+    equal_done += total;
+    const uint32_t stay = safe || (any && middle && x > prefix) || (equal && equal_before < want);
+    const uint32_t r = done + block_scan(stay, warp_sums, &total);
+    done += total;
+    if (stay) {
+      keep[r] = static_cast<int32_t>(j);
+      left[r] = v;
+    }
+  }
+}
+
+// One CTA moves one destination page of one plane, in 16-byte pieces.
+__global__ void __launch_bounds__(kCopyThreads) copy_kernel(EvictArgs a) {
+  const uint64_t page = blockIdx.x;
+  const uint32_t plane = blockIdx.y;
+  uint32_t lo = 0, hi = a.n_seq;  // dst_page_offsets[lo] <= page < dst_page_offsets[lo + 1]
+  while (hi - lo > 1) {
+    const uint32_t mid = (lo + hi) / 2;
+    if (a.dst_page_offsets[mid] <= page) lo = mid; else hi = mid;
+  }
+  uint32_t n, kept;
+  lengths(a, lo, &n, &kept);
+  const uint64_t r0 = (page - a.dst_page_offsets[lo]) * a.page_tokens;
+  if (r0 >= kept) return;
+  const uint32_t rows = static_cast<uint32_t>(min(static_cast<uint64_t>(a.page_tokens), kept - r0));
+  const uint32_t dst_slot = a.dst_page_table[page];
+  if (dst_slot >= a.pool_pages) {
+    if (threadIdx.x == 0) atomicCAS(a.status, 0u, 1u);
+    return;
+  }
+  const uint64_t plane_off = plane * a.pool_pages * a.page_bytes;
+  const uint32_t* table = a.page_table + a.page_offsets[lo];
+  const int32_t* keep = a.keep + static_cast<uint64_t>(plane / 2) * a.kv_heads * a.dst_capacity + page * a.page_tokens;
+  const uint32_t pieces = static_cast<uint32_t>(a.head_bytes / 16), per_token = pieces * a.kv_heads;
+  for (uint32_t i = threadIdx.x; i < rows * per_token; i += blockDim.x) {
+    const uint32_t r = i / per_token, head = i % per_token / pieces, piece = i % pieces;
+    const uint32_t j = static_cast<uint32_t>(keep[head * a.dst_capacity + r]);
+    const uint32_t slot = table[j / a.page_tokens];
+    if (slot >= a.pool_pages) {
+      atomicCAS(a.status, 0u, 1u);
+      continue;
+    }
+    const uint64_t in = head * a.head_bytes + piece * 16;
+    const uint4 v = *reinterpret_cast<const uint4*>(a.pool + plane_off + slot * a.page_bytes +
+                                                    j % a.page_tokens * a.token_bytes + in);
+    *reinterpret_cast<uint4*>(a.pool + plane_off + dst_slot * a.page_bytes + r * a.token_bytes + in) = v;
+  }
+}
+
+}  // namespace
+}  // namespace tcx
+
+using namespace tcx;
+
+extern "C" tcx_status tcx_kv_evict(const tcx_kv_evict_args* args, void* stream) {
+  if (args == nullptr) return set_error(TCX_INVALID_ARGUMENT, "null arguments");
+  const tcx_kv_evict_args& x = *args;
+  if (x.n_seq == 0) return TCX_OK;
+  if (x.d_pool == nullptr || x.d_page_offsets == nullptr || x.d_seq_tokens == nullptr ||
+      x.d_dst_page_offsets == nullptr || x.d_budgets == nullptr || x.d_weights == nullptr ||
+      x.d_dst_tokens == nullptr || x.d_status == nullptr)
+    return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
+  if (x.dst_total_pages != 0 && (x.d_page_table == nullptr || x.d_dst_page_table == nullptr || x.d_keep == nullptr ||
+                                 x.d_dst_weights == nullptr))
+    return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
+  if (x.planes == 0 || x.planes % 2 != 0 || x.pool_pages == 0 || x.page_tokens == 0 || x.kv_heads == 0)
+    return set_error(TCX_INVALID_ARGUMENT,
+                     "planes must be even, and planes, pool_pages, page_tokens and kv_heads > 0");
+  if (x.pool_pages > 0xffffffffull) return set_error(TCX_INVALID_ARGUMENT, "pool_pages exceeds 2^32");
+  if (x.head_bytes == 0 || x.head_bytes % 16 != 0 || x.head_bytes > (1u << 20))
+    return set_errorf(TCX_INVALID_ARGUMENT, "head_bytes must be a multiple of 16 up to 2^20, got %llu",
+                      static_cast<unsigned long long>(x.head_bytes));
+  if (x.planes > 65535 || x.kv_heads > 65535 || x.n_seq > 65535 || x.page_tokens > (1u << 20) ||
+      x.page_tokens * x.kv_heads * (x.head_bytes / 16) > 0x7fffffffull)
+    return set_error(TCX_INVALID_ARGUMENT, "planes, kv_heads, n_seq (65535) or page size out of range");
+  if (x.dst_total_pages > 0x7fffffffull / x.page_tokens)
+    return set_error(TCX_INVALID_ARGUMENT, "destination pages hold 2^31 tokens or more");
+  if (reinterpret_cast<uintptr_t>(x.d_pool) & 15u) return set_error(TCX_INVALID_ARGUMENT, "pool must be 16-byte aligned");
+  EvictArgs a{};
+  a.pool = static_cast<uint8_t*>(x.d_pool);
+  a.pool_pages = x.pool_pages;
+  a.head_bytes = x.head_bytes;
+  a.token_bytes = x.kv_heads * x.head_bytes;
+  a.page_bytes = x.page_tokens * a.token_bytes;
+  a.page_tokens = static_cast<uint32_t>(x.page_tokens);
+  a.kv_heads = static_cast<uint32_t>(x.kv_heads);
+  a.n_seq = static_cast<uint32_t>(x.n_seq);
+  a.page_table = x.d_page_table;
+  a.page_offsets = x.d_page_offsets;
+  a.seq_tokens = x.d_seq_tokens;
+  a.dst_page_table = x.d_dst_page_table;
+  a.dst_page_offsets = x.d_dst_page_offsets;
+  a.budgets = x.d_budgets;
+  a.dst_capacity = x.dst_total_pages * x.page_tokens;
+  a.sinks = x.sinks;
+  a.recent = x.recent;
+  a.weights = x.d_weights;
+  a.weights_layer_stride = x.weights_layer_stride;
+  a.weights_head_stride = x.weights_head_stride;
+  a.keep = x.d_keep;
+  a.dst_weights = x.d_dst_weights;
+  a.dst_tokens = x.d_dst_tokens;
+  a.status = x.d_status;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const dim3 select_grid(a.kv_heads, static_cast<unsigned>(x.planes / 2), a.n_seq);
+  select_kernel<<<select_grid, kSelectThreads, 0, s>>>(a);
+  note_launches(1);
+  TCX_CUDA_TRY(cudaGetLastError());
+  if (x.dst_total_pages != 0) {
+    const dim3 copy_grid(static_cast<unsigned>(x.dst_total_pages), static_cast<unsigned>(x.planes));
+    copy_kernel<<<copy_grid, kCopyThreads, 0, s>>>(a);
+    note_launches(1);
+    TCX_CUDA_TRY(cudaGetLastError());
+  }
+  return TCX_OK;
+}
