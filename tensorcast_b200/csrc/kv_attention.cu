@@ -9,79 +9,13 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
-#include "tcx_internal.h"
+#include "kv_attention.cuh"
 
 namespace tcx {
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr uint32_t kBadSlot = 1, kBadLength = 2;
-
-struct AttnArgs {
-  const uint8_t* pool;
-  uint64_t pool_pages, page_bytes, token_bytes, row_bytes;  // row: one head of one token
-  uint32_t page_tokens, kv_heads, group;
-  uint64_t k_plane, v_plane;
-  const uint32_t* page_table;
-  const uint64_t* page_offsets;
-  const uint32_t* seq_tokens;
-  const uint32_t* q_offsets;
-  uint32_t n_seq, q_tokens;
-  const uint32_t* prefix_table;
-  const uint32_t* prefix_tokens;
-  uint64_t prefix_pages;
-  int64_t window, sinks;
-  float scale_log2;  // scale * log2(e): exponents are powers of two
-  const uint8_t* q;
-  uint8_t* out;
-  uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;  // bytes
-  float* lse;
-  float* weights;
-  uint64_t weights_head_stride;
-  uint32_t* status;
-};
-
-// Tokens of sequence s, cut at its pages' capacity.
-__device__ __forceinline__ uint32_t seq_length(const AttnArgs& a, uint32_t s) {
-  const uint64_t cap = (a.page_offsets[s + 1] - a.page_offsets[s]) * a.page_tokens;
-  const uint32_t n = a.seq_tokens[s];
-  if (n > cap) {
-    atomicCAS(a.status, 0u, kBadLength);
-    return static_cast<uint32_t>(cap);
-  }
-  return n;
-}
-
-__device__ __forceinline__ uint32_t prefix_length(const AttnArgs& a) {
-  if (a.prefix_table == nullptr) return 0;
-  const uint64_t cap = a.prefix_pages * a.page_tokens;
-  const uint32_t n = *a.prefix_tokens;
-  if (n > cap) {
-    atomicCAS(a.status, 0u, kBadLength);
-    return static_cast<uint32_t>(cap);
-  }
-  return n;
-}
-
-// The sequence of query token t: q_offsets[s] <= t < q_offsets[s + 1].
-__device__ __forceinline__ uint32_t seq_of(const AttnArgs& a, uint32_t t) {
-  uint32_t lo = 0, hi = a.n_seq;
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (a.q_offsets[mid] <= t) lo = mid; else hi = mid;
-  }
-  return lo;
-}
-
-__device__ __forceinline__ uint64_t checked_slot(const AttnArgs& a, const uint32_t* table, uint64_t page) {
-  const uint32_t slot = table[page];
-  if (slot < a.pool_pages) return slot;
-  atomicCAS(a.status, 0u, kBadSlot);
-  return 0;
-}
 
 template <typename T>
 __device__ __forceinline__ float to_float(T v) {
@@ -164,11 +98,13 @@ __global__ void __launch_bounds__(128) attention_weights_kernel(AttnArgs a) {
 }
 
 template <typename T, int D>
-tcx_status launch(const AttnArgs& a, uint64_t max_tokens, cudaStream_t stream) {
-  const uint64_t rows = static_cast<uint64_t>(a.q_tokens) * a.kv_heads * a.group;
-  attention_row_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(a);
-  note_launches(1);
-  TCX_CUDA_TRY(cudaGetLastError());
+tcx_status launch(const AttnArgs& a, bool rows_done, uint64_t max_tokens, cudaStream_t stream) {
+  if (!rows_done) {
+    const uint64_t rows = static_cast<uint64_t>(a.q_tokens) * a.kv_heads * a.group;
+    attention_row_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(a);
+    note_launches(1);
+    TCX_CUDA_TRY(cudaGetLastError());
+  }
   if (a.weights != nullptr && max_tokens > 0) {
     const dim3 grid(static_cast<unsigned>((max_tokens + 3) / 4), a.kv_heads, a.n_seq);
     attention_weights_kernel<T, D><<<grid, 128, 0, stream>>>(a);
@@ -178,11 +114,7 @@ tcx_status launch(const AttnArgs& a, uint64_t max_tokens, cudaStream_t stream) {
   return TCX_OK;
 }
 
-tcx_status check(const tcx_kv_attention_args& a) {
-  if (a.d_pool == nullptr || a.d_page_offsets == nullptr || a.d_seq_tokens == nullptr ||
-      a.d_q_offsets == nullptr || a.d_q == nullptr || a.d_out == nullptr || a.d_lse == nullptr || a.d_status == nullptr)
-    return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
-  if (a.d_page_table == nullptr && a.total_pages != 0) return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
+tcx_status check_sizes(const tcx_kv_attention_args& a) {
   if (a.planes == 0 || a.pool_pages == 0 || a.page_tokens == 0 || a.kv_heads == 0 || a.q_heads == 0)
     return set_error(TCX_INVALID_ARGUMENT, "planes, pool_pages, page_tokens, kv_heads and q_heads must be > 0");
   if (a.page_tokens % 8 != 0 || a.page_tokens > (1u << 20))
@@ -209,6 +141,15 @@ tcx_status check(const tcx_kv_attention_args& a) {
     return set_error(TCX_INVALID_ARGUMENT, "window and sinks must be below 2^30");
   if (!(a.scale > 0) || !(a.scale * 1.4426950408889634 <= 3e38) || !(static_cast<float>(a.scale * kLog2e) > 0))
     return set_error(TCX_INVALID_ARGUMENT, "scale must be > 0 and finite");
+  return TCX_OK;
+}
+
+tcx_status check(const tcx_kv_attention_args& a) {
+  if (a.d_pool == nullptr || a.d_page_offsets == nullptr || a.d_seq_tokens == nullptr ||
+      a.d_q_offsets == nullptr || a.d_q == nullptr || a.d_out == nullptr || a.d_lse == nullptr || a.d_status == nullptr)
+    return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
+  if (a.d_page_table == nullptr && a.total_pages != 0) return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
+  if (const tcx_status st = check_sizes(a); st != TCX_OK) return st;
   if ((reinterpret_cast<uintptr_t>(a.d_pool) | reinterpret_cast<uintptr_t>(a.d_q) |
        reinterpret_cast<uintptr_t>(a.d_out)) & 15u)
     return set_error(TCX_INVALID_ARGUMENT, "pool, q and out must be 16-byte aligned");
@@ -256,17 +197,45 @@ AttnArgs device_args(const tcx_kv_attention_args& x) {
   a.weights = x.d_weights;
   a.weights_head_stride = x.weights_head_stride;
   a.status = x.d_status;
+  a.box_rows = std::min<uint32_t>(64, a.page_tokens & -a.page_tokens);
+  a.k_row0 = x.k_plane * x.pool_pages * x.page_tokens;
+  a.v_row0 = x.v_plane * x.pool_pages * x.page_tokens;
   return a;
 }
 
 }  // namespace
+
+tcx_status encode_pool_map(const tcx_kv_attention_args& x, uint32_t box_rows, CUtensorMap* map) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<void*> entry{nullptr};
+  void* f = entry.load(std::memory_order_relaxed);
+  if (f == nullptr) {
+    cudaDriverEntryPointQueryResult found;
+    TCX_CUDA_TRY(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &found));
+    if (found != cudaDriverEntryPointSuccess || f == nullptr)
+      return set_error(TCX_INTERNAL, "the driver has no cuTensorMapEncodeTiled");
+    entry.store(f, std::memory_order_relaxed);
+  }
+  const cuuint64_t dims[3] = {x.head_dim, x.kv_heads, x.planes * x.pool_pages * x.page_tokens};
+  const cuuint64_t strides[2] = {x.head_dim * 2, x.head_dim * 2 * x.kv_heads};
+  const cuuint32_t box[3] = {64, 1, box_rows}, ones[3] = {1, 1, 1};
+  const CUresult rc = reinterpret_cast<Encode>(f)(
+      map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<void*>(x.d_pool), dims, strides, box, ones,
+      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return set_errorf(TCX_INTERNAL, "cuTensorMapEncodeTiled failed: %d", static_cast<int>(rc));
+  return TCX_OK;
+}
+
 }  // namespace tcx
 
 using namespace tcx;
 
 extern "C" uint64_t tcx_kv_attention_scratch_bytes(const tcx_kv_attention_args* args) {
-  (void)args;
-  return 0;
+  if (args == nullptr || args->n_seq == 0 || args->q_tokens == 0 || check_sizes(*args) != TCX_OK) return 0;
+  return decode_fits(*args) ? decode_scratch_bytes(*args) : 0;
 }
 
 extern "C" tcx_status tcx_kv_attention(const tcx_kv_attention_args* args, void* d_scratch, uint64_t scratch_bytes,
@@ -279,10 +248,17 @@ extern "C" tcx_status tcx_kv_attention(const tcx_kv_attention_args* args, void* 
     return set_errorf(TCX_INVALID_ARGUMENT, "scratch too small: %llu bytes, %llu needed",
                       static_cast<unsigned long long>(scratch_bytes), static_cast<unsigned long long>(need));
   const AttnArgs a = device_args(*args);
+  const bool rows_done = decode_fits(*args);
+  if (rows_done) {
+    CUtensorMap map;
+    if (const tcx_status st = encode_pool_map(*args, a.box_rows, &map); st != TCX_OK) return st;
+    if (const tcx_status st = launch_decode(*args, a, map, d_scratch, static_cast<cudaStream_t>(stream)); st != TCX_OK)
+      return st;
+  }
   const uint64_t max_tokens = args->max_pages * args->page_tokens;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (args->dtype == TCX_KV_BF16)
-    return args->head_dim == 128 ? launch<__nv_bfloat16, 128>(a, max_tokens, s)
-                                 : launch<__nv_bfloat16, 64>(a, max_tokens, s);
-  return args->head_dim == 128 ? launch<__half, 128>(a, max_tokens, s) : launch<__half, 64>(a, max_tokens, s);
+    return args->head_dim == 128 ? launch<__nv_bfloat16, 128>(a, rows_done, max_tokens, s)
+                                 : launch<__nv_bfloat16, 64>(a, rows_done, max_tokens, s);
+  return args->head_dim == 128 ? launch<__half, 128>(a, rows_done, max_tokens, s) : launch<__half, 64>(a, rows_done, max_tokens, s);
 }

@@ -1,0 +1,464 @@
+// Attention of few query rows over long paged sequences (decode).
+//
+// A kv head's rows (query tokens x the head's group of q heads, up to 16) share
+// the keys and values, so the call is bound by reading every visible key and value
+// once from HBM. The visible tokens of all sequences are laid end to end in tiles
+// of 64, and that axis is cut into equal ranges, one CTA for each range and kv
+// head: every CTA reads the same number of bytes whatever the lengths are. CTAs of
+// one range and neighbouring heads run side by side, so the 256-byte rows of a
+// token's heads are fetched at about the same time.
+//
+// In a CTA one warp fills a ring of tiles with TMA (a box for each run of rows
+// within a page), four warps take 16 tokens of a tile each: scores by mma, a running
+// maximum and sum in 32 bits, probabilities rounded to the input type (half a step,
+// as the output is) for the second product, sums in 32 bits. Where a sequence ends
+// inside a range the four warps' parts are joined in the tile's memory and written;
+// a sequence cut by a range's border leaves parts in the scratch that
+// decode_join_kernel adds up in the ranges' order.
+#include <algorithm>
+#include <atomic>
+
+#include "kv_attention.cuh"
+
+namespace tcx {
+namespace {
+
+constexpr int kTile = 64;
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kRows = kDecodeRows;
+
+enum : uint32_t { kFirst = 1, kLast = 2, kMask = 4, kWhole = 8, kSecondSlot = 16 };
+
+// What the consumers need to know of a tile.
+struct TileInfo {
+  uint32_t flags, seq, q_first, queries;
+  int token, len, low, sinks;  // low: first token inside the first query's window
+};
+
+// What decode_join_kernel needs to know of a range.
+struct RangeInfo {
+  uint32_t seq;     // of its last piece
+  uint32_t starts;  // that sequence starts in this range
+  uint32_t goes_on; // and continues in the next one
+  uint32_t slot;
+};
+
+struct DecodeArgs {
+  AttnArgs a;
+  uint32_t ranges;
+  RangeInfo* info;  // [ranges]
+  float* part_o;    // [ranges][2][kv_heads][kRows][D], sums of 2^(z - m) v
+  float2* part_ml;  // the same rows' m and sum of 2^(z - m)
+};
+
+template <int D>
+struct Layout {
+  static constexpr int kHalf = kTile * 128;              // 64 values of each token: 128-byte rows, swizzled
+  static constexpr int kKeys = kHalf * (D / 64);
+  static constexpr int kQueryPitch = D * 2 + 16;          // 16 bytes more: rows in different banks
+  static constexpr int kQueries = kRows * kQueryPitch;
+  static constexpr int kStage = 2 * kKeys + (kQueries + 1023) / 1024 * 1024;
+  static constexpr int kStages = D == 128 ? 3 : 5;
+  static constexpr int kBytes = kStages * kStage + 1024;  // the first tile starts on a 1 KiB border
+};
+
+struct SeqInfo {
+  int len, low, sinks, sink_tiles, first_tile;  // tiles: [0, sink_tiles) and from first_tile on
+  uint32_t tiles, q_first, queries;
+};
+
+__device__ __forceinline__ SeqInfo seq_info(const AttnArgs& a, uint32_t s, int prefix) {
+  SeqInfo i;
+  i.q_first = a.q_offsets[s];
+  i.queries = a.q_offsets[s + 1] - i.q_first;
+  i.len = static_cast<int>(seq_length(a, s));
+  i.low = a.window ? static_cast<int>(max(int64_t{0}, i.len - static_cast<int64_t>(i.queries) - a.window + 1)) : 0;
+  i.sinks = static_cast<int>(max(int64_t{0}, a.sinks - prefix));
+  const int tiles = (i.len + kTile - 1) / kTile;
+  i.sink_tiles = i.low > 0 ? (min(i.sinks, i.len) + kTile - 1) / kTile : 0;
+  i.first_tile = max(i.low / kTile, i.sink_tiles);
+  // a sequence without tokens has one empty tile, so that its rows are written
+  i.tiles = i.queries == 0 ? 0 : max(i.sink_tiles + tiles - i.first_tile, 1);
+  return i;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_constant__ CUtensorMap map, DecodeArgs d) {
+  using L = Layout<D>;
+  extern __shared__ uint8_t raw[];
+  __shared__ TileInfo s_info[L::kStages];
+  __shared__ uint64_t s_full[L::kStages], s_empty[L::kStages];
+  __shared__ uint32_t s_scan[kThreads / 32], s_begin[2], s_gave_up;
+  __shared__ float2 s_ml[kWarps][kRows];
+  const AttnArgs& a = d.a;
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t head = blockIdx.x % a.kv_heads, range = blockIdx.x / a.kv_heads;
+  const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(smem_addr(&s_full[i]), 1);
+      mbar_init(smem_addr(&s_empty[i]), kWarps);
+    }
+    s_gave_up = 0;
+    mbar_init_fence();
+  }
+  // Rows of the query area that no query fills must hold finite values.
+  for (uint32_t i = threadIdx.x; i < L::kStages * (L::kQueries / 16); i += kThreads)
+    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + i / (L::kQueries / 16) * L::kStage +
+                                                                   2 * L::kKeys + i % (L::kQueries / 16) * 16),
+                 "r"(0)
+                 : "memory");
+  proxy_fence_smem();
+  const int prefix = static_cast<int>(prefix_length(a));
+  // Tiles of this thread's share of the sequences, and where this range begins.
+  const uint32_t share = (a.n_seq + kThreads - 1) / kThreads, s0 = min(threadIdx.x * share, a.n_seq),
+                 s1 = min(s0 + share, a.n_seq);
+  uint32_t mine = 0;
+  for (uint32_t s = s0; s < s1; ++s) mine += seq_info(a, s, prefix).tiles;
+  uint32_t inc = mine;
+  for (int x = 1; x < 32; x *= 2) {
+    const uint32_t up = __shfl_up_sync(~0u, inc, x);
+    if (lane >= x) inc += up;
+  }
+  if (lane == 31) s_scan[warp] = inc;
+  __syncthreads();
+  uint32_t total = 0, before = inc - mine;
+  for (uint32_t w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
+  }
+  const uint32_t ranges = min(d.ranges, total);
+  if (range >= ranges) {
+    if (head == 0 && threadIdx.x == 0) d.info[range] = RangeInfo{0, 0, 0, 0};
+    return;
+  }
+  const uint32_t t0 = static_cast<uint32_t>(static_cast<uint64_t>(range) * total / ranges);
+  const uint32_t t1 = static_cast<uint32_t>(static_cast<uint64_t>(range + 1) * total / ranges);
+  if (before <= t0 && t0 < before + mine) {
+    uint32_t s = s0, at = before;
+    for (;; ++s) {
+      const uint32_t n = seq_info(a, s, prefix).tiles;
+      if (t0 < at + n) break;
+      at += n;
+    }
+    s_begin[0] = s;
+    s_begin[1] = t0 - at;
+  }
+  __syncthreads();
+  const uint32_t count = t1 - t0;
+
+  if (warp == kWarps) {  // ---- the producer
+    const uint32_t boxes = kTile / a.box_rows, halves = D / 64;
+    uint32_t s = s_begin[0], t = s_begin[1];
+    SeqInfo q = seq_info(a, s, prefix);
+    bool fresh = true;  // the next tile is the first of its piece
+    uint32_t pieces = 0;
+    for (uint32_t i = 0; i < count; ++i) {
+      const uint32_t stage = i % L::kStages;
+      const int tile = t < static_cast<uint32_t>(q.sink_tiles) ? t : q.first_tile + (t - q.sink_tiles);
+      const int token = tile * kTile, end = min(token + kTile, q.len);
+      TileInfo info{fresh ? kFirst : 0u, s, q.q_first, q.queries, token, q.len, q.low, q.sinks};
+      const bool seq_done = t + 1 == q.tiles;
+      if (seq_done || i + 1 == count) info.flags |= kLast;
+      const bool starts = s != s_begin[0] || s_begin[1] == 0;
+      if (seq_done && starts) info.flags |= kWhole;
+      if (pieces > 0) info.flags |= kSecondSlot;
+      const int last_low = a.window ? q.low + static_cast<int>(q.queries) - 1 : 0;  // at least the last query's
+      if (token + kTile - 1 > q.len - static_cast<int>(q.queries) ||
+          (token < last_low && token + kTile > q.sinks))
+        info.flags |= kMask;
+      mbar_wait(smem_addr(&s_empty[stage]), (i / L::kStages & 1) ^ 1, &s_gave_up, a.status);
+      const uint32_t full = smem_addr(&s_full[stage]), at = base + stage * L::kStage;
+      // lane: one box of the keys or values and one half of the head
+      const uint32_t box = lane % boxes, half = lane / boxes % halves, plane = lane / boxes / halves;
+      const int from = token + static_cast<int>(box * a.box_rows), to = from + static_cast<int>(a.box_rows);
+      const bool wanted = lane < 2 * halves * boxes && from < end && (to > q.low || from < q.sinks);
+      const uint32_t rows = fresh ? min(q.queries * a.group, static_cast<uint32_t>(kRows)) : 0;
+      const uint32_t bytes = __popc(__ballot_sync(~0u, wanted)) * a.box_rows * 128 + rows * D * 2;
+      uint64_t row = 0;
+      if (wanted)
+        row = checked_slot(a, a.page_table + a.page_offsets[s], from / a.page_tokens) * a.page_tokens +
+              from % a.page_tokens + (plane ? a.v_row0 : a.k_row0);
+      if (lane == 0) {
+        s_info[stage] = info;
+        if (bytes) mbar_arrive_expect(full, bytes); else mbar_arrive(full);
+      }
+      __syncwarp();
+      if (wanted)
+        tma_load_3d(at + plane * L::kKeys + half * L::kHalf + box * a.box_rows * 128, &map, half * 64, head,
+                    static_cast<int>(row), full);
+      if (lane < rows)
+        bulk_load(at + 2 * L::kKeys + lane * L::kQueryPitch,
+                  a.q + (q.q_first + lane / a.group) * a.q_token_stride +
+                      (head * a.group + lane % a.group) * a.q_head_stride,
+                  D * 2, full);
+      fresh = false;
+      ++t;
+      if (i + 1 == count && head == 0 && lane == 0)
+        d.info[range] = RangeInfo{s, starts, !seq_done, pieces > 0};
+      if (seq_done && i + 1 < count) {
+        do q = seq_info(a, ++s, prefix); while (q.tiles == 0);
+        t = 0;
+        fresh = true;
+        ++pieces;
+      }
+    }
+    // No copy may be in flight when the CTA ends.
+    for (uint32_t i = count > L::kStages ? count - L::kStages : 0; i < count; ++i)
+      mbar_wait(smem_addr(&s_full[i % L::kStages]), i / L::kStages & 1, &s_gave_up, a.status);
+    return;
+  }
+
+  // ---- the consumers: rows lane / 4 and lane / 4 + 8, tokens 16 warp .. 16 warp + 15 of each tile
+  uint32_t qf[D / 16][4];
+  float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  for (uint32_t i = 0; i < count; ++i) {
+    const uint32_t stage = i % L::kStages, at = base + stage * L::kStage;
+    mbar_wait(smem_addr(&s_full[stage]), i / L::kStages & 1, &s_gave_up, a.status);
+    const TileInfo info = s_info[stage];
+    if (info.flags & kFirst) {
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+        ldmatrix4(qf[k], at + 2 * L::kKeys + lane % 16 * L::kQueryPitch + k * 32 + lane / 16 * 16);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+      m[0] = m[1] = -INFINITY;
+      l[0] = l[1] = 0.f;
+    }
+    // scores: tokens 0-7 (z[0]) and 8-15 (z[1]) of this warp's 16
+    float z[2][4] = {};
+    {
+      const uint32_t token = warp * 16 + lane / 16 * 8 + lane % 8, chunk = lane / 8 % 2;
+      const uint32_t row = at + token * 128;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t b[4];
+        ldmatrix4(b, row + k / 4 * L::kHalf + (((k % 4 * 2 + chunk) ^ (token & 7)) << 4));
+        mma16816<T>(z[0], qf[k], b[0], b[1]);
+        mma16816<T>(z[1], qf[k], b[2], b[3]);
+      }
+    }
+    if (info.flags & kMask) {
+      const int first = info.token + static_cast<int>(warp) * 16;
+      // values that no row sees are cleared: 0 x NaN is not 0
+      const int hidden = first + static_cast<int>(lane % 16);
+      const bool clear = hidden >= info.len || (hidden < info.low && hidden >= info.sinks);
+      if (__any_sync(~0u, clear)) {
+        if (clear) {
+          const uint32_t row = at + L::kKeys + lane / 16 * (L::kHalf * (D / 128)) + (warp * 16 + lane % 16) * 128;
+          if (lane < 16 || D == 128)
+            for (int c = 0; c < 8; ++c)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(row + c * 16), "r"(0) : "memory");
+        }
+        proxy_fence_smem();
+        __syncwarp();
+      }
+      const uint32_t r = lane / 4;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int j = first + n * 8 + static_cast<int>(lane % 4) * 2 + e % 2;
+          const int i_q = static_cast<int>((r + e / 2 * 8) / a.group);
+          const int pos = info.len - static_cast<int>(info.queries) + i_q;
+          const bool see = j <= pos && (a.window == 0 || j > pos - a.window || j < info.sinks);
+          if (!see) z[n][e] = -INFINITY;
+        }
+    }
+    uint32_t p[4];
+    float scale[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float top = fmaxf(fmaxf(z[0][2 * r], z[0][2 * r + 1]), fmaxf(z[1][2 * r], z[1][2 * r + 1]));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(~0u, top, 2)) * a.scale_log2;
+      top = fmaxf(top, m[r]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      scale[r] = exp2_approx(m[r] - ref);
+      m[r] = top;
+      float sum = 0.f;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float& x = z[n][2 * r + e];
+          x = exp2_approx(fmaf(x, a.scale_log2, -ref));
+          sum += x;
+        }
+      l[r] = l[r] * scale[r] + sum;  // of this lane's columns
+    }
+    p[0] = pack2<T>(z[0][0], z[0][1]);
+    p[1] = pack2<T>(z[0][2], z[0][3]);
+    p[2] = pack2<T>(z[1][0], z[1][1]);
+    p[3] = pack2<T>(z[1][2], z[1][3]);
+    if (__any_sync(~0u, scale[0] != 1.f || scale[1] != 1.f)) {
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[n][e] *= scale[e / 2];
+    }
+    {
+      const uint32_t token = warp * 16 + lane % 16;
+      const uint32_t row = at + L::kKeys + token * 128;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        uint32_t b[4];
+        ldmatrix4_t(b, row + n / 4 * L::kHalf + (((n % 4 * 2 + lane / 16) ^ (token & 7)) << 4));
+        mma16816<T>(o[2 * n], p, b[0], b[1]);
+        mma16816<T>(o[2 * n + 1], p, b[2], b[3]);
+      }
+    }
+    if (info.flags & kLast) {
+      // The four warps' parts are joined in this tile's memory, which all have read.
+      const uint32_t rows = min(info.queries * a.group, static_cast<uint32_t>(kRows));
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        l[r] += __shfl_xor_sync(~0u, l[r], 1);
+        l[r] += __shfl_xor_sync(~0u, l[r], 2);
+        if (lane % 4 == 0) s_ml[warp][lane / 4 + 8 * r] = make_float2(m[r], l[r]);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      float* join = reinterpret_cast<float*>(raw + (at - smem_addr(raw)));  // [warp][row][D]
+#pragma unroll
+      for (int r = 0; r < 2; ++r)
+        if (lane / 4 + 8 * r < rows)
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(join + (warp * kRows + lane / 4 + 8 * r) * D + n * 8 + lane % 4 * 2) =
+                make_float2(o[n][2 * r], o[n][2 * r + 1]);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      constexpr uint32_t kLanes = D / 4;  // threads of a row: 4 values each
+      for (uint32_t r = threadIdx.x / kLanes; r < rows; r += 128 / kLanes) {
+        const uint32_t e = threadIdx.x % kLanes * 4;
+        float top = -INFINITY, sum = 0.f;
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][r].x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = exp2_approx(s_ml[w][r].x - ref);
+          sum += f * s_ml[w][r].y;
+          const float4 x = *reinterpret_cast<const float4*>(join + (w * kRows + r) * D + e);
+          v.x += f * x.x;
+          v.y += f * x.y;
+          v.z += f * x.z;
+          v.w += f * x.w;
+        }
+        if (s_gave_up) continue;
+        if (info.flags & kWhole) {
+          const uint32_t t = info.q_first + r / a.group, h = head * a.group + r % a.group;
+          const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          *reinterpret_cast<uint2*>(a.out + t * a.out_token_stride + h * a.out_head_stride + e * 2) =
+              make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
+          if (e == 0) a.lse[static_cast<uint64_t>(t) * a.kv_heads * a.group + h] = kLn2 * (top + log2f(sum));
+        } else {
+          const uint64_t row = (static_cast<uint64_t>(range * 2 + (info.flags & kSecondSlot ? 1 : 0)) * a.kv_heads + head) *
+                                   kRows + r;
+          *reinterpret_cast<float4*>(d.part_o + row * D + e) = v;
+          if (e == 0) d.part_ml[row] = make_float2(top, sum);
+        }
+      }
+      proxy_fence_smem();  // these accesses come before the copies of the next tile here
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_addr(&s_empty[stage]));
+  }
+}
+
+// One CTA per row of the sequence that starts in a range and continues past it:
+// the parts of its ranges, in their order, two values of the row for each lane.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) decode_join_kernel(DecodeArgs d) {
+  constexpr int E = D / 32;
+  const AttnArgs& a = d.a;
+  const uint32_t range = blockIdx.x, head = blockIdx.y, r = blockIdx.z, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const RangeInfo own = d.info[range];
+  if (!own.goes_on || !own.starts) return;
+  const uint32_t q_first = a.q_offsets[own.seq], rows = (a.q_offsets[own.seq + 1] - q_first) * a.group;
+  if (r >= rows) return;
+  uint32_t end = range + 1;
+  for (;; ++end) {  // the last range of this sequence: the next one starts with another, or ends here
+    const RangeInfo next = d.info[end];
+    if (next.seq != own.seq || !next.goes_on) break;
+  }
+  auto row_of = [&](uint32_t k) {
+    return (static_cast<uint64_t>(k * 2 + (k == range ? own.slot : 0)) * a.kv_heads + head) * kRows + r;
+  };
+  float top = -INFINITY, sum = 0.f, v[E] = {};
+  for (uint32_t k = range + lane; k <= end; k += 32) top = fmaxf(top, d.part_ml[row_of(k)].x);
+  for (int x = 16; x; x /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+  const float ref = top == -INFINITY ? 0.f : top;
+  for (uint32_t k = range + warp; k <= end; k += 4) {
+    const uint64_t row = row_of(k);
+    const float2 ml = d.part_ml[row];
+    const float f = exp2_approx(ml.x - ref);
+    sum += f * ml.y;
+    for (int e = 0; e < E; ++e) v[e] += f * d.part_o[row * D + e * 32 + lane];
+  }
+  __shared__ float s_v[4][D], s_sum[4];
+  for (int e = 0; e < E; ++e) s_v[warp][e * 32 + lane] = v[e];
+  if (lane == 0) s_sum[warp] = sum;
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+  const float x = s_v[0][threadIdx.x] + s_v[1][threadIdx.x] + s_v[2][threadIdx.x] + s_v[3][threadIdx.x];
+  const uint32_t t = q_first + r / a.group, h = head * a.group + r % a.group;
+  reinterpret_cast<T*>(a.out + t * a.out_token_stride + h * a.out_head_stride)[threadIdx.x] =
+      static_cast<T>(sum == 0.f ? 0.f : x / sum);
+  if (threadIdx.x == 0) a.lse[static_cast<uint64_t>(t) * a.kv_heads * a.group + h] = kLn2 * (top + log2f(sum));
+}
+
+// Two CTAs fit an SM. A range holds one tile at least.
+uint32_t decode_ranges(const tcx_kv_attention_args& x) {
+  const uint64_t tiles = x.total_pages * x.page_tokens / kTile + x.n_seq;
+  return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(tiles, 2ull * sm_count() / x.kv_heads)));
+}
+
+uint64_t align256(uint64_t n) { return (n + 255) / 256 * 256; }
+
+template <typename T, int D>
+tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint32_t rows, cudaStream_t stream) {
+  using L = Layout<D>;
+  TCX_CUDA_TRY(cudaFuncSetAttribute(decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+  decode_kernel<T, D><<<d.ranges * d.a.kv_heads, kThreads, L::kBytes, stream>>>(map, d);
+  note_launches(1);
+  TCX_CUDA_TRY(cudaGetLastError());
+  if (d.ranges > 1) {
+    decode_join_kernel<T, D><<<dim3(d.ranges - 1, d.a.kv_heads, rows), 128, 0, stream>>>(d);
+    note_launches(1);
+    TCX_CUDA_TRY(cudaGetLastError());
+  }
+  return TCX_OK;
+}
+
+}  // namespace
+
+bool decode_fits(const tcx_kv_attention_args& x) {
+  return x.max_q * (x.q_heads / x.kv_heads) <= kDecodeRows && x.d_prefix_table == nullptr;
+}
+
+uint64_t decode_scratch_bytes(const tcx_kv_attention_args& x) {
+  const uint64_t parts = decode_ranges(x) * 2ull * x.kv_heads * kRows;
+  return align256(decode_ranges(x) * sizeof(RangeInfo)) + align256(parts * sizeof(float2)) + parts * x.head_dim * 4;
+}
+
+tcx_status launch_decode(const tcx_kv_attention_args& x, const AttnArgs& a, const CUtensorMap& map, void* scratch,
+                         cudaStream_t stream) {
+  DecodeArgs d{};
+  d.a = a;
+  d.ranges = decode_ranges(x);
+  const uint64_t parts = d.ranges * 2ull * x.kv_heads * kRows;
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  d.info = reinterpret_cast<RangeInfo*>(at);
+  d.part_ml = reinterpret_cast<float2*>(at += align256(d.ranges * sizeof(RangeInfo)));
+  d.part_o = reinterpret_cast<float*>(at + align256(parts * sizeof(float2)));
+  const uint32_t rows = static_cast<uint32_t>(x.max_q) * a.group;
+  if (x.dtype == TCX_KV_BF16)
+    return x.head_dim == 128 ? launch<__nv_bfloat16, 128>(d, map, rows, stream)
+                             : launch<__nv_bfloat16, 64>(d, map, rows, stream);
+  return x.head_dim == 128 ? launch<__half, 128>(d, map, rows, stream) : launch<__half, 64>(d, map, rows, stream);
+}
+
+}  // namespace tcx
