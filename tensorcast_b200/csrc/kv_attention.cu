@@ -22,49 +22,6 @@ __device__ __forceinline__ float to_float(T v) {
   return static_cast<float>(v);
 }
 
-// One warp per row; a lane holds D / 32 dimensions. The running maximum and sum
-// of the softmax are kept in 32 bits over one pass of the visible tokens.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attention_row_kernel(AttnArgs a) {
-  constexpr int E = D / 32;
-  const uint32_t lane = threadIdx.x % 32;
-  const uint64_t row = static_cast<uint64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
-  const uint32_t q_heads = a.kv_heads * a.group;
-  if (row >= static_cast<uint64_t>(a.q_tokens) * q_heads) return;
-  const uint32_t t = static_cast<uint32_t>(row / q_heads), h = static_cast<uint32_t>(row % q_heads);
-  const uint32_t kvh = h / a.group, s = seq_of(a, t);
-  const int64_t len = seq_length(a, s), prefix = prefix_length(a);
-  const int64_t nq = a.q_offsets[s + 1] - a.q_offsets[s];
-  const int64_t pos = prefix + len - nq + (t - a.q_offsets[s]);
-  float q[E], o[E] = {}, m = -INFINITY, l = 0.f;
-  const T* qp = reinterpret_cast<const T*>(a.q + t * a.q_token_stride + h * a.q_head_stride);
-  for (int e = 0; e < E; ++e) q[e] = to_float(qp[lane * E + e]);
-  const int64_t low = a.window ? max(int64_t{0}, pos - a.window + 1) : 0;
-  for (int64_t j = 0; j <= pos; ++j) {
-    if (j >= a.sinks && j < low) j = low;
-    const uint32_t* table = j < prefix ? a.prefix_table : a.page_table + a.page_offsets[s];
-    const int64_t k = j < prefix ? j : j - prefix;
-    const uint64_t off = checked_slot(a, table, k / a.page_tokens) * a.page_bytes +
-                         (k % a.page_tokens) * a.token_bytes + kvh * a.row_bytes;
-    const uint64_t plane = a.pool_pages * a.page_bytes;
-    const T* kp = reinterpret_cast<const T*>(a.pool + a.k_plane * plane + off);
-    const T* vp = reinterpret_cast<const T*>(a.pool + a.v_plane * plane + off);
-    float z = 0.f;
-    for (int e = 0; e < E; ++e) z += q[e] * to_float(kp[lane * E + e]);
-    for (int x = 16; x; x /= 2) z += __shfl_xor_sync(~0u, z, x);
-    z *= a.scale_log2;
-    const float top = fmaxf(m, z), old = m == -INFINITY ? 0.f : exp2f(m - top);
-    const float p = exp2f(z - top);
-    l = l * old + p;
-    for (int e = 0; e < E; ++e) o[e] = o[e] * old + p * to_float(vp[lane * E + e]);
-    m = top;
-  }
-  T* op = reinterpret_cast<T*>(a.out + t * a.out_token_stride + h * a.out_head_stride);
-  const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // a NaN sum stays one
-  for (int e = 0; e < E; ++e) op[lane * E + e] = static_cast<T>(o[e] * inv);
-  if (lane == 0) a.lse[static_cast<uint64_t>(t) * q_heads + h] = kLn2 * (m + log2f(l));
-}
-
 // One warp per token and kv head: the token's weights of all rows, added in the
 // rows' order, so that the sum does not depend on the run.
 template <typename T, int D>
@@ -98,19 +55,12 @@ __global__ void __launch_bounds__(128) attention_weights_kernel(AttnArgs a) {
 }
 
 template <typename T, int D>
-tcx_status launch(const AttnArgs& a, bool rows_done, uint64_t max_tokens, cudaStream_t stream) {
-  if (!rows_done) {
-    const uint64_t rows = static_cast<uint64_t>(a.q_tokens) * a.kv_heads * a.group;
-    attention_row_kernel<T, D><<<static_cast<unsigned>((rows + 3) / 4), 128, 0, stream>>>(a);
-    note_launches(1);
-    TCX_CUDA_TRY(cudaGetLastError());
-  }
-  if (a.weights != nullptr && max_tokens > 0) {
-    const dim3 grid(static_cast<unsigned>((max_tokens + 3) / 4), a.kv_heads, a.n_seq);
-    attention_weights_kernel<T, D><<<grid, 128, 0, stream>>>(a);
-    note_launches(1);
-    TCX_CUDA_TRY(cudaGetLastError());
-  }
+tcx_status launch_weights(const AttnArgs& a, uint64_t max_tokens, cudaStream_t stream) {
+  if (max_tokens == 0) return TCX_OK;
+  const dim3 grid(static_cast<unsigned>((max_tokens + 3) / 4), a.kv_heads, a.n_seq);
+  attention_weights_kernel<T, D><<<grid, 128, 0, stream>>>(a);
+  note_launches(1);
+  TCX_CUDA_TRY(cudaGetLastError());
   return TCX_OK;
 }
 
@@ -161,6 +111,11 @@ tcx_status check(const tcx_kv_attention_args& a) {
       return set_error(TCX_INVALID_ARGUMENT, "weights are not accumulated with a shared prefix");
   }
   return TCX_OK;
+}
+
+// The rows' parts over a shared prefix.
+uint64_t prior_bytes(const tcx_kv_attention_args& x) {
+  return align256(x.q_tokens * x.q_heads * (x.head_dim + 1) * sizeof(float));
 }
 
 AttnArgs device_args(const tcx_kv_attention_args& x) {
@@ -235,7 +190,10 @@ using namespace tcx;
 
 extern "C" uint64_t tcx_kv_attention_scratch_bytes(const tcx_kv_attention_args* args) {
   if (args == nullptr || args->n_seq == 0 || args->q_tokens == 0 || check_sizes(*args) != TCX_OK) return 0;
-  return decode_fits(*args) ? decode_scratch_bytes(*args) : 0;
+  uint64_t own = decode_fits(*args) ? decode_scratch_bytes(*args) : tile_scratch_bytes(*args, false);
+  if (args->d_prefix_table != nullptr)  // the two run one after the other
+    own = std::max(own, tile_scratch_bytes(*args, true)) + prior_bytes(*args);
+  return own;
 }
 
 extern "C" tcx_status tcx_kv_attention(const tcx_kv_attention_args* args, void* d_scratch, uint64_t scratch_bytes,
@@ -244,21 +202,32 @@ extern "C" tcx_status tcx_kv_attention(const tcx_kv_attention_args* args, void* 
   if (args->n_seq == 0 || args->q_tokens == 0) return TCX_OK;
   if (const tcx_status st = check(*args); st != TCX_OK) return st;
   const uint64_t need = tcx_kv_attention_scratch_bytes(args);
-  if (scratch_bytes < need || (need != 0 && d_scratch == nullptr))
-    return set_errorf(TCX_INVALID_ARGUMENT, "scratch too small: %llu bytes, %llu needed",
-                      static_cast<unsigned long long>(scratch_bytes), static_cast<unsigned long long>(need));
-  const AttnArgs a = device_args(*args);
-  const bool rows_done = decode_fits(*args);
-  if (rows_done) {
-    CUtensorMap map;
-    if (const tcx_status st = encode_pool_map(*args, a.box_rows, &map); st != TCX_OK) return st;
-    if (const tcx_status st = launch_decode(*args, a, map, d_scratch, static_cast<cudaStream_t>(stream)); st != TCX_OK)
-      return st;
-  }
-  const uint64_t max_tokens = args->max_pages * args->page_tokens;
+  if (scratch_bytes < need || d_scratch == nullptr || (reinterpret_cast<uintptr_t>(d_scratch) & 255u))
+    return set_errorf(TCX_INVALID_ARGUMENT, "scratch of %llu bytes, 256-byte aligned, needed (got %llu)",
+                      static_cast<unsigned long long>(need), static_cast<unsigned long long>(scratch_bytes));
+  AttnArgs a = device_args(*args);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  CUtensorMap map;
+  if (const tcx_status st = encode_pool_map(*args, a.box_rows, &map); st != TCX_OK) return st;
+  uint8_t* scratch = static_cast<uint8_t*>(d_scratch);
+  if (args->d_prefix_table != nullptr) {
+    a.part_o = reinterpret_cast<float*>(scratch);
+    a.part_lse = a.part_o + args->q_tokens * args->q_heads * args->head_dim;
+    scratch += prior_bytes(*args);
+    if (const tcx_status st = launch_tile(*args, a, map, true, scratch, s); st != TCX_OK) return st;
+    a.prior_o = a.part_o;
+    a.prior_lse = a.part_lse;
+    a.part_o = a.part_lse = nullptr;
+  }
+  if (const tcx_status st = decode_fits(*args) ? launch_decode(*args, a, map, scratch, s)
+                                               : launch_tile(*args, a, map, false, scratch, s);
+      st != TCX_OK)
+    return st;
+  if (args->d_weights == nullptr) return TCX_OK;
+  const uint64_t max_tokens = args->max_pages * args->page_tokens;
   if (args->dtype == TCX_KV_BF16)
-    return args->head_dim == 128 ? launch<__nv_bfloat16, 128>(a, rows_done, max_tokens, s)
-                                 : launch<__nv_bfloat16, 64>(a, rows_done, max_tokens, s);
-  return args->head_dim == 128 ? launch<__half, 128>(a, rows_done, max_tokens, s) : launch<__half, 64>(a, rows_done, max_tokens, s);
+    return args->head_dim == 128 ? launch_weights<__nv_bfloat16, 128>(a, max_tokens, s)
+                                 : launch_weights<__nv_bfloat16, 64>(a, max_tokens, s);
+  return args->head_dim == 128 ? launch_weights<__half, 128>(a, max_tokens, s)
+                               : launch_weights<__half, 64>(a, max_tokens, s);
 }

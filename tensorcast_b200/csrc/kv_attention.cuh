@@ -32,6 +32,10 @@ struct AttnArgs {
   float* weights;
   uint64_t weights_head_stride;
   uint32_t* status;
+  // Where there is a shared prefix: the rows' parts over it (o normalised, lse in
+  // powers of two, [q token][q head]) are written to `part` and then read as `prior`.
+  float *part_o, *part_lse;
+  const float *prior_o, *prior_lse;
   uint32_t box_rows;  // token rows of one TMA box: divides page_tokens and 64
   uint64_t k_row0, v_row0;  // first token row of the planes in the pool's map
 };
@@ -75,6 +79,78 @@ __device__ __forceinline__ uint64_t checked_slot(const AttnArgs& a, const uint32
   return 0;
 }
 
+// A finished row: o = sum of 2^(z - m) v and l = sum of 2^(z - m) become
+//   o * own + prior_o * prior,  lse (in powers of two)
+struct Finish {
+  float own, prior, lse;
+};
+
+__device__ __forceinline__ Finish finish_row(const AttnArgs& a, uint64_t row, float m, float l) {
+  Finish f;
+  f.own = l == 0.f ? 0.f : 1.f / l;
+  f.prior = 0.f;
+  f.lse = m + log2f(l);  // l 0: m is -inf, and so is this
+  if (a.prior_lse != nullptr) {
+    const float p = a.prior_lse[row];
+    const float top = fmaxf(f.lse, p), ref = top == -INFINITY ? 0.f : top;
+    const float w = exp2f(f.lse - ref), wp = exp2f(p - ref), sum = w + wp;
+    f.own = w == 0.f ? 0.f : f.own * w / sum;
+    f.prior = wp == 0.f ? 0.f : wp / sum;
+    f.lse = top + log2f(sum);
+  }
+  return f;
+}
+
+// N values of a finished row from column e on, N a multiple of 4.
+template <typename T, int D, int N>
+__device__ __forceinline__ void store_row(const AttnArgs& a, uint32_t t, uint32_t h, uint32_t e, const Finish& f,
+                                          const float (&v)[N]) {
+  const uint64_t row = static_cast<uint64_t>(t) * a.kv_heads * a.group + h;
+  float x[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = v[i] * f.own;
+  if (f.own == 0.f) {  // nothing seen here: 0, whatever the sums hold
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = 0.f;
+  }
+  if (f.prior != 0.f) {
+    const float4* p = reinterpret_cast<const float4*>(a.prior_o + row * D + e);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const float4 y = p[i];
+      x[4 * i] += f.prior * y.x;
+      x[4 * i + 1] += f.prior * y.y;
+      x[4 * i + 2] += f.prior * y.z;
+      x[4 * i + 3] += f.prior * y.w;
+    }
+  }
+  if (a.part_o != nullptr) {
+    float4* p = reinterpret_cast<float4*>(a.part_o + row * D + e);
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    return;
+  }
+  uint8_t* out = a.out + t * a.out_token_stride + h * a.out_head_stride + e * 2;
+  if constexpr (N % 8 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 8; ++i)
+      reinterpret_cast<uint4*>(out)[i] = make_uint4(pack2<T>(x[8 * i], x[8 * i + 1]), pack2<T>(x[8 * i + 2], x[8 * i + 3]),
+                                                    pack2<T>(x[8 * i + 4], x[8 * i + 5]),
+                                                    pack2<T>(x[8 * i + 6], x[8 * i + 7]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i)
+      reinterpret_cast<uint2*>(out)[i] = make_uint2(pack2<T>(x[4 * i], x[4 * i + 1]), pack2<T>(x[4 * i + 2], x[4 * i + 3]));
+  }
+}
+
+__device__ __forceinline__ void store_lse(const AttnArgs& a, uint32_t t, uint32_t h, const Finish& f) {
+  const uint64_t row = static_cast<uint64_t>(t) * a.kv_heads * a.group + h;
+  if (a.part_o != nullptr) a.part_lse[row] = f.lse; else a.lse[row] = kLn2 * f.lse;
+}
+
+inline uint64_t align256(uint64_t n) { return (n + 255) / 256 * 256; }
+
 // The pool as a tensor of [planes x slots x page tokens][kv heads][head_dim] 16-bit
 // values, read in boxes of `box_rows` token rows of 64 values of one head.
 tcx_status encode_pool_map(const tcx_kv_attention_args& x, uint32_t box_rows, CUtensorMap* map);
@@ -85,5 +161,11 @@ bool decode_fits(const tcx_kv_attention_args& x);
 uint64_t decode_scratch_bytes(const tcx_kv_attention_args& x);
 tcx_status launch_decode(const tcx_kv_attention_args& x, const AttnArgs& a, const CUtensorMap& map, void* scratch,
                          cudaStream_t stream);
+
+// Many rows: prompts, and the shared prefix of a batch (kv_tile.cu). With
+// `prefix` the rows of all sequences attend over the prefix.
+uint64_t tile_scratch_bytes(const tcx_kv_attention_args& x, bool prefix);
+tcx_status launch_tile(const tcx_kv_attention_args& x, const AttnArgs& a, const CUtensorMap& map, bool prefix,
+                       void* scratch, cudaStream_t stream);
 
 }  // namespace tcx

@@ -168,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       if (token + kTile - 1 > q.len - static_cast<int>(q.queries) ||
           (token < last_low && token + kTile > q.sinks))
         info.flags |= kMask;
-      mbar_wait(smem_addr(&s_empty[stage]), (i / L::kStages & 1) ^ 1, &s_gave_up, a.status);
+      mbar_wait_warp(smem_addr(&s_empty[stage]), (i / L::kStages & 1) ^ 1, &s_gave_up, a.status);
       const uint32_t full = smem_addr(&s_full[stage]), at = base + stage * L::kStage;
       // lane: one box of the keys or values and one half of the head
       const uint32_t box = lane % boxes, half = lane / boxes % halves, plane = lane / boxes / halves;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     }
     // No copy may be in flight when the CTA ends.
     for (uint32_t i = count > L::kStages ? count - L::kStages : 0; i < count; ++i)
-      mbar_wait(smem_addr(&s_full[i % L::kStages]), i / L::kStages & 1, &s_gave_up, a.status);
+      mbar_wait_warp(smem_addr(&s_full[i % L::kStages]), i / L::kStages & 1, &s_gave_up, a.status);
     return;
   }
 
@@ -215,7 +215,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   for (uint32_t i = 0; i < count; ++i) {
     const uint32_t stage = i % L::kStages, at = base + stage * L::kStage;
-    mbar_wait(smem_addr(&s_full[stage]), i / L::kStages & 1, &s_gave_up, a.status);
+    mbar_wait_warp(smem_addr(&s_full[stage]), i / L::kStages & 1, &s_gave_up, a.status);
     const TileInfo info = s_info[stage];
     if (info.flags & kFirst) {
 #pragma unroll
@@ -349,10 +349,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
         if (s_gave_up) continue;
         if (info.flags & kWhole) {
           const uint32_t t = info.q_first + r / a.group, h = head * a.group + r % a.group;
-          const float inv = sum == 0.f ? 0.f : 1.f / sum;
-          *reinterpret_cast<uint2*>(a.out + t * a.out_token_stride + h * a.out_head_stride + e * 2) =
-              make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
-          if (e == 0) a.lse[static_cast<uint64_t>(t) * a.kv_heads * a.group + h] = kLn2 * (top + log2f(sum));
+          const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
+          store_row<T, D, 4>(a, t, h, e, f, {v.x, v.y, v.z, v.w});
+          if (e == 0) store_lse(a, t, h, f);
         } else {
           const uint64_t row = (static_cast<uint64_t>(range * 2 + (info.flags & kSecondSlot ? 1 : 0)) * a.kv_heads + head) *
                                    kRows + r;
@@ -401,13 +400,15 @@ __global__ void __launch_bounds__(128) decode_join_kernel(DecodeArgs d) {
   for (int e = 0; e < E; ++e) s_v[warp][e * 32 + lane] = v[e];
   if (lane == 0) s_sum[warp] = sum;
   __syncthreads();
-  if (threadIdx.x >= D) return;
+  const uint32_t e = threadIdx.x * 4;
+  if (e >= D) return;
   sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-  const float x = s_v[0][threadIdx.x] + s_v[1][threadIdx.x] + s_v[2][threadIdx.x] + s_v[3][threadIdx.x];
+  float x[4];
+  for (int i = 0; i < 4; ++i) x[i] = s_v[0][e + i] + s_v[1][e + i] + s_v[2][e + i] + s_v[3][e + i];
   const uint32_t t = q_first + r / a.group, h = head * a.group + r % a.group;
-  reinterpret_cast<T*>(a.out + t * a.out_token_stride + h * a.out_head_stride)[threadIdx.x] =
-      static_cast<T>(sum == 0.f ? 0.f : x / sum);
-  if (threadIdx.x == 0) a.lse[static_cast<uint64_t>(t) * a.kv_heads * a.group + h] = kLn2 * (top + log2f(sum));
+  const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
+  store_row<T, D, 4>(a, t, h, e, f, x);
+  if (e == 0) store_lse(a, t, h, f);
 }
 
 // Two CTAs fit an SM. A range holds one tile at least.
@@ -415,8 +416,6 @@ uint32_t decode_ranges(const tcx_kv_attention_args& x) {
   const uint64_t tiles = x.total_pages * x.page_tokens / kTile + x.n_seq;
   return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(tiles, 2ull * sm_count() / x.kv_heads)));
 }
-
-uint64_t align256(uint64_t n) { return (n + 255) / 256 * 256; }
 
 template <typename T, int D>
 tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint32_t rows, cudaStream_t stream) {
@@ -436,7 +435,7 @@ tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint32_t rows, cu
 }  // namespace
 
 bool decode_fits(const tcx_kv_attention_args& x) {
-  return x.max_q * (x.q_heads / x.kv_heads) <= kDecodeRows && x.d_prefix_table == nullptr;
+  return x.max_q * (x.q_heads / x.kv_heads) <= kDecodeRows;
 }
 
 uint64_t decode_scratch_bytes(const tcx_kv_attention_args& x) {

@@ -1,0 +1,650 @@
+// Attention of many query rows over paged keys and values: prompts, the last chunk
+// of one, and the shared prefix of a batch, whose sequences' rows all read the same
+// tokens.
+//
+// A kv head's rows are its query tokens x its group of q heads, in tiles of 256. A
+// CTA takes a tile of rows through tiles of 128 tokens: two products of 128 x 128
+// scores on the tensor cores (one for each half of the rows, so that one half's
+// softmax runs beside the other half's products), a softmax with a running maximum
+// and sum in 32 bits, one thread for each row, and two products with the values.
+// Scores, probabilities (rounded to the input type in place of the scores, half a
+// step, as the output is) and the output's sums (32 bits) stay in tensor memory; a
+// row's sums are scaled to a new maximum only where it has grown by more than 2^8,
+// which the 32-bit sums carry exactly as well.
+//
+// Roles: warps 0-3 and 4-7 the halves' softmax, warp 8 issues the products, warp 9
+// loads keys and values with TMA into a ring (a box for each run of rows in a page).
+//
+// Work: the visible (row tile, kv head, token tile) units laid end to end and cut
+// into equal ranges, one CTA on every SM, whatever the prompts' lengths and masks
+// are; row tiles cut by a border leave parts that tile_join_kernel adds up in the
+// ranges' order. tile_plan_kernel lays the units out from the device's lengths.
+#include <algorithm>
+
+#include "kv_attention.cuh"
+
+namespace tcx {
+namespace {
+
+constexpr int kTokens = 128;
+constexpr int kHalfRows = 128;
+constexpr int kRows = 2 * kHalfRows;
+constexpr int kThreads = 384;
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanCache = 2048;
+
+// A tile of rows: row r is query token q_first + (row0 + r) / group.
+struct Item {
+  uint32_t q_first, row0, rows;
+  int pos0;                      // position of query token q_first, from the first token of `table`
+  uint32_t tiles;                // token tiles: [0, sink_tiles) and from first_tile on
+  int sink_tiles, first_tile;
+  int limit, low, sinks;         // tokens seen lie below limit, and below sinks or from low on
+  uint64_t table;                // first entry in the page table
+};
+
+struct RangeBegin {
+  uint32_t item, head, tile;
+};
+
+struct RangeEnd {
+  uint32_t item, head;  // of the last piece
+  uint32_t starts, goes_on, slot;
+};
+
+struct TileArgs {
+  AttnArgs a;
+  uint32_t prefix;  // rows of all sequences over the shared prefix
+  uint32_t max_q, max_ranges;
+  uint32_t* item_first;  // [n_seq + 1]
+  Item* items;
+  uint64_t* unit_first;  // [items + 1]
+  RangeBegin* begin;     // [max_ranges + 1]
+  RangeEnd* end;         // [max_ranges]
+  uint32_t* counts;      // items, ranges
+  float* part_o;         // [max_ranges][2][kRows][D], sums of 2^(z - m) v
+  float2* part_ml;       // the same rows' m and sum of 2^(z - m)
+};
+
+__device__ __forceinline__ uint32_t items_of(const TileArgs& d, uint32_t s) {
+  const uint64_t rows = static_cast<uint64_t>(d.a.q_offsets[s + 1] - d.a.q_offsets[s]) * d.a.group;
+  return static_cast<uint32_t>((rows + kRows - 1) / kRows);
+}
+
+__device__ Item make_item(const TileArgs& d, uint32_t s, uint32_t index, int prefix) {
+  const AttnArgs& a = d.a;
+  Item it;
+  const uint32_t first = d.prefix ? 0 : a.q_offsets[s], last = d.prefix ? a.q_tokens : a.q_offsets[s + 1];
+  it.q_first = first;
+  it.row0 = index * kRows;
+  it.rows = min(static_cast<uint32_t>(kRows), (last - first) * a.group - it.row0);
+  int from, to;  // positions of the first and last row
+  if (d.prefix) {
+    it.table = 0;
+    it.pos0 = 0;
+    it.sinks = static_cast<int>(a.sinks);
+    to = prefix - 1;
+    from = prefix - static_cast<int>(d.max_q);  // at most: a row's own position decides
+  } else {
+    it.table = a.page_offsets[s];
+    it.pos0 = static_cast<int>(seq_length(a, s)) - static_cast<int>(last - first);
+    it.sinks = static_cast<int>(max(int64_t{0}, a.sinks - prefix));
+    from = it.pos0 + static_cast<int>(it.row0 / a.group);
+    to = it.pos0 + static_cast<int>((it.row0 + it.rows - 1) / a.group);
+  }
+  it.limit = max(to + 1, 0);
+  it.low = a.window ? static_cast<int>(max(int64_t{0}, from - a.window + 1)) : 0;
+  it.sink_tiles = it.low > 0 ? (min(it.sinks, it.limit) + kTokens - 1) / kTokens : 0;
+  it.first_tile = max(it.low / kTokens, it.sink_tiles);
+  // one tile at least, so that the rows are written
+  it.tiles = max(it.sink_tiles + max((it.limit + kTokens - 1) / kTokens - it.first_tile, 0), 1);
+  return it;
+}
+
+// Exclusive sum over the CTA; *total gets the sum.
+__device__ uint64_t plan_scan(uint64_t v, uint64_t* sums, uint64_t* total) {
+  const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  uint64_t inc = v;
+  for (int x = 1; x < 32; x *= 2) {
+    const uint64_t up = __shfl_up_sync(~0u, inc, x);
+    if (lane >= x) inc += up;
+  }
+  __syncthreads();
+  if (lane == 31) sums[warp] = inc;
+  __syncthreads();
+  uint64_t before = 0, all = 0;
+  for (uint32_t w = 0; w < kPlanThreads / 32; ++w) {
+    if (w < warp) before += sums[w];
+    all += sums[w];
+  }
+  *total = all;
+  return before + inc - v;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(TileArgs d) {
+  __shared__ uint64_t s_sums[kPlanThreads / 32], s_units[kPlanCache];
+  __shared__ uint32_t s_first[kPlanCache];
+  const AttnArgs& a = d.a;
+  const int prefix = static_cast<int>(prefix_length(a));
+  uint64_t total;
+  uint32_t items;
+  if (d.prefix) {
+    items = static_cast<uint32_t>((static_cast<uint64_t>(a.q_tokens) * a.group + kRows - 1) / kRows);
+  } else {
+    const uint32_t share = (a.n_seq + kPlanThreads - 1) / kPlanThreads, s0 = min(threadIdx.x * share, a.n_seq),
+                   s1 = min(s0 + share, a.n_seq);
+    uint32_t mine = 0;
+    for (uint32_t s = s0; s < s1; ++s) mine += items_of(d, s);
+    uint32_t at = static_cast<uint32_t>(plan_scan(mine, s_sums, &total));
+    items = static_cast<uint32_t>(total);
+    for (uint32_t s = s0; s < s1; ++s) {
+      if (s < kPlanCache) s_first[s] = at; else d.item_first[s] = at;
+      at += items_of(d, s);
+    }
+    __syncthreads();
+  }
+  uint64_t units = 0;
+  for (uint32_t i0 = 0; i0 < items; i0 += kPlanThreads) {
+    const uint32_t i = i0 + threadIdx.x;
+    uint64_t mine = 0;
+    if (i < items) {
+      uint32_t s = 0, first = 0;
+      if (!d.prefix) {  // the last sequence whose items begin at i or before
+        uint32_t hi = a.n_seq;
+        while (hi - s > 1) {
+          const uint32_t mid = (s + hi) / 2;
+          if ((mid < kPlanCache ? s_first[mid] : d.item_first[mid]) <= i) s = mid; else hi = mid;
+        }
+        first = s < kPlanCache ? s_first[s] : d.item_first[s];
+      }
+      const Item it = make_item(d, s, i - first, prefix);
+      d.items[i] = it;
+      mine = static_cast<uint64_t>(it.tiles) * a.kv_heads;
+    }
+    const uint64_t before = units + plan_scan(mine, s_sums, &total);
+    units += total;
+    if (i < items) {
+      d.unit_first[i] = before;
+      if (i < kPlanCache) s_units[i] = before;
+    }
+  }
+  __syncthreads();
+  const uint32_t ranges = static_cast<uint32_t>(min(static_cast<uint64_t>(d.max_ranges), units));
+  if (threadIdx.x == 0) {
+    d.counts[0] = items;
+    d.counts[1] = ranges;
+    d.unit_first[items] = units;
+  }
+  for (uint32_t r = threadIdx.x; r < ranges; r += kPlanThreads) {
+    const uint64_t unit = units * r / ranges;
+    uint32_t lo = 0, hi = items;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if ((mid < kPlanCache ? s_units[mid] : d.unit_first[mid]) <= unit) lo = mid; else hi = mid;
+    }
+    const uint32_t tiles = d.items[lo].tiles;
+    const uint64_t in = unit - (lo < kPlanCache ? s_units[lo] : d.unit_first[lo]);
+    d.begin[r] = RangeBegin{lo, static_cast<uint32_t>(in / tiles), static_cast<uint32_t>(in % tiles)};
+  }
+  for (uint32_t r = ranges + threadIdx.x; r < d.max_ranges; r += kPlanThreads) d.end[r] = RangeEnd{0, 0, 0, 0, 0};
+}
+
+template <int D>
+struct TileLayout {
+  static constexpr int kBlock = kTokens * 128;          // 64 values of 128 rows, swizzled
+  static constexpr int kOperand = kBlock * (D / 64);    // 128 rows
+  static constexpr int kStages = D == 128 ? 5 : 8;
+  static constexpr int kBytes = (2 + kStages) * kOperand + 1024;
+  static constexpr uint32_t kScores = 0, kSums = 256, kColumns = 512;
+};
+
+__device__ __forceinline__ int first_token(const Item& it, uint32_t tile) {
+  return (tile < static_cast<uint32_t>(it.sink_tiles) ? static_cast<int>(tile)
+                                                     : it.first_tile + static_cast<int>(tile) - it.sink_tiles) * kTokens;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map, TileArgs d) {
+  using L = TileLayout<D>;
+  constexpr uint32_t kStages = L::kStages;
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t s_bar[2 * kStages + 8];
+  __shared__ uint32_t s_tmem, s_gave_up;
+  __shared__ int s_seen[2][8][4];
+  const AttnArgs& a = d.a;
+  const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, range = blockIdx.x;
+  const uint32_t base = (smem_addr(raw) + 1023) & ~1023u, ring = base + 2 * L::kOperand;
+  auto full = [&](uint32_t i) { return smem_addr(&s_bar[i]); };
+  auto empty = [&](uint32_t i) { return smem_addr(&s_bar[kStages + i]); };
+  auto bar = [&](uint32_t kind, uint32_t half) { return smem_addr(&s_bar[2 * kStages + kind * 2 + half]); };
+  enum : uint32_t { kQueries, kScored, kWeighed, kSummed };
+  if (threadIdx.x == 0) {
+    for (uint32_t i = 0; i < kStages; ++i) {
+      mbar_init(full(i), 1);
+      mbar_init(empty(i), 1);
+    }
+    for (uint32_t h = 0; h < 2; ++h) {
+      mbar_init(bar(kQueries, h), kHalfRows);
+      mbar_init(bar(kScored, h), 1);
+      mbar_init(bar(kWeighed, h), kHalfRows);
+      mbar_init(bar(kSummed, h), 1);
+    }
+    s_gave_up = 0;
+    mbar_init_fence();
+  }
+  const uint32_t ranges = d.counts[1];
+  if (range >= ranges) return;
+  if (warp == 8) tmem_alloc(smem_addr(&s_tmem), L::kColumns);
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  const uint32_t tmem = s_tmem;
+  const uint64_t units = d.unit_first[d.counts[0]];
+  const uint32_t count = static_cast<uint32_t>(units * (range + 1) / ranges - units * range / ranges);
+  const RangeBegin begin = d.begin[range];
+
+  // Every role walks the range's pieces: the token tiles [at, at + n) of one item and head.
+  uint32_t item = begin.item, head = begin.head, at = begin.tile;
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 9) {  // ---- keys and values
+      const uint32_t boxes = kTokens / a.box_rows;
+      const uint32_t box = lane % boxes, half = lane / boxes;
+      uint32_t slot_at = 0;  // ring position
+      for (uint32_t left = count; left > 0;) {
+        const Item it = d.items[item];
+        const uint32_t n = min(it.tiles - at, left);
+        const uint32_t* table = (d.prefix ? a.prefix_table : a.page_table) + it.table;
+        for (uint32_t j = 0; j < n; ++j) {
+          const int from = first_token(it, at + j) + static_cast<int>(box * a.box_rows),
+                    to = from + static_cast<int>(a.box_rows);
+          const bool wanted = half < D / 64 && from < it.limit && (to > it.low || from < it.sinks);
+          const uint32_t bytes = __popc(__ballot_sync(~0u, wanted)) * a.box_rows * 128;
+          uint64_t row = 0;
+          if (wanted) row = checked_slot(a, table, from / a.page_tokens) * a.page_tokens + from % a.page_tokens;
+#pragma unroll
+          for (int plane = 0; plane < 2; ++plane, ++slot_at) {
+            const uint32_t stage = slot_at % kStages;
+            mbar_wait_warp(empty(stage), (slot_at / kStages & 1) ^ 1, &s_gave_up, a.status);
+            if (lane == 0) {
+              if (bytes) mbar_arrive_expect(full(stage), bytes); else mbar_arrive(full(stage));
+            }
+            __syncwarp();
+            if (wanted)
+              tma_load_3d(ring + stage * L::kOperand + half * L::kBlock + box * a.box_rows * 128, &map, half * 64,
+                          head, static_cast<int>(row + (plane ? a.v_row0 : a.k_row0)), full(stage));
+          }
+        }
+        left -= n;
+        at = 0;
+        if (++head == a.kv_heads) {
+          head = 0;
+          ++item;
+        }
+      }
+      // No copy may be in flight when the CTA ends.
+      for (uint32_t i = slot_at > kStages ? slot_at - kStages : 0; i < slot_at; ++i)
+        mbar_wait_warp(full(i % kStages), i / kStages & 1, &s_gave_up, a.status);
+    } else if (warp == 8 && lane == 0) {  // ---- the products
+      constexpr uint32_t kScoreShape = mma_shape<T>(kTokens, false), kValueShape = mma_shape<T>(D, true);
+      uint32_t slot_at = 0, pieces[2] = {0, 0}, done[2] = {0, 0};
+      auto wait = [&](uint32_t b, uint32_t phase) {
+        mbar_wait(b, phase & 1, &s_gave_up, a.status);
+        tmem_fence_after();
+      };
+      auto score = [&](uint32_t h, uint32_t slot) {  // scores of half h: its queries x the keys at `slot`
+        const uint32_t q = base + h * L::kOperand, k = ring + slot % kStages * L::kOperand;
+#pragma unroll
+        for (int e = 0; e < D / 16; ++e)
+          mma_ss(tmem + L::kScores + h * kTokens, smem_operand(q + e / 4 * L::kBlock + e % 4 * 32, 16, 1024),
+                 smem_operand(k + e / 4 * L::kBlock + e % 4 * 32, 16, 1024), kScoreShape, e > 0);
+        mma_commit(bar(kScored, h));
+      };
+      auto value = [&](uint32_t h, uint32_t slot, bool add) {  // sums of half h: its probabilities x the values
+        const uint32_t v = ring + slot % kStages * L::kOperand;
+#pragma unroll
+        for (int j = 0; j < kTokens / 16; ++j)
+          mma_ts(tmem + L::kSums + h * D, tmem + L::kScores + h * kTokens + j * 8,
+                 smem_operand(v + j * 16 * 128, L::kBlock, 1024), kValueShape, add || j > 0);
+        mma_commit(bar(kSummed, h));
+      };
+      for (uint32_t left = count; left > 0;) {
+        const uint32_t tiles = d.items[item].tiles, n = min(tiles - at, left);
+        const bool two = d.items[item].rows > kHalfRows;
+        wait(bar(kQueries, 0), pieces[0]++);
+        wait(full(slot_at % kStages), slot_at / kStages);
+        score(0, slot_at);
+        if (two) {
+          wait(bar(kQueries, 1), pieces[1]++);
+          score(1, slot_at);
+        }
+        mma_commit(empty(slot_at % kStages));
+        for (uint32_t j = 0; j < n; ++j, slot_at += 2) {
+          const uint32_t v = slot_at + 1, k = slot_at + 2;
+          const bool more = j + 1 < n;
+          wait(full(v % kStages), v / kStages);
+          wait(bar(kWeighed, 0), done[0]++);
+          value(0, v, j > 0);
+          if (more) {
+            wait(full(k % kStages), k / kStages);
+            score(0, k);
+          }
+          if (two) {
+            wait(bar(kWeighed, 1), done[1]++);
+            value(1, v, j > 0);
+          }
+          mma_commit(empty(v % kStages));
+          if (more) {
+            if (two) score(1, k);
+            mma_commit(empty(k % kStages));
+          }
+        }
+        left -= n;
+        at = 0;
+        if (++head == a.kv_heads) {
+          head = 0;
+          ++item;
+        }
+      }
+    }
+    __syncwarp();
+  } else {  // ---- the softmax of half `h`, one thread for each row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    const uint32_t h = warp / 4, r = threadIdx.x, quarter = warp % 4 * 32 << 16;
+    const uint32_t scores = tmem + quarter + L::kScores + h * kTokens, sums = tmem + quarter + L::kSums + h * D;
+    const int prefix = static_cast<int>(prefix_length(a));
+    uint32_t pieces = 0, done = 0, tiles_done = 0;
+    for (uint32_t left = count; left > 0; ++pieces) {
+      const Item it = d.items[item];
+      const uint32_t n = min(it.tiles - at, left);
+      const uint32_t row = it.row0 + r, t = it.q_first + row / a.group, q_head = head * a.group + row % a.group;
+      int hi = -1, lo = 0;
+      if (r < it.rows) {
+        if (d.prefix) {
+          const uint32_t s = seq_of(a, t);
+          const int nq = static_cast<int>(a.q_offsets[s + 1] - a.q_offsets[s]);
+          const int pos = prefix + static_cast<int>(seq_length(a, s)) - nq + static_cast<int>(t - a.q_offsets[s]);
+          hi = min(pos, prefix - 1);
+          lo = a.window ? static_cast<int>(max(int64_t{0}, pos - a.window + 1)) : 0;
+        } else {
+          hi = it.pos0 + static_cast<int>(row / a.group);
+          lo = a.window ? static_cast<int>(max(int64_t{0}, hi - a.window + 1)) : 0;
+        }
+      }
+      // What all, and what any, of the rows see: this half's [0, all_hi] from all_lo on, the item's any_*.
+      {
+        const bool valid = r < it.rows;
+        int v[4] = {valid ? hi : 0x7fffffff, valid ? lo : 0, hi, valid ? lo : 0x7fffffff};
+        v[0] = __reduce_min_sync(~0u, v[0]);
+        v[1] = __reduce_max_sync(~0u, v[1]);
+        v[2] = __reduce_max_sync(~0u, v[2]);
+        v[3] = __reduce_min_sync(~0u, v[3]);
+        if (lane < 4) s_seen[pieces & 1][warp][lane] = lane == 0 ? v[0] : lane == 1 ? v[1] : lane == 2 ? v[2] : v[3];
+      }
+      const bool active = h * kHalfRows < it.rows;
+      if (active) {  // this row's query, swizzled as the products read it
+        const uint32_t to = base + h * L::kOperand + r % kHalfRows * 128;
+        const uint4* q = reinterpret_cast<const uint4*>(a.q + t * a.q_token_stride + q_head * a.q_head_stride);
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 x = r < it.rows ? q[c] : make_uint4(0, 0, 0, 0);
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + c / 8 * L::kBlock + ((c % 8 ^ (r & 7)) << 4)),
+                       "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
+                       : "memory");
+        }
+        proxy_fence_smem();
+        mbar_arrive(bar(kQueries, h));
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      int all_hi = 0x7fffffff, all_lo = 0, any_hi = -1, any_lo = 0x7fffffff;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        const int* v = s_seen[pieces & 1][w];
+        if (static_cast<uint32_t>(w) / 4 == h) {
+          all_hi = min(all_hi, v[0]);
+          all_lo = max(all_lo, v[1]);
+        }
+        any_hi = max(any_hi, v[2]);
+        any_lo = min(any_lo, v[3]);
+      }
+      if (active) {
+        float m = -INFINITY, l = 0.f;
+        for (uint32_t j = 0; j < n; ++j, ++done) {
+          const int token = first_token(it, at + j);
+          mbar_wait_warp(bar(kScored, h), done & 1, &s_gave_up, a.status);
+          tmem_fence_after();
+          uint32_t z[kTokens];
+          tmem_load128(z, scores);
+          if (token + kTokens - 1 > all_hi || (token < all_lo && token + kTokens > it.sinks)) {
+            const int last = hi - token, from = lo - token, sink = it.sinks - token;
+#pragma unroll
+            for (int i = 0; i < kTokens; ++i)
+              if (i > last || (i < from && i >= sink)) z[i] = 0xff800000u;
+          }
+          float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < kTokens; ++i) top4[i % 4] = fmaxf(top4[i % 4], __uint_as_float(z[i]));
+          const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * a.scale_log2;
+          const bool grown = top > m + 8.f;
+          if (__any_sync(~0u, grown)) {
+            const float old = m;
+            if (grown) m = top;
+            const float f = grown ? exp2_approx(old - m) : 1.f;
+            l *= f;
+            if (j > 0) {
+              mbar_wait_warp(bar(kSummed, h), (done - 1) & 1, &s_gave_up, a.status);
+              tmem_fence_after();
+              for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_load32(o, sums + c);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_store32(sums + c, o);
+              }
+            }
+          }
+          const float ref = m == -INFINITY ? 0.f : m;
+          const float2 c2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
+          float2 sum[2] = {};
+          uint32_t p[kTokens / 2];
+#pragma unroll
+          for (int i = 0; i < kTokens / 2; ++i) {
+            float2 x = fma2(make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])), c2, ref2);
+            x.x = exp2_approx(x.x);
+            x.y = exp2_approx(x.y);
+            sum[i % 2] = add2(sum[i % 2], x);
+            p[i] = pack2<T>(x.x, x.y);
+          }
+          tmem_store64(scores, p);
+          sum[0] = add2(sum[0], sum[1]);
+          l += sum[0].x + sum[0].y;
+          // values that no row sees are cleared: 0 x NaN is not 0
+          if (h == 0 && (token + kTokens - 1 > any_hi || (token < any_lo && token + kTokens > it.sinks))) {
+            const uint32_t v = 2 * (tiles_done + j) + 1;
+            mbar_wait_warp(full(v % kStages), v / kStages & 1, &s_gave_up, a.status);
+            const int mine = token + static_cast<int>(r);
+            if (mine > any_hi || (mine < any_lo && mine >= it.sinks)) {
+              const uint32_t to = ring + v % kStages * L::kOperand + r * 128;
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + c / 8 * L::kBlock + c % 8 * 16), "r"(0)
+                             : "memory");
+            }
+            proxy_fence_smem();
+          }
+          __syncwarp();
+          tmem_wait_store();
+          tmem_fence_before();
+          mbar_arrive(bar(kWeighed, h));
+        }
+        mbar_wait_warp(bar(kSummed, h), (done - 1) & 1, &s_gave_up, a.status);
+        tmem_fence_after();
+        const bool whole = at == 0 && n == it.tiles, write = r < it.rows && !s_gave_up;
+        const uint64_t part = static_cast<uint64_t>(range * 2 + (pieces > 0)) * kRows + r;
+        Finish f{};
+        if (whole && write) {
+          f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + q_head, m, l);
+          store_lse(a, t, q_head, f);
+        } else if (write) {
+          d.part_ml[part] = make_float2(m, l);
+        }
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_load32(o, sums + c);
+          if (write) {
+            float x[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(o[i]);
+            if (whole) {
+              store_row<T, D, 32>(a, t, q_head, c, f, x);
+            } else {
+              float4* to = reinterpret_cast<float4*>(d.part_o + part * D + c);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) to[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            }
+          }
+        }
+        __syncwarp();
+        tmem_fence_before();
+      }
+      left -= n;
+      tiles_done += n;
+      if (left == 0 && threadIdx.x == 0)
+        d.end[range] = RangeEnd{item, head, at == 0, at + n < it.tiles, pieces > 0};
+      at = 0;
+      if (++head == a.kv_heads) {
+        head = 0;
+        ++item;
+      }
+    }
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  if (warp == 8) tmem_free(tmem, L::kColumns);
+}
+
+// Adds up the parts of the row tile that begins in a range and goes on in the next
+// ones, in the ranges' order: one warp for each row.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) tile_join_kernel(TileArgs d) {
+  constexpr int E = D / 32;
+  const AttnArgs& a = d.a;
+  const uint32_t range = blockIdx.x, r = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  const RangeEnd own = d.end[range];
+  if (!own.goes_on || !own.starts) return;
+  const Item it = d.items[own.item];
+  if (r >= it.rows) return;
+  uint32_t end = range + 1;
+  for (;; ++end) {
+    const RangeEnd next = d.end[end];
+    if (next.item != own.item || next.head != own.head || !next.goes_on) break;
+  }
+  auto row_of = [&](uint32_t k) { return static_cast<uint64_t>(k * 2 + (k == range ? own.slot : 0)) * kRows + r; };
+  float top = -INFINITY, sum = 0.f, x[E] = {};
+  for (uint32_t k = range + lane; k <= end; k += 32) top = fmaxf(top, d.part_ml[row_of(k)].x);
+  for (int i = 16; i; i /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
+  const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+  for (uint32_t k = range; k <= end; ++k) {
+    const uint64_t row = row_of(k);
+    const float2 ml = d.part_ml[row];
+    const float f = exp2_approx(ml.x - ref);
+    sum += f * ml.y;
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] += f * d.part_o[row * D + lane * E + e];
+  }
+  const uint32_t row = it.row0 + r, t = it.q_first + row / a.group, h = own.head * a.group + row % a.group;
+  const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
+  if constexpr (E == 4) {
+    store_row<T, D, 4>(a, t, h, lane * 4, f, x);
+  } else {  // two lanes' values in one
+    const float y[4] = {x[0], x[1], __shfl_down_sync(~0u, x[0], 1), __shfl_down_sync(~0u, x[1], 1)};
+    if (lane % 2 == 0) store_row<T, D, 4>(a, t, h, lane * 2, f, y);
+  }
+  if (lane == 0) store_lse(a, t, h, f);
+}
+
+uint64_t max_items(const tcx_kv_attention_args& x, bool prefix) {
+  return x.q_tokens * (x.q_heads / x.kv_heads) / kRows + (prefix ? 1 : x.n_seq);
+}
+
+// One CTA on every SM; a range holds one unit at least.
+uint32_t max_ranges(const tcx_kv_attention_args& x, bool prefix) {
+  const uint64_t pages = prefix ? x.prefix_pages : x.max_pages;
+  const uint64_t units = max_items(x, prefix) * x.kv_heads * (pages * x.page_tokens / kTokens + 2);
+  return static_cast<uint32_t>(std::min<uint64_t>(sm_count(), units));
+}
+
+struct Parts {
+  uint64_t item_first, items, unit_first, begin, end, counts, ml, o, total;
+};
+
+Parts parts(const tcx_kv_attention_args& x, bool prefix) {
+  const uint64_t items = max_items(x, prefix), ranges = max_ranges(x, prefix);
+  Parts p;
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t here = at;
+    at += align256(bytes);
+    return here;
+  };
+  p.item_first = take((x.n_seq + 1) * 4);
+  p.items = take(items * sizeof(Item));
+  p.unit_first = take((items + 1) * 8);
+  p.begin = take(ranges * sizeof(RangeBegin));
+  p.end = take(ranges * sizeof(RangeEnd));
+  p.counts = take(8);
+  p.ml = take(ranges * 2 * kRows * sizeof(float2));
+  p.o = take(ranges * 2 * kRows * x.head_dim * sizeof(float));
+  p.total = at;
+  return p;
+}
+
+template <typename T, int D>
+tcx_status launch(const TileArgs& d, const CUtensorMap& map, cudaStream_t stream) {
+  using L = TileLayout<D>;
+  tile_plan_kernel<<<1, kPlanThreads, 0, stream>>>(d);
+  note_launches(1);
+  TCX_CUDA_TRY(cudaGetLastError());
+  TCX_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+  tile_kernel<T, D><<<d.max_ranges, kThreads, L::kBytes, stream>>>(map, d);
+  note_launches(1);
+  TCX_CUDA_TRY(cudaGetLastError());
+  if (d.max_ranges > 1) {
+    tile_join_kernel<T, D><<<dim3(d.max_ranges - 1, kRows / 8), 256, 0, stream>>>(d);
+    note_launches(1);
+    TCX_CUDA_TRY(cudaGetLastError());
+  }
+  return TCX_OK;
+}
+
+}  // namespace
+
+uint64_t tile_scratch_bytes(const tcx_kv_attention_args& x, bool prefix) { return parts(x, prefix).total; }
+
+tcx_status launch_tile(const tcx_kv_attention_args& x, const AttnArgs& a, const CUtensorMap& map, bool prefix,
+                       void* scratch, cudaStream_t stream) {
+  const Parts p = parts(x, prefix);
+  uint8_t* at = static_cast<uint8_t*>(scratch);
+  TileArgs d{};
+  d.a = a;
+  d.prefix = prefix;
+  d.max_q = static_cast<uint32_t>(x.max_q);
+  d.max_ranges = max_ranges(x, prefix);
+  d.item_first = reinterpret_cast<uint32_t*>(at + p.item_first);
+  d.items = reinterpret_cast<Item*>(at + p.items);
+  d.unit_first = reinterpret_cast<uint64_t*>(at + p.unit_first);
+  d.begin = reinterpret_cast<RangeBegin*>(at + p.begin);
+  d.end = reinterpret_cast<RangeEnd*>(at + p.end);
+  d.counts = reinterpret_cast<uint32_t*>(at + p.counts);
+  d.part_ml = reinterpret_cast<float2*>(at + p.ml);
+  d.part_o = reinterpret_cast<float*>(at + p.o);
+  if (x.dtype == TCX_KV_BF16)
+    return x.head_dim == 128 ? launch<__nv_bfloat16, 128>(d, map, stream) : launch<__nv_bfloat16, 64>(d, map, stream);
+  return x.head_dim == 128 ? launch<__half, 128>(d, map, stream) : launch<__half, 64>(d, map, stream);
+}
+
+}  // namespace tcx

@@ -30,7 +30,7 @@ from .kvcache import KvWorkload
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _STATUS = {1: "page slot outside the pool", 2: "more tokens than the sequence's pages hold",
-           3: "budget past the destination pages"}
+           3: "budget past the destination pages", 4: "a copy into shared memory did not arrive"}
 
 
 def _refuse(message: str):
