@@ -20,6 +20,7 @@
 // are; row tiles cut by a border leave parts that tile_join_kernel adds up in the
 // ranges' order. tile_plan_kernel lays the units out from the device's lengths.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_attention.cuh"
 
@@ -32,6 +33,9 @@ constexpr int kRows = 2 * kHalfRows;
 constexpr int kThreads = 384;
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCache = 2048;
+// What a piece of a row tile costs beside its token tiles (its queries, its first
+// scores, its output), in token tiles: counted when the work is cut into ranges.
+constexpr uint32_t kPieceCost = 3;
 
 // A tile of rows: row r is query token q_first + (row0 + r) / group.
 struct Item {
@@ -45,6 +49,7 @@ struct Item {
 
 struct RangeBegin {
   uint32_t item, head, tile;
+  uint64_t unit;  // token tiles before it
 };
 
 struct RangeEnd {
@@ -58,7 +63,7 @@ struct TileArgs {
   uint32_t max_q, max_ranges;
   uint32_t* item_first;  // [n_seq + 1]
   Item* items;
-  uint64_t* unit_first;  // [items + 1]
+  uint64_t* unit_first;  // [items]: token tiles of all heads before it
   RangeBegin* begin;     // [max_ranges + 1]
   RangeEnd* end;         // [max_ranges]
   uint32_t* counts;      // items, ranges
@@ -170,21 +175,28 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(TileArgs d) {
   }
   __syncthreads();
   const uint32_t ranges = static_cast<uint32_t>(min(static_cast<uint64_t>(d.max_ranges), units));
+  // Every range must hold more than a piece's cost to hold a tile.
+  const uint64_t pieces = static_cast<uint64_t>(items) * a.kv_heads;
+  const uint64_t cost = (units + kPieceCost * pieces) / ranges > kPieceCost ? kPieceCost : 0;
   if (threadIdx.x == 0) {
     d.counts[0] = items;
     d.counts[1] = ranges;
-    d.unit_first[items] = units;
+    d.begin[ranges] = RangeBegin{items, 0, 0, units};
   }
   for (uint32_t r = threadIdx.x; r < ranges; r += kPlanThreads) {
-    const uint64_t unit = units * r / ranges;
+    const uint64_t at = (units + cost * pieces) * r / ranges;
+    auto first_of = [&](uint32_t i) {
+      return (i < kPlanCache ? s_units[i] : d.unit_first[i]) + cost * a.kv_heads * i;
+    };
     uint32_t lo = 0, hi = items;
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
-      if ((mid < kPlanCache ? s_units[mid] : d.unit_first[mid]) <= unit) lo = mid; else hi = mid;
+      if (first_of(mid) <= at) lo = mid; else hi = mid;
     }
-    const uint32_t tiles = d.items[lo].tiles;
-    const uint64_t in = unit - (lo < kPlanCache ? s_units[lo] : d.unit_first[lo]);
-    d.begin[r] = RangeBegin{lo, static_cast<uint32_t>(in / tiles), static_cast<uint32_t>(in % tiles)};
+    const uint64_t in = at - first_of(lo), tiles = d.items[lo].tiles, head = in / (tiles + cost);
+    const uint64_t tile = max(in % (tiles + cost), cost) - cost;
+    d.begin[r] = RangeBegin{lo, static_cast<uint32_t>(head), static_cast<uint32_t>(tile),
+                            first_of(lo) - cost * a.kv_heads * lo + head * tiles + tile};
   }
   for (uint32_t r = ranges + threadIdx.x; r < d.max_ranges; r += kPlanThreads) d.end[r] = RangeEnd{0, 0, 0, 0, 0};
 }
@@ -208,16 +220,16 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   using L = TileLayout<D>;
   constexpr uint32_t kStages = L::kStages;
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t s_bar[2 * kStages + 8];
+  __shared__ uint64_t s_bar[2 * kStages + 10];
   __shared__ uint32_t s_tmem, s_gave_up;
-  __shared__ int s_seen[2][8][4];
+  __shared__ __align__(16) int s_seen[2][8][4];
   const AttnArgs& a = d.a;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, range = blockIdx.x;
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u, ring = base + 2 * L::kOperand;
   auto full = [&](uint32_t i) { return smem_addr(&s_bar[i]); };
   auto empty = [&](uint32_t i) { return smem_addr(&s_bar[kStages + i]); };
   auto bar = [&](uint32_t kind, uint32_t half) { return smem_addr(&s_bar[2 * kStages + kind * 2 + half]); };
-  enum : uint32_t { kQueries, kScored, kWeighed, kSummed };
+  enum : uint32_t { kQueries, kScored, kWeighed, kWeighedAll, kSummed };
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < kStages; ++i) {
       mbar_init(full(i), 1);
@@ -227,6 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       mbar_init(bar(kQueries, h), kHalfRows);
       mbar_init(bar(kScored, h), 1);
       mbar_init(bar(kWeighed, h), kHalfRows);
+      mbar_init(bar(kWeighedAll, h), kHalfRows);
       mbar_init(bar(kSummed, h), 1);
     }
     s_gave_up = 0;
@@ -239,9 +252,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = s_tmem;
-  const uint64_t units = d.unit_first[d.counts[0]];
-  const uint32_t count = static_cast<uint32_t>(units * (range + 1) / ranges - units * range / ranges);
+  const uint32_t items = d.counts[0];
   const RangeBegin begin = d.begin[range];
+  const uint32_t count = static_cast<uint32_t>(d.begin[range + 1].unit - begin.unit);
 
   // Every role walks the range's pieces: the token tiles [at, at + n) of one item and head.
   uint32_t item = begin.item, head = begin.head, at = begin.tile;
@@ -251,8 +264,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       const uint32_t boxes = kTokens / a.box_rows;
       const uint32_t box = lane % boxes, half = lane / boxes;
       uint32_t slot_at = 0;  // ring position
+      Item it = d.items[item];
       for (uint32_t left = count; left > 0;) {
-        const Item it = d.items[item];
         const uint32_t n = min(it.tiles - at, left);
         const uint32_t* table = (d.prefix ? a.prefix_table : a.page_table) + it.table;
         for (uint32_t j = 0; j < n; ++j) {
@@ -277,9 +290,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
         left -= n;
         at = 0;
-        if (++head == a.kv_heads) {
+        if (++head == a.kv_heads && left > 0) {
           head = 0;
-          ++item;
+          it = d.items[++item];
         }
       }
       // No copy may be in flight when the CTA ends.
@@ -300,17 +313,24 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                  smem_operand(k + e / 4 * L::kBlock + e % 4 * 32, 16, 1024), kScoreShape, e > 0);
         mma_commit(bar(kScored, h));
       };
-      auto value = [&](uint32_t h, uint32_t slot, bool add) {  // sums of half h: its probabilities x the values
-        const uint32_t v = ring + slot % kStages * L::kOperand;
+      // Sums of half h: its probabilities x the values. The last quarter of the
+      // probabilities follows the others.
+      auto value = [&](uint32_t h, uint32_t slot, bool add) {
+        const uint32_t v = ring + slot % kStages * L::kOperand, phase = done[h]++;
+        wait(bar(kWeighed, h), phase);
 #pragma unroll
-        for (int j = 0; j < kTokens / 16; ++j)
+        for (int j = 0; j < kTokens / 16; ++j) {
+          if (j == kTokens / 16 * 3 / 4) wait(bar(kWeighedAll, h), phase);
           mma_ts(tmem + L::kSums + h * D, tmem + L::kScores + h * kTokens + j * 8,
                  smem_operand(v + j * 16 * 128, L::kBlock, 1024), kValueShape, add || j > 0);
+        }
         mma_commit(bar(kSummed, h));
       };
+      uint32_t tiles = d.items[item].tiles, rows = d.items[item].rows;
+      uint32_t next = min(item + 1, items - 1), next_tiles = d.items[next].tiles, next_rows = d.items[next].rows;
       for (uint32_t left = count; left > 0;) {
-        const uint32_t tiles = d.items[item].tiles, n = min(tiles - at, left);
-        const bool two = d.items[item].rows > kHalfRows;
+        const uint32_t n = min(tiles - at, left);
+        const bool two = rows > kHalfRows;
         wait(bar(kQueries, 0), pieces[0]++);
         wait(full(slot_at % kStages), slot_at / kStages);
         score(0, slot_at);
@@ -323,16 +343,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           const uint32_t v = slot_at + 1, k = slot_at + 2;
           const bool more = j + 1 < n;
           wait(full(v % kStages), v / kStages);
-          wait(bar(kWeighed, 0), done[0]++);
           value(0, v, j > 0);
           if (more) {
             wait(full(k % kStages), k / kStages);
             score(0, k);
           }
-          if (two) {
-            wait(bar(kWeighed, 1), done[1]++);
-            value(1, v, j > 0);
-          }
+          if (two) value(1, v, j > 0);
           mma_commit(empty(v % kStages));
           if (more) {
             if (two) score(1, k);
@@ -343,88 +359,126 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         at = 0;
         if (++head == a.kv_heads) {
           head = 0;
-          ++item;
+          tiles = next_tiles;
+          rows = next_rows;
+          next = min(next + 1, items - 1);
+          next_tiles = d.items[next].tiles;
+          next_rows = d.items[next].rows;
         }
       }
     }
     __syncwarp();
   } else {  // ---- the softmax of half `h`, one thread for each row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+    // A warp moves its 32 rows' queries in, and outputs out, with kLanes lanes to a row.
+    constexpr uint32_t kLanes = D / 8, kMoves = kLanes;
     const uint32_t h = warp / 4, r = threadIdx.x, quarter = warp % 4 * 32 << 16;
     const uint32_t scores = tmem + quarter + L::kScores + h * kTokens, sums = tmem + quarter + L::kSums + h * D;
+    const uint32_t own = base + h * L::kOperand + warp % 4 * 32 * 128;  // the warp's rows in shared memory
+    auto place = [&](uint32_t row, uint32_t c) {  // 16-byte piece c of a row, swizzled as the products read it
+      return own + c / 8 * L::kBlock + row * 128 + ((c % 8 ^ (row & 7)) << 4);
+    };
     const int prefix = static_cast<int>(prefix_length(a));
-    uint32_t pieces = 0, done = 0, tiles_done = 0;
+    uint32_t pieces = 0, done = 0, tiles_done = 0, t, q_head;
+    Item it = d.items[item];
+    uint4 q[kMoves];
+    auto fetch = [&] {  // this piece's row, and its warp's queries from global memory
+      const uint32_t row = it.row0 + r;
+      t = it.q_first + row / a.group;
+      q_head = head * a.group + row % a.group;
+      const uint64_t from = t * a.q_token_stride + q_head * a.q_head_stride;
+#pragma unroll
+      for (uint32_t i = 0; i < kMoves; ++i) {
+        const uint32_t src = i * (32 / kLanes) + lane / kLanes;
+        const uint64_t at_row = __shfl_sync(~0u, from, src);
+        q[i] = (r & ~31u) + src < it.rows ? *reinterpret_cast<const uint4*>(a.q + at_row + lane % kLanes * 16)
+                                          : make_uint4(0, 0, 0, 0);
+      }
+    };
+    fetch();
     for (uint32_t left = count; left > 0; ++pieces) {
-      const Item it = d.items[item];
       const uint32_t n = min(it.tiles - at, left);
-      const uint32_t row = it.row0 + r, t = it.q_first + row / a.group, q_head = head * a.group + row % a.group;
-      int hi = -1, lo = 0;
-      if (r < it.rows) {
-        if (d.prefix) {
+      const uint32_t row = it.row0 + r;
+      const bool active = h * kHalfRows < it.rows;
+      if (active) {
+#pragma unroll
+        for (uint32_t i = 0; i < kMoves; ++i)
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                           place(i * (32 / kLanes) + lane / kLanes, lane % kLanes)),
+                       "r"(q[i].x), "r"(q[i].y), "r"(q[i].z), "r"(q[i].w)
+                       : "memory");
+        proxy_fence_smem();
+        mbar_arrive(bar(kQueries, h));
+      }
+      // What this row sees: [0, hi] from lo on, and the sinks. What all rows of this
+      // half see (all_*), and what any row of the item sees (any_*).
+      int hi = -1, lo = 0, all_hi, all_lo, any_hi, any_lo;
+      auto low_of = [&](int pos) {
+        return a.window ? static_cast<int>(max(int64_t{0}, pos - a.window + 1)) : 0;
+      };
+      if (d.prefix) {
+        if (r < it.rows) {
           const uint32_t s = seq_of(a, t);
           const int nq = static_cast<int>(a.q_offsets[s + 1] - a.q_offsets[s]);
           const int pos = prefix + static_cast<int>(seq_length(a, s)) - nq + static_cast<int>(t - a.q_offsets[s]);
           hi = min(pos, prefix - 1);
-          lo = a.window ? static_cast<int>(max(int64_t{0}, pos - a.window + 1)) : 0;
-        } else {
-          hi = it.pos0 + static_cast<int>(row / a.group);
-          lo = a.window ? static_cast<int>(max(int64_t{0}, hi - a.window + 1)) : 0;
+          lo = low_of(pos);
         }
-      }
-      // What all, and what any, of the rows see: this half's [0, all_hi] from all_lo on, the item's any_*.
-      {
         const bool valid = r < it.rows;
-        int v[4] = {valid ? hi : 0x7fffffff, valid ? lo : 0, hi, valid ? lo : 0x7fffffff};
-        v[0] = __reduce_min_sync(~0u, v[0]);
-        v[1] = __reduce_max_sync(~0u, v[1]);
-        v[2] = __reduce_max_sync(~0u, v[2]);
-        v[3] = __reduce_min_sync(~0u, v[3]);
-        if (lane < 4) s_seen[pieces & 1][warp][lane] = lane == 0 ? v[0] : lane == 1 ? v[1] : lane == 2 ? v[2] : v[3];
-      }
-      const bool active = h * kHalfRows < it.rows;
-      if (active) {  // this row's query, swizzled as the products read it
-        const uint32_t to = base + h * L::kOperand + r % kHalfRows * 128;
-        const uint4* q = reinterpret_cast<const uint4*>(a.q + t * a.q_token_stride + q_head * a.q_head_stride);
+        all_hi = __reduce_min_sync(~0u, valid ? hi : 0x7fffffff);
+        all_lo = __reduce_max_sync(~0u, valid ? lo : 0);
+        any_hi = __reduce_max_sync(~0u, hi);
+        any_lo = __reduce_min_sync(~0u, valid ? lo : 0x7fffffff);
+        if (lane == 0) *reinterpret_cast<int4*>(s_seen[pieces & 1][warp]) = make_int4(all_hi, all_lo, any_hi, any_lo);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 x = r < it.rows ? q[c] : make_uint4(0, 0, 0, 0);
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + c / 8 * L::kBlock + ((c % 8 ^ (r & 7)) << 4)),
-                       "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
-                       : "memory");
+        for (int w = 0; w < 8; ++w) {
+          const int* v = s_seen[pieces & 1][w];
+          if (static_cast<uint32_t>(w) / 4 == h) {
+            all_hi = min(all_hi, v[0]);
+            all_lo = max(all_lo, v[1]);
+          }
+          any_hi = max(any_hi, v[2]);
+          any_lo = min(any_lo, v[3]);
         }
-        proxy_fence_smem();
-        mbar_arrive(bar(kQueries, h));
+      } else {
+        hi = r < it.rows ? it.pos0 + static_cast<int>(row / a.group) : -1;
+        lo = low_of(hi);
+        all_hi = it.pos0 + static_cast<int>((it.row0 + h * kHalfRows) / a.group);
+        all_lo = low_of(it.pos0 + static_cast<int>((it.row0 + it.rows - 1) / a.group));
+        any_hi = it.limit - 1;
+        any_lo = it.low;
       }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      int all_hi = 0x7fffffff, all_lo = 0, any_hi = -1, any_lo = 0x7fffffff;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        const int* v = s_seen[pieces & 1][w];
-        if (static_cast<uint32_t>(w) / 4 == h) {
-          all_hi = min(all_hi, v[0]);
-          all_lo = max(all_lo, v[1]);
-        }
-        any_hi = max(any_hi, v[2]);
-        any_lo = min(any_lo, v[3]);
-      }
+      float m = -INFINITY, l = 0.f;
       if (active) {
-        float m = -INFINITY, l = 0.f;
         for (uint32_t j = 0; j < n; ++j, ++done) {
           const int token = first_token(it, at + j);
           mbar_wait_warp(bar(kScored, h), done & 1, &s_gave_up, a.status);
           tmem_fence_after();
           uint32_t z[kTokens];
           tmem_load128(z, scores);
+          bool plain = true;
           if (token + kTokens - 1 > all_hi || (token < all_lo && token + kTokens > it.sinks)) {
-            const int last = hi - token, from = lo - token, sink = it.sinks - token;
+            plain = false;
+            // bits of the tile's tokens below x
+            auto below = [&](int x, int word) {
+              const int n_bits = min(max(x - token - word * 32, 0), 32);
+              return n_bits == 32 ? ~0u : (1u << n_bits) - 1;
+            };
 #pragma unroll
-            for (int i = 0; i < kTokens; ++i)
-              if (i > last || (i < from && i >= sink)) z[i] = 0xff800000u;
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t see = below(hi + 1, w) & (~below(lo, w) | below(it.sinks, w));
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(see >> i & 1)) z[w * 32 + i] = 0xff800000u;
+            }
           }
-          float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          float top2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < kTokens; ++i) top4[i % 4] = fmaxf(top4[i % 4], __uint_as_float(z[i]));
-          const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * a.scale_log2;
+          for (int i = 0; i < kTokens; i += 2)
+            top2[i / 2 % 2] = max3_nan(top2[i / 2 % 2], __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
+          const float top = max3_nan(top2[0], top2[1], top2[0]) * a.scale_log2;
+          plain = plain && !__any_sync(~0u, !(fabsf(top) < INFINITY));
           const bool grown = top > m + 8.f;
           if (__any_sync(~0u, grown)) {
             const float old = m;
@@ -443,21 +497,6 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
               }
             }
           }
-          const float ref = m == -INFINITY ? 0.f : m;
-          const float2 c2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
-          float2 sum[2] = {};
-          uint32_t p[kTokens / 2];
-#pragma unroll
-          for (int i = 0; i < kTokens / 2; ++i) {
-            float2 x = fma2(make_float2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])), c2, ref2);
-            x.x = exp2_approx(x.x);
-            x.y = exp2_approx(x.y);
-            sum[i % 2] = add2(sum[i % 2], x);
-            p[i] = pack2<T>(x.x, x.y);
-          }
-          tmem_store64(scores, p);
-          sum[0] = add2(sum[0], sum[1]);
-          l += sum[0].x + sum[0].y;
           // values that no row sees are cleared: 0 x NaN is not 0
           if (h == 0 && (token + kTokens - 1 > any_hi || (token < any_lo && token + kTokens > it.sinks))) {
             const uint32_t v = 2 * (tiles_done + j) + 1;
@@ -467,56 +506,148 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
               const uint32_t to = ring + v % kStages * L::kOperand + r * 128;
 #pragma unroll
               for (int c = 0; c < D / 8; ++c)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + c / 8 * L::kBlock + c % 8 * 16), "r"(0)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + c / 8 * L::kBlock + ((c % 8 ^ (r & 7)) << 4)),
+                             "r"(0)
                              : "memory");
             }
             proxy_fence_smem();
+            __syncwarp();
           }
-          __syncwarp();
-          tmem_wait_store();
-          tmem_fence_before();
-          mbar_arrive(bar(kWeighed, h));
+          const float ref = m == -INFINITY ? 0.f : m;
+          const float2 c2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
+          float2 sum[2] = {};
+          // Every fourth pair's exponentials run on the FMA units: the exponential
+          // units alone need as long as the products do.
+          auto weigh = [&](auto mixed) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t p[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int k = c * 32 + 2 * i;
+                float2 x = fma2(make_float2(__uint_as_float(z[k]), __uint_as_float(z[k + 1])), c2, ref2);
+                if (decltype(mixed)::value && i % 4 == 3) {
+                  x = exp2_fma(x);
+                } else {
+                  x.x = exp2_approx(x.x);
+                  x.y = exp2_approx(x.y);
+                }
+                sum[i % 2] = add2(sum[i % 2], x);
+                p[i] = pack2<T>(x.x, x.y);
+              }
+              tmem_store16(scores + c * 16, p);
+              if (c >= 2) {
+                tmem_wait_store();
+                tmem_fence_before();
+                mbar_arrive(bar(c == 2 ? kWeighed : kWeighedAll, h));
+              }
+            }
+          };
+          if (plain) weigh(std::true_type{}); else weigh(std::false_type{});
+          sum[0] = add2(sum[0], sum[1]);
+          l += sum[0].x + sum[0].y;
         }
+      }
+      const bool whole = at == 0 && n == it.tiles, final = whole && a.part_o == nullptr;
+      const bool write = active && r < it.rows && !s_gave_up;
+      // rows of this warp that are written
+      const uint32_t first_row = r & ~31u, rows = active && !s_gave_up && first_row < it.rows ? min(it.rows - first_row, 32u) : 0;
+      const uint64_t q_row = static_cast<uint64_t>(t) * a.kv_heads * a.group + q_head;
+      const uint64_t part = static_cast<uint64_t>(range * 2 + (pieces > 0)) * kRows + r;
+      const uint64_t out_at = t * a.out_token_stride + q_head * a.out_head_stride;
+      if (threadIdx.x == 0 && left == n)
+        d.end[range] = RangeEnd{item, head, at == 0, at + n < it.tiles, pieces > 0};
+      left -= n;
+      tiles_done += n;
+      at = 0;
+      if (left > 0) {  // the next piece's queries are on their way while this one's output leaves
+        if (++head == a.kv_heads) {
+          head = 0;
+          it = d.items[++item];
+        }
+        fetch();
+      }
+      if (active) {
         mbar_wait_warp(bar(kSummed, h), (done - 1) & 1, &s_gave_up, a.status);
         tmem_fence_after();
-        const bool whole = at == 0 && n == it.tiles, write = r < it.rows && !s_gave_up;
-        const uint64_t part = static_cast<uint64_t>(range * 2 + (pieces > 0)) * kRows + r;
         Finish f{};
-        if (whole && write) {
-          f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + q_head, m, l);
-          store_lse(a, t, q_head, f);
+        if (write && whole) {
+          f = finish_row(a, q_row, m, l);
+          if (final) a.lse[q_row] = kLn2 * f.lse; else a.part_lse[q_row] = f.lse;
         } else if (write) {
           d.part_ml[part] = make_float2(m, l);
         }
+        __syncwarp();
+        // The rows leave through the queries' place in shared memory, which the
+        // products have read.
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
-          __syncwarp();
           tmem_load32(o, sums + c);
-          if (write) {
-            float x[32];
+          float x[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(o[i]);
-            if (whole) {
-              store_row<T, D, 32>(a, t, q_head, c, f, x);
-            } else {
-              float4* to = reinterpret_cast<float4*>(d.part_o + part * D + c);
+          for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(o[i]);
+          if (whole) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) to[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+            for (int i = 0; i < 32; ++i) x[i] = f.own == 0.f ? 0.f : x[i] * f.own;  // nothing seen: 0
+            if (f.prior != 0.f) {
+              const float4* y = reinterpret_cast<const float4*>(a.prior_o + q_row * D + c);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 v = y[i];
+                x[4 * i] += f.prior * v.x;
+                x[4 * i + 1] += f.prior * v.y;
+                x[4 * i + 2] += f.prior * v.z;
+                x[4 * i + 3] += f.prior * v.w;
+              }
             }
           }
+          if (final) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, c / 8 + i)),
+                           "r"(pack2<T>(x[8 * i], x[8 * i + 1])), "r"(pack2<T>(x[8 * i + 2], x[8 * i + 3])),
+                           "r"(pack2<T>(x[8 * i + 4], x[8 * i + 5])), "r"(pack2<T>(x[8 * i + 6], x[8 * i + 7]))
+                           : "memory");
+          } else {
+            // 32 values of each row, 128 bytes, in the first block
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, i)),
+                           "f"(x[4 * i]), "f"(x[4 * i + 1]), "f"(x[4 * i + 2]), "f"(x[4 * i + 3])
+                           : "memory");
+            __syncwarp();
+            float* to = whole ? a.part_o + q_row * D : d.part_o + part * D;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+              const uint32_t src = i * 4 + lane / 8;
+              float* at_row = reinterpret_cast<float*>(__shfl_sync(~0u, reinterpret_cast<uint64_t>(to), src));
+              uint4 v;
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                           : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                           : "r"(place(src, lane % 8))
+                           : "memory");
+              if (src < rows) *reinterpret_cast<uint4*>(at_row + c + lane % 8 * 4) = v;
+            }
+            __syncwarp();
+          }
         }
-        __syncwarp();
+        if (final) {
+          __syncwarp();
+#pragma unroll
+          for (uint32_t i = 0; i < kMoves; ++i) {
+            const uint32_t src = i * (32 / kLanes) + lane / kLanes;
+            const uint64_t at_row = __shfl_sync(~0u, out_at, src);
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(place(src, lane % kLanes))
+                         : "memory");
+            if (src < rows) *reinterpret_cast<uint4*>(a.out + at_row + lane % kLanes * 16) = v;
+          }
+          __syncwarp();
+        }
         tmem_fence_before();
-      }
-      left -= n;
-      tiles_done += n;
-      if (left == 0 && threadIdx.x == 0)
-        d.end[range] = RangeEnd{item, head, at == 0, at + n < it.tiles, pieces > 0};
-      at = 0;
-      if (++head == a.kv_heads) {
-        head = 0;
-        ++item;
       }
     }
   }
@@ -593,8 +724,8 @@ Parts parts(const tcx_kv_attention_args& x, bool prefix) {
   };
   p.item_first = take((x.n_seq + 1) * 4);
   p.items = take(items * sizeof(Item));
-  p.unit_first = take((items + 1) * 8);
-  p.begin = take(ranges * sizeof(RangeBegin));
+  p.unit_first = take(items * 8);
+  p.begin = take((ranges + 1) * sizeof(RangeBegin));
   p.end = take(ranges * sizeof(RangeEnd));
   p.counts = take(8);
   p.ml = take(ranges * 2 * kRows * sizeof(float2));
