@@ -17,53 +17,6 @@
 namespace tcx {
 namespace {
 
-template <typename T>
-__device__ __forceinline__ float to_float(T v) {
-  return static_cast<float>(v);
-}
-
-// One warp per token and kv head: the token's weights of all rows, added in the
-// rows' order, so that the sum does not depend on the run.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attention_weights_kernel(AttnArgs a) {
-  constexpr int E = D / 32;
-  const uint32_t lane = threadIdx.x % 32, kvh = blockIdx.y, s = blockIdx.z;
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 4 + threadIdx.x / 32;
-  const int64_t len = seq_length(a, s);
-  if (j >= len) return;
-  const int64_t nq = a.q_offsets[s + 1] - a.q_offsets[s];
-  const uint32_t q_heads = a.kv_heads * a.group;
-  const uint64_t off = checked_slot(a, a.page_table + a.page_offsets[s], j / a.page_tokens) * a.page_bytes +
-                       (j % a.page_tokens) * a.token_bytes + kvh * a.row_bytes;
-  const T* kp = reinterpret_cast<const T*>(a.pool + a.k_plane * a.pool_pages * a.page_bytes + off);
-  float k[E], sum = 0.f;
-  for (int e = 0; e < E; ++e) k[e] = to_float(kp[lane * E + e]);
-  for (int64_t i = 0; i < nq; ++i) {
-    const int64_t pos = len - nq + i;
-    if (j > pos || (a.window && j <= pos - a.window && j >= a.sinks)) continue;
-    const uint64_t t = a.q_offsets[s] + i;
-    for (uint32_t g = 0; g < a.group; ++g) {
-      const uint32_t h = kvh * a.group + g;
-      const T* qp = reinterpret_cast<const T*>(a.q + t * a.q_token_stride + h * a.q_head_stride);
-      float z = 0.f;
-      for (int e = 0; e < E; ++e) z += to_float(qp[lane * E + e]) * k[e];
-      for (int x = 16; x; x /= 2) z += __shfl_xor_sync(~0u, z, x);
-      sum += exp2f(z * a.scale_log2 - a.lse[t * q_heads + h] * kLog2e);
-    }
-  }
-  if (lane == 0) a.weights[kvh * a.weights_head_stride + a.page_offsets[s] * a.page_tokens + j] += sum;
-}
-
-template <typename T, int D>
-tcx_status launch_weights(const AttnArgs& a, uint64_t max_tokens, cudaStream_t stream) {
-  if (max_tokens == 0) return TCX_OK;
-  const dim3 grid(static_cast<unsigned>((max_tokens + 3) / 4), a.kv_heads, a.n_seq);
-  attention_weights_kernel<T, D><<<grid, 128, 0, stream>>>(a);
-  note_launches(1);
-  TCX_CUDA_TRY(cudaGetLastError());
-  return TCX_OK;
-}
-
 tcx_status check_sizes(const tcx_kv_attention_args& a) {
   if (a.planes == 0 || a.pool_pages == 0 || a.page_tokens == 0 || a.kv_heads == 0 || a.q_heads == 0)
     return set_error(TCX_INVALID_ARGUMENT, "planes, pool_pages, page_tokens, kv_heads and q_heads must be > 0");
@@ -223,11 +176,6 @@ extern "C" tcx_status tcx_kv_attention(const tcx_kv_attention_args* args, void* 
                                                : launch_tile(*args, a, map, false, scratch, s);
       st != TCX_OK)
     return st;
-  if (args->d_weights == nullptr) return TCX_OK;
-  const uint64_t max_tokens = args->max_pages * args->page_tokens;
-  if (args->dtype == TCX_KV_BF16)
-    return args->head_dim == 128 ? launch_weights<__nv_bfloat16, 128>(a, max_tokens, s)
-                                 : launch_weights<__nv_bfloat16, 64>(a, max_tokens, s);
-  return args->head_dim == 128 ? launch_weights<__half, 128>(a, max_tokens, s)
-                               : launch_weights<__half, 64>(a, max_tokens, s);
+  if (args->d_weights == nullptr || decode_fits(*args)) return TCX_OK;
+  return launch_weights(*args, a, map, s);
 }

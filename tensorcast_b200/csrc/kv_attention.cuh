@@ -168,4 +168,8 @@ uint64_t tile_scratch_bytes(const tcx_kv_attention_args& x, bool prefix);
 tcx_status launch_tile(const tcx_kv_attention_args& x, const AttnArgs& a, const CUtensorMap& map, bool prefix,
                        void* scratch, cudaStream_t stream);
 
+// Adds every token's softmax weights of many rows, whose lse is known (kv_weights.cu).
+tcx_status launch_weights(const tcx_kv_attention_args& x, const AttnArgs& a, const CUtensorMap& map,
+                          cudaStream_t stream);
+
 }  // namespace tcx

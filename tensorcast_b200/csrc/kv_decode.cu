@@ -14,7 +14,9 @@
 // as the output is) for the second product, sums in 32 bits. Where a sequence ends
 // inside a range the four warps' parts are joined in the tile's memory and written;
 // a sequence cut by a range's border leaves parts in the scratch that
-// decode_join_kernel adds up in the ranges' order.
+// decode_join_kernel adds up in the ranges' order. Where weights are accumulated, the
+// scores go to the scratch as well (rows x 4 bytes for a token, against its 4 D), and
+// decode_weights_kernel takes them up once the rows' sums are known.
 #include <algorithm>
 #include <atomic>
 
@@ -50,6 +52,9 @@ struct DecodeArgs {
   RangeInfo* info;  // [ranges]
   float* part_o;    // [ranges][2][kv_heads][kRows][D], sums of 2^(z - m) v
   float2* part_ml;  // the same rows' m and sum of 2^(z - m)
+  float* scores;    // [kv_heads][rows][columns], in powers of two, where weights are added up
+  uint32_t score_rows;
+  uint64_t columns;
 };
 
 template <int D>
@@ -83,13 +88,13 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnArgs& a, uint32_t s, int p
   return i;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kScores>
 __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_constant__ CUtensorMap map, DecodeArgs d) {
   using L = Layout<D>;
   extern __shared__ uint8_t raw[];
   __shared__ TileInfo s_info[L::kStages];
   __shared__ uint64_t s_full[L::kStages], s_empty[L::kStages];
-  __shared__ uint32_t s_scan[kThreads / 32], s_begin[2], s_gave_up;
+  __shared__ uint32_t s_scan[kThreads / 32], s_begin[2], s_gave_up, s_drained;
   __shared__ float2 s_ml[kWarps][kRows];
   const AttnArgs& a = d.a;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -100,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       mbar_init(smem_addr(&s_full[i]), 1);
       mbar_init(smem_addr(&s_empty[i]), kWarps);
     }
-    s_gave_up = 0;
+    s_gave_up = s_drained = 0;
     mbar_init_fence();
   }
   // Rows of the query area that no query fills must hold finite values.
@@ -154,7 +159,8 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     SeqInfo q = seq_info(a, s, prefix);
     bool fresh = true;  // the next tile is the first of its piece
     uint32_t pieces = 0;
-    for (uint32_t i = 0; i < count; ++i) {
+    uint32_t i = 0;
+    for (; i < count; ++i) {
       const uint32_t stage = i % L::kStages;
       const int tile = t < static_cast<uint32_t>(q.sink_tiles) ? t : q.first_tile + (t - q.sink_tiles);
       const int token = tile * kTile, end = min(token + kTile, q.len);
@@ -168,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       if (token + kTile - 1 > q.len - static_cast<int>(q.queries) ||
           (token < last_low && token + kTile > q.sinks))
         info.flags |= kMask;
-      mbar_wait_warp(smem_addr(&s_empty[stage]), (i / L::kStages & 1) ^ 1, &s_gave_up, a.status);
+      if (!mbar_wait_warp(smem_addr(&s_empty[stage]), (i / L::kStages & 1) ^ 1, &s_gave_up, a.status)) break;
       const uint32_t full = smem_addr(&s_full[stage]), at = base + stage * L::kStage;
       // lane: one box of the keys or values and one half of the head
       const uint32_t box = lane % boxes, half = lane / boxes % halves, plane = lane / boxes / halves;
@@ -205,17 +211,18 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       }
     }
     // No copy may be in flight when the CTA ends.
-    for (uint32_t i = count > L::kStages ? count - L::kStages : 0; i < count; ++i)
-      mbar_wait_warp(smem_addr(&s_full[i % L::kStages]), i / L::kStages & 1, &s_gave_up, a.status);
+    for (uint32_t k = i > L::kStages ? i - L::kStages : 0; k < i; ++k)
+      mbar_wait_warp(smem_addr(&s_full[k % L::kStages]), k / L::kStages & 1, &s_drained, a.status);
     return;
   }
 
   // ---- the consumers: rows lane / 4 and lane / 4 + 8, tokens 16 warp .. 16 warp + 15 of each tile
   uint32_t qf[D / 16][4];
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  bool alive = true;
   for (uint32_t i = 0; i < count; ++i) {
     const uint32_t stage = i % L::kStages, at = base + stage * L::kStage;
-    mbar_wait_warp(smem_addr(&s_full[stage]), i / L::kStages & 1, &s_gave_up, a.status);
+    alive = alive && mbar_wait_warp(smem_addr(&s_full[stage]), i / L::kStages & 1, &s_gave_up, a.status);
     const TileInfo info = s_info[stage];
     if (info.flags & kFirst) {
 #pragma unroll
@@ -267,6 +274,22 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
           const bool see = j <= pos && (a.window == 0 || j > pos - a.window || j < info.sinks);
           if (!see) z[n][e] = -INFINITY;
         }
+    }
+    if constexpr (kScores) {
+      const uint64_t column = a.page_offsets[info.seq] * a.page_tokens;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const uint32_t row = lane / 4 + 8 * r;
+        if (row < info.queries * a.group && row < d.score_rows && alive) {
+          float* to = d.scores + (static_cast<uint64_t>(head) * d.score_rows + row) * d.columns + column;
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            const int j = info.token + static_cast<int>(warp * 16 + n * 8 + lane % 4 * 2);
+            if (j < info.len)  // an even place: the pair's second is within the page
+              *reinterpret_cast<float2*>(to + j) = make_float2(z[n][2 * r] * a.scale_log2, z[n][2 * r + 1] * a.scale_log2);
+          }
+        }
+      }
     }
     uint32_t p[4];
     float scale[2];
@@ -346,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
           v.z += f * x.z;
           v.w += f * x.w;
         }
-        if (s_gave_up) continue;
+        if (!alive) continue;
         if (info.flags & kWhole) {
           const uint32_t t = info.q_first + r / a.group, h = head * a.group + r % a.group;
           const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
@@ -361,8 +384,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       }
       proxy_fence_smem();  // these accesses come before the copies of the next tile here
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(smem_addr(&s_empty[stage]));
+    mbar_arrive_warp(smem_addr(&s_empty[stage]), lane, alive);
   }
 }
 
@@ -411,17 +433,47 @@ __global__ void __launch_bounds__(128) decode_join_kernel(DecodeArgs d) {
   if (e == 0) store_lse(a, t, h, f);
 }
 
+// A token's softmax weights, of the scores that decode_kernel left: one thread for
+// each token and kv head, the rows in their order.
+__global__ void __launch_bounds__(256) decode_weights_kernel(DecodeArgs d) {
+  const AttnArgs& a = d.a;
+  const uint32_t s = blockIdx.z, head = blockIdx.y, q_first = a.q_offsets[s], queries = a.q_offsets[s + 1] - q_first;
+  __shared__ float s_lse[kRows];
+  const uint32_t rows = min(queries * a.group, d.score_rows);
+  if (rows == 0) return;
+  if (threadIdx.x < rows)
+    s_lse[threadIdx.x] = kLog2e * a.lse[(q_first + threadIdx.x / a.group) * static_cast<uint64_t>(a.kv_heads) * a.group +
+                                        head * a.group + threadIdx.x % a.group];
+  __syncthreads();
+  const SeqInfo q = seq_info(a, s, 0);
+  const uint64_t column = a.page_offsets[s] * a.page_tokens;
+  const float* z = d.scores + static_cast<uint64_t>(head) * d.score_rows * d.columns + column;
+  float* w = a.weights + head * a.weights_head_stride + column;
+  for (int j = static_cast<int>(blockIdx.x * 256 + threadIdx.x); j < q.len; j += static_cast<int>(gridDim.x * 256)) {
+    if (j < q.low && j >= q.sinks) continue;  // no row sees it, and no tile held it
+    float sum = 0.f;
+#pragma unroll 4
+    for (uint32_t r = 0; r < rows; ++r) {
+      const float lse = s_lse[r], x = z[r * d.columns + j];
+      sum += lse == -INFINITY ? 0.f : exp2f(x - lse);
+    }
+    w[j] += sum;
+  }
+}
+
 // Two CTAs fit an SM. A range holds one tile at least.
 uint32_t decode_ranges(const tcx_kv_attention_args& x) {
   const uint64_t tiles = x.total_pages * x.page_tokens / kTile + x.n_seq;
   return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(tiles, 2ull * sm_count() / x.kv_heads)));
 }
 
-template <typename T, int D>
-tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint32_t rows, cudaStream_t stream) {
+template <typename T, int D, bool kScores>
+tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint32_t rows, uint64_t max_tokens,
+                  cudaStream_t stream) {
   using L = Layout<D>;
-  TCX_CUDA_TRY(cudaFuncSetAttribute(decode_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
-  decode_kernel<T, D><<<d.ranges * d.a.kv_heads, kThreads, L::kBytes, stream>>>(map, d);
+  TCX_CUDA_TRY(
+      cudaFuncSetAttribute(decode_kernel<T, D, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+  decode_kernel<T, D, kScores><<<d.ranges * d.a.kv_heads, kThreads, L::kBytes, stream>>>(map, d);
   note_launches(1);
   TCX_CUDA_TRY(cudaGetLastError());
   if (d.ranges > 1) {
@@ -429,7 +481,25 @@ tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint32_t rows, cu
     note_launches(1);
     TCX_CUDA_TRY(cudaGetLastError());
   }
+  if (kScores && max_tokens > 0) {
+    const uint64_t blocks = std::min<uint64_t>((max_tokens + 255) / 256, 64);
+    decode_weights_kernel<<<dim3(static_cast<unsigned>(blocks), d.a.kv_heads, d.a.n_seq), 256, 0, stream>>>(d);
+    note_launches(1);
+    TCX_CUDA_TRY(cudaGetLastError());
+  }
   return TCX_OK;
+}
+
+template <typename T, int D>
+tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint32_t rows, uint64_t max_tokens,
+                  cudaStream_t stream) {
+  return d.scores != nullptr ? launch<T, D, true>(d, map, rows, max_tokens, stream)
+                             : launch<T, D, false>(d, map, rows, max_tokens, stream);
+}
+
+uint64_t score_bytes(const tcx_kv_attention_args& x) {
+  if (x.d_weights == nullptr) return 0;
+  return align256(x.max_q * x.q_heads * x.total_pages * x.page_tokens * sizeof(float));
 }
 
 }  // namespace
@@ -440,7 +510,8 @@ bool decode_fits(const tcx_kv_attention_args& x) {
 
 uint64_t decode_scratch_bytes(const tcx_kv_attention_args& x) {
   const uint64_t parts = decode_ranges(x) * 2ull * x.kv_heads * kRows;
-  return align256(decode_ranges(x) * sizeof(RangeInfo)) + align256(parts * sizeof(float2)) + parts * x.head_dim * 4;
+  return align256(decode_ranges(x) * sizeof(RangeInfo)) + align256(parts * sizeof(float2)) +
+         align256(parts * x.head_dim * 4) + score_bytes(x);
 }
 
 tcx_status launch_decode(const tcx_kv_attention_args& x, const AttnArgs& a, const CUtensorMap& map, void* scratch,
@@ -452,12 +523,18 @@ tcx_status launch_decode(const tcx_kv_attention_args& x, const AttnArgs& a, cons
   uint8_t* at = static_cast<uint8_t*>(scratch);
   d.info = reinterpret_cast<RangeInfo*>(at);
   d.part_ml = reinterpret_cast<float2*>(at += align256(d.ranges * sizeof(RangeInfo)));
-  d.part_o = reinterpret_cast<float*>(at + align256(parts * sizeof(float2)));
+  d.part_o = reinterpret_cast<float*>(at += align256(parts * sizeof(float2)));
   const uint32_t rows = static_cast<uint32_t>(x.max_q) * a.group;
+  if (x.d_weights != nullptr) {
+    d.scores = reinterpret_cast<float*>(at + align256(parts * x.head_dim * 4));
+    d.score_rows = rows;
+    d.columns = x.total_pages * x.page_tokens;
+  }
+  const uint64_t max_tokens = x.max_pages * x.page_tokens;
   if (x.dtype == TCX_KV_BF16)
-    return x.head_dim == 128 ? launch<__nv_bfloat16, 128>(d, map, rows, stream)
-                             : launch<__nv_bfloat16, 64>(d, map, rows, stream);
-  return x.head_dim == 128 ? launch<__half, 128>(d, map, rows, stream) : launch<__half, 64>(d, map, rows, stream);
+    return x.head_dim == 128 ? launch<__nv_bfloat16, 128>(d, map, rows, max_tokens, stream)
+                             : launch<__nv_bfloat16, 64>(d, map, rows, max_tokens, stream);
+  return x.head_dim == 128 ? launch<__half, 128>(d, map, rows, max_tokens, stream) : launch<__half, 64>(d, map, rows, max_tokens, stream);
 }
 
 }  // namespace tcx

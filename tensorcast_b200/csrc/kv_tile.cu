@@ -205,8 +205,9 @@ template <int D>
 struct TileLayout {
   static constexpr int kBlock = kTokens * 128;          // 64 values of 128 rows, swizzled
   static constexpr int kOperand = kBlock * (D / 64);    // 128 rows
-  static constexpr int kStages = D == 128 ? 5 : 8;
-  static constexpr int kBytes = (2 + kStages) * kOperand + 1024;
+  static constexpr int kStages = D == 128 ? 4 : 8;
+  static constexpr int kOut = 8 * 32 * 128;              // 128 bytes of each row, on their way out
+  static constexpr int kBytes = (2 + kStages) * kOperand + kOut + 1024;
   static constexpr uint32_t kScores = 0, kSums = 256, kColumns = 512;
 };
 
@@ -221,28 +222,33 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   constexpr uint32_t kStages = L::kStages;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t s_bar[2 * kStages + 10];
-  __shared__ uint32_t s_tmem, s_gave_up;
+  __shared__ uint32_t s_tmem, s_gave_up, s_drained;
   __shared__ __align__(16) int s_seen[2][8][4];
   const AttnArgs& a = d.a;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, range = blockIdx.x;
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u, ring = base + 2 * L::kOperand;
-  auto full = [&](uint32_t i) { return smem_addr(&s_bar[i]); };
-  auto empty = [&](uint32_t i) { return smem_addr(&s_bar[kStages + i]); };
-  auto bar = [&](uint32_t kind, uint32_t half) { return smem_addr(&s_bar[2 * kStages + kind * 2 + half]); };
+  // Ring place 2 i holds tile i's keys, 2 i + 1 its values. A tile's values and the
+  // next one's keys are waited for together (pair p: places 2 p - 1 and 2 p); each is
+  // given back by itself.
+  // As many pairs' barriers as places: the first lap's copies wait for no place, and
+  // must not arrive at a pair whose phase is still open.
+  constexpr uint32_t kPairs = kStages;
+  auto full = [&](uint32_t pair) { return smem_addr(&s_bar[pair % kPairs]); };
+  auto full_phase = [&](uint32_t pair) { return pair / kPairs & 1; };
+  auto empty = [&](uint32_t i) { return smem_addr(&s_bar[kPairs + i]); };
+  auto bar = [&](uint32_t kind, uint32_t half) { return smem_addr(&s_bar[kPairs + kStages + kind * 2 + half]); };
   enum : uint32_t { kQueries, kScored, kWeighed, kWeighedAll, kSummed };
   if (threadIdx.x == 0) {
-    for (uint32_t i = 0; i < kStages; ++i) {
-      mbar_init(full(i), 1);
-      mbar_init(empty(i), 1);
-    }
+    for (uint32_t i = 0; i < kPairs; ++i) mbar_init(full(i), 2);
+    for (uint32_t i = 0; i < kStages; ++i) mbar_init(empty(i), 1);
     for (uint32_t h = 0; h < 2; ++h) {
-      mbar_init(bar(kQueries, h), kHalfRows);
+      mbar_init(bar(kQueries, h), 4);  // a warp's lane for all of them
       mbar_init(bar(kScored, h), 1);
-      mbar_init(bar(kWeighed, h), kHalfRows);
-      mbar_init(bar(kWeighedAll, h), kHalfRows);
+      mbar_init(bar(kWeighed, h), 4);
+      mbar_init(bar(kWeighedAll, h), 4);
       mbar_init(bar(kSummed, h), 1);
     }
-    s_gave_up = 0;
+    s_gave_up = s_drained = 0;
     mbar_init_fence();
   }
   const uint32_t ranges = d.counts[1];
@@ -265,10 +271,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       const uint32_t box = lane % boxes, half = lane / boxes;
       uint32_t slot_at = 0;  // ring position
       Item it = d.items[item];
-      for (uint32_t left = count; left > 0;) {
+      if (lane == 0) mbar_arrive(full(0));  // no values before the first keys
+      bool alive = true;
+      for (uint32_t left = count; left > 0 && alive;) {
         const uint32_t n = min(it.tiles - at, left);
         const uint32_t* table = (d.prefix ? a.prefix_table : a.page_table) + it.table;
-        for (uint32_t j = 0; j < n; ++j) {
+        for (uint32_t j = 0; j < n && alive; ++j) {
           const int from = first_token(it, at + j) + static_cast<int>(box * a.box_rows),
                     to = from + static_cast<int>(a.box_rows);
           const bool wanted = half < D / 64 && from < it.limit && (to > it.low || from < it.sinks);
@@ -278,14 +286,16 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 #pragma unroll
           for (int plane = 0; plane < 2; ++plane, ++slot_at) {
             const uint32_t stage = slot_at % kStages;
-            mbar_wait_warp(empty(stage), (slot_at / kStages & 1) ^ 1, &s_gave_up, a.status);
+            alive = alive && mbar_wait_warp(empty(stage), (slot_at / kStages & 1) ^ 1, &s_gave_up, a.status);
+            if (!alive) break;
+            const uint32_t arrived = full((slot_at + 1) / 2);
             if (lane == 0) {
-              if (bytes) mbar_arrive_expect(full(stage), bytes); else mbar_arrive(full(stage));
+              if (bytes) mbar_arrive_expect(arrived, bytes); else mbar_arrive(arrived);
             }
             __syncwarp();
             if (wanted)
               tma_load_3d(ring + stage * L::kOperand + half * L::kBlock + box * a.box_rows * 128, &map, half * 64,
-                          head, static_cast<int>(row + (plane ? a.v_row0 : a.k_row0)), full(stage));
+                          head, static_cast<int>(row + (plane ? a.v_row0 : a.k_row0)), arrived);
           }
         }
         left -= n;
@@ -295,72 +305,99 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           it = d.items[++item];
         }
       }
+      const uint32_t last = slot_at / 2;
+      if (lane == 0 && alive) mbar_arrive(full(last));  // no keys behind the last values
       // No copy may be in flight when the CTA ends.
-      for (uint32_t i = slot_at > kStages ? slot_at - kStages : 0; i < slot_at; ++i)
-        mbar_wait_warp(full(i % kStages), i / kStages & 1, &s_gave_up, a.status);
-    } else if (warp == 8 && lane == 0) {  // ---- the products
+      for (uint32_t p = last > kStages / 2 ? last - kStages / 2 : 0; p <= last; ++p)
+        mbar_wait_warp(full(p), full_phase(p), &s_drained, a.status);
+    } else if (warp == 8) {  // ---- the products
       constexpr uint32_t kScoreShape = mma_shape<T>(kTokens, false), kValueShape = mma_shape<T>(D, true);
+      const uint32_t tm = __shfl_sync(~0u, tmem, 0);
+      const uint64_t q_operand = smem_operand(base, 16, 1024), k_operand = smem_operand(ring, 16, 1024),
+                     v_operand = smem_operand(ring, L::kBlock, 1024);
       uint32_t slot_at = 0, pieces[2] = {0, 0}, done[2] = {0, 0};
       auto wait = [&](uint32_t b, uint32_t phase) {
-        mbar_wait(b, phase & 1, &s_gave_up, a.status);
+        const bool there = mbar_wait_warp(b, phase & 1, &s_gave_up, a.status);
         tmem_fence_after();
+        return there;
       };
-      auto score = [&](uint32_t h, uint32_t slot) {  // scores of half h: its queries x the keys at `slot`
-        const uint32_t q = base + h * L::kOperand, k = ring + slot % kStages * L::kOperand;
+      // Scores of half h: its queries x the keys at `slot`. An operand's place is its
+      // descriptor's low bits, in 16-byte units.
+      auto score = [&](uint32_t h, uint32_t slot) {
+        const uint64_t q = q_operand + h * (L::kOperand / 16), k = k_operand + slot % kStages * (L::kOperand / 16);
+        if (elect_one()) {
 #pragma unroll
-        for (int e = 0; e < D / 16; ++e)
-          mma_ss(tmem + L::kScores + h * kTokens, smem_operand(q + e / 4 * L::kBlock + e % 4 * 32, 16, 1024),
-                 smem_operand(k + e / 4 * L::kBlock + e % 4 * 32, 16, 1024), kScoreShape, e > 0);
-        mma_commit(bar(kScored, h));
+          for (int e = 0; e < D / 16; ++e) {
+            const uint32_t off = e / 4 * (L::kBlock / 16) + e % 4 * 2;
+            mma_ss(tm + L::kScores + h * kTokens, q + off, k + off, kScoreShape, e > 0);
+          }
+          mma_commit(bar(kScored, h));
+        }
+        __syncwarp();
       };
       // Sums of half h: its probabilities x the values. The last quarter of the
       // probabilities follows the others.
-      auto value = [&](uint32_t h, uint32_t slot, bool add) {
-        const uint32_t v = ring + slot % kStages * L::kOperand, phase = done[h]++;
-        wait(bar(kWeighed, h), phase);
+      auto value = [&](uint32_t h, uint32_t slot, bool add, bool last) {
+        const uint64_t v = v_operand + slot % kStages * (L::kOperand / 16);
+        const uint32_t phase = done[h]++;
+        constexpr int kSteps = kTokens / 16, kEarly = kSteps * 3 / 4;
+        auto steps = [&](int from, int to) {
 #pragma unroll
-        for (int j = 0; j < kTokens / 16; ++j) {
-          if (j == kTokens / 16 * 3 / 4) wait(bar(kWeighedAll, h), phase);
-          mma_ts(tmem + L::kSums + h * D, tmem + L::kScores + h * kTokens + j * 8,
-                 smem_operand(v + j * 16 * 128, L::kBlock, 1024), kValueShape, add || j > 0);
+          for (int j = from; j < to; ++j)
+            mma_ts(tm + L::kSums + h * D, tm + L::kScores + h * kTokens + j * 8, v + j * 128, kValueShape, add || j > 0);
+        };
+        if (!wait(bar(kWeighed, h), phase)) return false;
+        if (elect_one()) steps(0, kEarly);
+        __syncwarp();
+        if (!wait(bar(kWeighedAll, h), phase)) return false;
+        if (elect_one()) {
+          steps(kEarly, kSteps);
+          if (last) mma_commit(bar(kSummed, h));
         }
-        mma_commit(bar(kSummed, h));
+        __syncwarp();
+        return true;
       };
-      uint32_t tiles = d.items[item].tiles, rows = d.items[item].rows;
+      auto release = [&](uint32_t slot) {
+        if (elect_one()) mma_commit(empty(slot % kStages));
+        __syncwarp();
+      };
+      auto uniform = [&](uint32_t x) { return __shfl_sync(~0u, x, 0); };
+      uint32_t tiles = uniform(d.items[item].tiles), rows = uniform(d.items[item].rows);
       uint32_t next = min(item + 1, items - 1), next_tiles = d.items[next].tiles, next_rows = d.items[next].rows;
-      for (uint32_t left = count; left > 0;) {
+      at = uniform(at);
+      head = uniform(head);
+      for (uint32_t left = uniform(count); left > 0;) {
         const uint32_t n = min(tiles - at, left);
         const bool two = rows > kHalfRows;
-        wait(bar(kQueries, 0), pieces[0]++);
-        wait(full(slot_at % kStages), slot_at / kStages);
+        bool alive = wait(bar(kQueries, 0), pieces[0]++) && wait(full(slot_at / 2), full_phase(slot_at / 2));
+        if (!alive) break;
         score(0, slot_at);
         if (two) {
-          wait(bar(kQueries, 1), pieces[1]++);
+          if (!wait(bar(kQueries, 1), pieces[1]++)) break;
           score(1, slot_at);
         }
-        mma_commit(empty(slot_at % kStages));
+        release(slot_at);
         for (uint32_t j = 0; j < n; ++j, slot_at += 2) {
           const uint32_t v = slot_at + 1, k = slot_at + 2;
           const bool more = j + 1 < n;
-          wait(full(v % kStages), v / kStages);
-          value(0, v, j > 0);
-          if (more) {
-            wait(full(k % kStages), k / kStages);
-            score(0, k);
-          }
-          if (two) value(1, v, j > 0);
-          mma_commit(empty(v % kStages));
+          alive = wait(full(k / 2), full_phase(k / 2)) && value(0, v, j > 0, !more);  // both places are there
+          if (!alive) break;
+          if (more) score(0, k);
+          if (two) alive = value(1, v, j > 0, !more);
+          if (!alive) break;
+          release(v);
           if (more) {
             if (two) score(1, k);
-            mma_commit(empty(k % kStages));
+            release(k);
           }
         }
+        if (!alive) break;
         left -= n;
         at = 0;
         if (++head == a.kv_heads) {
           head = 0;
-          tiles = next_tiles;
-          rows = next_rows;
+          tiles = uniform(next_tiles);
+          rows = uniform(next_rows);
           next = min(next + 1, items - 1);
           next_tiles = d.items[next].tiles;
           next_rows = d.items[next].rows;
@@ -370,46 +407,52 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     __syncwarp();
   } else {  // ---- the softmax of half `h`, one thread for each row
     asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    // A warp moves its 32 rows' queries in, and outputs out, with kLanes lanes to a row.
-    constexpr uint32_t kLanes = D / 8, kMoves = kLanes;
     const uint32_t h = warp / 4, r = threadIdx.x, quarter = warp % 4 * 32 << 16;
     const uint32_t scores = tmem + quarter + L::kScores + h * kTokens, sums = tmem + quarter + L::kSums + h * D;
-    const uint32_t own = base + h * L::kOperand + warp % 4 * 32 * 128;  // the warp's rows in shared memory
-    auto place = [&](uint32_t row, uint32_t c) {  // 16-byte piece c of a row, swizzled as the products read it
-      return own + c / 8 * L::kBlock + row * 128 + ((c % 8 ^ (row & 7)) << 4);
-    };
+    const uint32_t staged = base + (2 + kStages) * L::kOperand + warp * 4096;
     const int prefix = static_cast<int>(prefix_length(a));
-    uint32_t pieces = 0, done = 0, tiles_done = 0, t, q_head;
-    Item it = d.items[item];
-    uint4 q[kMoves];
-    auto fetch = [&] {  // this piece's row, and its warp's queries from global memory
-      const uint32_t row = it.row0 + r;
-      t = it.q_first + row / a.group;
-      q_head = head * a.group + row % a.group;
-      const uint64_t from = t * a.q_token_stride + q_head * a.q_head_stride;
+    uint32_t pieces = 0, done = 0, summed = 0, tiles_done = 0;
+    bool alive = true;
+    auto wait = [&](uint32_t b, uint32_t phase) { alive = alive && mbar_wait_warp(b, phase & 1, &s_gave_up, a.status); };
+    // Starts the copies of this warp's 32 queries of a piece, D / 8 lanes to a row,
+    // swizzled as the products read them.
+    auto fetch = [&](uint32_t q_first, uint32_t row0, uint32_t rows, uint32_t kv_head) {
+      constexpr uint32_t kLanes = D / 8;
+      const uint32_t row = row0 + r, first = r & ~31u;
+      const uint64_t from = (q_first + row / a.group) * a.q_token_stride +
+                            (kv_head * a.group + row % a.group) * a.q_head_stride;
 #pragma unroll
-      for (uint32_t i = 0; i < kMoves; ++i) {
-        const uint32_t src = i * (32 / kLanes) + lane / kLanes;
+      for (uint32_t i = 0; i < kLanes; ++i) {
+        const uint32_t src = i * (32 / kLanes) + lane / kLanes, c = lane % kLanes, mine = first + src;
+        const bool valid = mine < rows;
         const uint64_t at_row = __shfl_sync(~0u, from, src);
-        q[i] = (r & ~31u) + src < it.rows ? *reinterpret_cast<const uint4*>(a.q + at_row + lane % kLanes * 16)
-                                          : make_uint4(0, 0, 0, 0);
+        async_copy16(base + h * L::kOperand + c / 8 * L::kBlock + mine % kHalfRows * 128 + ((c % 8 ^ (mine & 7)) << 4),
+                     a.q + (valid ? at_row + c * 16 : 0), valid ? 16 : 0);
       }
     };
-    fetch();
+    Item it = d.items[item];
+    if (h * kHalfRows < it.rows) fetch(it.q_first, it.row0, it.rows, head);
     for (uint32_t left = count; left > 0; ++pieces) {
       const uint32_t n = min(it.tiles - at, left);
       const uint32_t row = it.row0 + r;
       const bool active = h * kHalfRows < it.rows;
       if (active) {
-#pragma unroll
-        for (uint32_t i = 0; i < kMoves; ++i)
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                           place(i * (32 / kLanes) + lane / kLanes, lane % kLanes)),
-                       "r"(q[i].x), "r"(q[i].y), "r"(q[i].z), "r"(q[i].w)
-                       : "memory");
+        async_copies_done();
         proxy_fence_smem();
-        mbar_arrive(bar(kQueries, h));
+        mbar_arrive_warp(bar(kQueries, h), lane, alive);
       }
+      // The next piece's queries follow once this one's last scores are there.
+      auto fetch_next = [&] {
+        if (left == n) return;
+        if (head + 1 < a.kv_heads) {
+          if (active) fetch(it.q_first, it.row0, it.rows, head + 1);
+        } else {
+          const Item& next = d.items[item + 1];
+          const uint32_t rows = next.rows;
+          if (h * kHalfRows < rows) fetch(next.q_first, next.row0, rows, 0);
+        }
+      };
+      if (!active) fetch_next();
       // What this row sees: [0, hi] from lo on, and the sinks. What all rows of this
       // half see (all_*), and what any row of the item sees (any_*).
       int hi = -1, lo = 0, all_hi, all_lo, any_hi, any_lo;
@@ -418,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       };
       if (d.prefix) {
         if (r < it.rows) {
-          const uint32_t s = seq_of(a, t);
+          const uint32_t t = it.q_first + row / a.group, s = seq_of(a, t);
           const int nq = static_cast<int>(a.q_offsets[s + 1] - a.q_offsets[s]);
           const int pos = prefix + static_cast<int>(seq_length(a, s)) - nq + static_cast<int>(t - a.q_offsets[s]);
           hi = min(pos, prefix - 1);
@@ -453,8 +496,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       if (active) {
         for (uint32_t j = 0; j < n; ++j, ++done) {
           const int token = first_token(it, at + j);
-          mbar_wait_warp(bar(kScored, h), done & 1, &s_gave_up, a.status);
+          wait(bar(kScored, h), done);
           tmem_fence_after();
+          if (j + 1 == n) fetch_next();
           uint32_t z[kTokens];
           tmem_load128(z, scores);
           bool plain = true;
@@ -472,104 +516,106 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
               for (int i = 0; i < 32; ++i)
                 if (!(see >> i & 1)) z[w * 32 + i] = 0xff800000u;
             }
-          }
-          float top2[2] = {-INFINITY, -INFINITY};
+            // values that no row sees are cleared: 0 x NaN is not 0
+            if (h == 0 && (token + kTokens - 1 > any_hi || (token < any_lo && token + kTokens > it.sinks))) {
+              const uint32_t v = 2 * (tiles_done + j) + 1;
+              wait(full((v + 1) / 2), full_phase((v + 1) / 2));
+              const int mine = token + static_cast<int>(r);
+              if (mine > any_hi || (mine < any_lo && mine >= it.sinks)) {
+                const uint32_t to = ring + v % kStages * L::kOperand + r * 128;
 #pragma unroll
-          for (int i = 0; i < kTokens; i += 2)
-            top2[i / 2 % 2] = max3_nan(top2[i / 2 % 2], __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
-          const float top = max3_nan(top2[0], top2[1], top2[0]) * a.scale_log2;
-          plain = plain && !__any_sync(~0u, !(fabsf(top) < INFINITY));
-          const bool grown = top > m + 8.f;
-          if (__any_sync(~0u, grown)) {
-            const float old = m;
-            if (grown) m = top;
-            const float f = grown ? exp2_approx(old - m) : 1.f;
-            l *= f;
-            if (j > 0) {
-              mbar_wait_warp(bar(kSummed, h), (done - 1) & 1, &s_gave_up, a.status);
-              tmem_fence_after();
-              for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_load32(o, sums + c);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                tmem_store32(sums + c, o);
+                for (int c = 0; c < D / 8; ++c)
+                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + c / 8 * L::kBlock +
+                                                                               ((c % 8 ^ (r & 7)) << 4)),
+                               "r"(0)
+                               : "memory");
               }
+              proxy_fence_smem();
+              __syncwarp();
             }
           }
-          // values that no row sees are cleared: 0 x NaN is not 0
-          if (h == 0 && (token + kTokens - 1 > any_hi || (token < any_lo && token + kTokens > it.sinks))) {
-            const uint32_t v = 2 * (tiles_done + j) + 1;
-            mbar_wait_warp(full(v % kStages), v / kStages & 1, &s_gave_up, a.status);
-            const int mine = token + static_cast<int>(r);
-            if (mine > any_hi || (mine < any_lo && mine >= it.sinks)) {
-              const uint32_t to = ring + v % kStages * L::kOperand + r * 128;
+          auto largest = [&] {
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-              for (int c = 0; c < D / 8; ++c)
-                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + c / 8 * L::kBlock + ((c % 8 ^ (r & 7)) << 4)),
-                             "r"(0)
-                             : "memory");
-            }
-            proxy_fence_smem();
-            __syncwarp();
-          }
-          const float ref = m == -INFINITY ? 0.f : m;
-          const float2 c2 = make_float2(a.scale_log2, a.scale_log2), ref2 = make_float2(-ref, -ref);
-          float2 sum[2] = {};
-          // Every fourth pair's exponentials run on the FMA units: the exponential
-          // units alone need as long as the products do.
-          auto weigh = [&](auto mixed) {
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t p[16];
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const int k = c * 32 + 2 * i;
-                float2 x = fma2(make_float2(__uint_as_float(z[k]), __uint_as_float(z[k + 1])), c2, ref2);
-                if (decltype(mixed)::value && i % 4 == 3) {
-                  x = exp2_fma(x);
-                } else {
-                  x.x = exp2_approx(x.x);
-                  x.y = exp2_approx(x.y);
-                }
-                sum[i % 2] = add2(sum[i % 2], x);
-                p[i] = pack2<T>(x.x, x.y);
-              }
-              tmem_store16(scores + c * 16, p);
-              if (c >= 2) {
-                tmem_wait_store();
-                tmem_fence_before();
-                mbar_arrive(bar(c == 2 ? kWeighed : kWeighedAll, h));
-              }
-            }
+            for (int i = 0; i < kTokens; i += 2)
+              top[i / 2 % 4] = max3_nan(top[i / 2 % 4], __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
+            return max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
           };
-          if (plain) weigh(std::true_type{}); else weigh(std::false_type{});
+          const float2 c2 = make_float2(a.scale_log2, a.scale_log2);
+          float2 sum[2];
+          // Probabilities of 32 tokens, in place of their scores. Mixed: every eighth
+          // pair's exponentials run on the FMA units, since the exponential units
+          // alone need as long as the products do.
+          auto weigh = [&](int c, auto mixed) {
+            const float ref = m == -INFINITY ? 0.f : m;
+            const float2 ref2 = make_float2(-ref, -ref);
+            uint32_t p[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int k = c * 32 + 2 * i;
+              float2 x = fma2(make_float2(__uint_as_float(z[k]), __uint_as_float(z[k + 1])), c2, ref2);
+              if (decltype(mixed)::value && i % 8 == 7) {
+                x = exp2_fma(x);
+              } else {
+                x.x = exp2_approx(x.x);
+                x.y = exp2_approx(x.y);
+              }
+              sum[i % 2] = add2(sum[i % 2], x);
+              p[i] = pack2<T>(x.x, x.y);
+            }
+            tmem_store16(scores + c * 16, p);
+          };
+          // A tile that all rows see whole is weighed by the maximum so far at once,
+          // while its own is found; it is weighed again where that has grown too far.
+          bool again = true;
+          float top;
+          if (plain && !__any_sync(~0u, m == -INFINITY)) {
+            sum[0] = sum[1] = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < 3; ++c) weigh(c, std::true_type{});
+            top = largest();
+            again = __any_sync(~0u, !(top <= m + 8.f));
+          } else {
+            top = largest();
+          }
+          if (again) {
+            const bool grown = top > m + 8.f;
+            if (__any_sync(~0u, grown)) {
+              const float old = m;
+              if (grown) m = top;
+              const float f = grown ? exp2_approx(old - m) : 1.f;
+              l *= f;
+              if (j > 0) {  // these scores are there, so the sums before them are done
+                for (int c = 0; c < D; c += 32) {
+                  uint32_t o[32];
+                  tmem_load32(o, sums + c);
+#pragma unroll
+                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                  tmem_store32(sums + c, o);
+                }
+              }
+            }
+            sum[0] = sum[1] = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int c = 0; c < 3; ++c) weigh(c, std::false_type{});
+          }
+          tmem_wait_store();
+          tmem_fence_before();
+          mbar_arrive_warp(bar(kWeighed, h), lane, alive);
+          weigh(3, std::false_type{});
+          tmem_wait_store();
+          tmem_fence_before();
+          mbar_arrive_warp(bar(kWeighedAll, h), lane, alive);
           sum[0] = add2(sum[0], sum[1]);
           l += sum[0].x + sum[0].y;
         }
-      }
-      const bool whole = at == 0 && n == it.tiles, final = whole && a.part_o == nullptr;
-      const bool write = active && r < it.rows && !s_gave_up;
-      // rows of this warp that are written
-      const uint32_t first_row = r & ~31u, rows = active && !s_gave_up && first_row < it.rows ? min(it.rows - first_row, 32u) : 0;
-      const uint64_t q_row = static_cast<uint64_t>(t) * a.kv_heads * a.group + q_head;
-      const uint64_t part = static_cast<uint64_t>(range * 2 + (pieces > 0)) * kRows + r;
-      const uint64_t out_at = t * a.out_token_stride + q_head * a.out_head_stride;
-      if (threadIdx.x == 0 && left == n)
-        d.end[range] = RangeEnd{item, head, at == 0, at + n < it.tiles, pieces > 0};
-      left -= n;
-      tiles_done += n;
-      at = 0;
-      if (left > 0) {  // the next piece's queries are on their way while this one's output leaves
-        if (++head == a.kv_heads) {
-          head = 0;
-          it = d.items[++item];
-        }
-        fetch();
-      }
-      if (active) {
-        mbar_wait_warp(bar(kSummed, h), (done - 1) & 1, &s_gave_up, a.status);
+        wait(bar(kSummed, h), summed++);
         tmem_fence_after();
+        const bool whole = at == 0 && n == it.tiles, final = whole && a.part_o == nullptr;
+        const bool write = r < it.rows && alive;
+        const uint32_t t = it.q_first + row / a.group, q_head = head * a.group + row % a.group;
+        const uint64_t q_row = static_cast<uint64_t>(t) * a.kv_heads * a.group + q_head;
+        const uint64_t part = static_cast<uint64_t>(range * 2 + (pieces > 0)) * kRows + r;
         Finish f{};
         if (write && whole) {
           f = finish_row(a, q_row, m, l);
@@ -578,76 +624,81 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           d.part_ml[part] = make_float2(m, l);
         }
         __syncwarp();
-        // The rows leave through the queries' place in shared memory, which the
-        // products have read.
-#pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
+        const uint64_t to = !write ? 0
+                            : final ? reinterpret_cast<uint64_t>(a.out + t * a.out_token_stride + q_head * a.out_head_stride)
+                            : whole ? reinterpret_cast<uint64_t>(a.part_o + q_row * D)
+                                    : reinterpret_cast<uint64_t>(d.part_o + part * D);
+        // 32 values of the row, a finished one's with its factors
+        auto values = [&](float (&x)[32], int c) {
           uint32_t o[32];
           tmem_load32(o, sums + c);
-          float x[32];
 #pragma unroll
           for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(o[i]);
-          if (whole) {
+          if (!whole) return;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) x[i] = f.own == 0.f ? 0.f : x[i] * f.own;  // nothing seen: 0
-            if (f.prior != 0.f) {
-              const float4* y = reinterpret_cast<const float4*>(a.prior_o + q_row * D + c);
+          for (int i = 0; i < 32; ++i) x[i] = f.own == 0.f ? 0.f : x[i] * f.own;  // nothing seen: 0
+          if (f.prior != 0.f) {
+            const float4* y = reinterpret_cast<const float4*>(a.prior_o + q_row * D + c);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 v = y[i];
-                x[4 * i] += f.prior * v.x;
-                x[4 * i + 1] += f.prior * v.y;
-                x[4 * i + 2] += f.prior * v.z;
-                x[4 * i + 3] += f.prior * v.w;
-              }
+            for (int i = 0; i < 8; ++i) {
+              const float4 v = y[i];
+              x[4 * i] += f.prior * v.x;
+              x[4 * i + 1] += f.prior * v.y;
+              x[4 * i + 2] += f.prior * v.z;
+              x[4 * i + 3] += f.prior * v.w;
             }
           }
-          if (final) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, c / 8 + i)),
-                           "r"(pack2<T>(x[8 * i], x[8 * i + 1])), "r"(pack2<T>(x[8 * i + 2], x[8 * i + 3])),
-                           "r"(pack2<T>(x[8 * i + 4], x[8 * i + 5])), "r"(pack2<T>(x[8 * i + 6], x[8 * i + 7]))
-                           : "memory");
-          } else {
-            // 32 values of each row, 128 bytes, in the first block
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, i)),
-                           "f"(x[4 * i]), "f"(x[4 * i + 1]), "f"(x[4 * i + 2]), "f"(x[4 * i + 3])
-                           : "memory");
-            __syncwarp();
-            float* to = whole ? a.part_o + q_row * D : d.part_o + part * D;
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-              const uint32_t src = i * 4 + lane / 8;
-              float* at_row = reinterpret_cast<float*>(__shfl_sync(~0u, reinterpret_cast<uint64_t>(to), src));
-              uint4 v;
-              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                           : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                           : "r"(place(src, lane % 8))
-                           : "memory");
-              if (src < rows) *reinterpret_cast<uint4*>(at_row + c + lane % 8 * 4) = v;
-            }
-            __syncwarp();
-          }
-        }
-        if (final) {
+          __syncwarp();
+        };
+        // 128 bytes of each of the warp's rows go through shared memory, so that 8
+        // lanes write one row's.
+        auto place = [&](uint32_t of, uint32_t c) { return staged + of * 128 + ((c ^ (of & 7)) << 4); };
+        auto leave = [&](uint32_t byte) {
           __syncwarp();
 #pragma unroll
-          for (uint32_t i = 0; i < kMoves; ++i) {
-            const uint32_t src = i * (32 / kLanes) + lane / kLanes;
-            const uint64_t at_row = __shfl_sync(~0u, out_at, src);
+          for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t src = i * 4 + lane / 8;
+            const uint64_t at_row = __shfl_sync(~0u, to, src);
             uint4 v;
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                          : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                         : "r"(place(src, lane % kLanes))
+                         : "r"(place(src, lane % 8))
                          : "memory");
-            if (src < rows) *reinterpret_cast<uint4*>(a.out + at_row + lane % kLanes * 16) = v;
+            if (at_row) *reinterpret_cast<uint4*>(at_row + byte + lane % 8 * 16) = v;
           }
           __syncwarp();
+        };
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float x[32];
+          values(x, c);
+          if (final) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, c % 64 / 8 + i)),
+                           "r"(pack2<T>(x[8 * i], x[8 * i + 1])), "r"(pack2<T>(x[8 * i + 2], x[8 * i + 3])),
+                           "r"(pack2<T>(x[8 * i + 4], x[8 * i + 5])), "r"(pack2<T>(x[8 * i + 6], x[8 * i + 7]))
+                           : "memory");
+            if (c % 64 == 32) leave((c - 32) * 2);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(place(lane, i)), "f"(x[4 * i]),
+                           "f"(x[4 * i + 1]), "f"(x[4 * i + 2]), "f"(x[4 * i + 3])
+                           : "memory");
+            leave(c * 4);
+          }
         }
         tmem_fence_before();
+      }
+      left -= n;
+      tiles_done += n;
+      if (left == 0 && threadIdx.x == 0)
+        d.end[range] = RangeEnd{item, head, at == 0, at + n < it.tiles, pieces > 0};
+      at = 0;
+      if (++head == a.kv_heads && left > 0) {
+        head = 0;
+        it = d.items[++item];
       }
     }
   }

@@ -32,6 +32,12 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// One arrival for the whole warp, unless a wait of it ran out.
+__device__ __forceinline__ void mbar_arrive_warp(uint32_t bar, uint32_t lane, bool alive) {
+  __syncwarp();
+  if (lane == 0 && alive) mbar_arrive(bar);
+}
+
 __device__ __forceinline__ void mbar_arrive_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
@@ -48,28 +54,22 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
-// Waits for the phase of this parity. A wait that runs out records it, in the
-// CTA's `gave_up` and the call's status, and from then on no wait of the CTA
-// waits: its loops run to their ends, and nothing is stored.
-__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up,
-                                          uint32_t* status) {
-  if (mbar_try(bar, parity)) return;
+// A whole warp waits for the phase of this parity. False where the wait ran out, in
+// this warp or another one of the CTA: that is recorded in the CTA's `gave_up` and the
+// call's status. The warp then arrives nowhere and issues nothing more (an arrival
+// out of turn is a fault), and nothing is stored.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up,
+                                               uint32_t* status) {
+  if (__all_sync(~0u, mbar_try(bar, parity))) return true;
   const long long start = clock64();
-  while (!mbar_try(bar, parity)) {
-    if (*gave_up) return;
+  while (!__all_sync(~0u, mbar_try(bar, parity))) {
     if (clock64() - start > kWaitClocks) {
       *gave_up = 1;
       atomicCAS(status, 0u, kWaitExpired);
-      return;
     }
+    if (__any_sync(~0u, *gave_up)) return false;
   }
-}
-
-// The same for a whole warp, whose lanes go on together.
-__device__ __forceinline__ void mbar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* gave_up,
-                                               uint32_t* status) {
-  mbar_wait(bar, parity, gave_up, status);
-  __syncwarp();
+  return true;
 }
 
 __device__ __forceinline__ void proxy_fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -87,6 +87,13 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
 }
+
+// 16 bytes, of which the first `bytes` are read and the others are 0.
+__device__ __forceinline__ void async_copy16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void async_copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -151,6 +158,16 @@ __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fenc
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// True in one lane of the (whole) warp, always the same one. Products are issued
+// under this: 64 cycles for each of 128 x 128 x 16, the tensor cores' rate. With a
+// condition on the lane number instead, the operands go through vector registers
+// and issuing takes 68 cycles alone and 100 to 130 beside busy warps (measured).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 // All products issued before by this thread arrive at the barrier when they are done.
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -171,20 +188,20 @@ __device__ __forceinline__ constexpr uint32_t mma_shape(uint32_t n, bool across)
   return 1u << 4 | type << 7 | type << 10 | (across ? 1u << 16 : 0u) | n / 8 << 17 | 128 / 16 << 24;
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add))
+      "l"(a), "l"(b), "r"(shape), "r"(add)
       : "memory");
 }
 
 // a in tensor memory
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, uint32_t add) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(shape), "r"(static_cast<uint32_t>(add))
+      "r"(a), "l"(b), "r"(shape), "r"(add)
       : "memory");
 }
 
