@@ -553,6 +553,7 @@ tcx_status tcx_kv_gather(const void* d_pool, uint32_t planes, uint64_t pool_page
 
 #define TCX_KV_BF16 0
 #define TCX_KV_FP16 1
+#define TCX_KV_COUNTERS 2048 /* 32-bit words a call needs beside its scratch */
 
 /* One attention call. Sequence s has len = d_seq_tokens[s] tokens in its pages
  * and nq = d_q_offsets[s+1] - d_q_offsets[s] query tokens, its newest ones: query
@@ -592,6 +593,8 @@ typedef struct tcx_kv_attention_args {
   float* d_weights;               /* NULL, or accumulators: see below */
   uint64_t weights_head_stride;   /* in elements */
   uint32_t* d_status;             /* zero before the first call */
+  uint32_t* d_counters;           /* TCX_KV_COUNTERS words, zero before the first call, which every
+                                     call leaves at zero (not one that ended with status 4) */
 } tcx_kv_attention_args;
 
 /* Scratch of a call with these sizes (pointers are not looked at). */
@@ -606,7 +609,8 @@ uint64_t tcx_kv_attention_scratch_bytes(const tcx_kv_attention_args* args);
  * touched. Table entries are checked on the device: a bad one leaves a non-zero
  * code in *d_status (1 slot out of the pool, 2 more tokens than the pages hold;
  * 4: a wait inside the kernel ran out) and nothing outside the pool is read; the rows of that sequence are then not
- * meaningful. A call with the same scratch must have ended. Values of tokens that
+ * meaningful. Calls that may run at the same time need their own scratch and
+ * counters. Values of tokens that
  * none of a sequence's queries sees are never used, whatever they hold; a
  * non-finite value of a token that some of them see may reach the others. */
 tcx_status tcx_kv_attention(const tcx_kv_attention_args* args, void* d_scratch, uint64_t scratch_bytes, void* stream);

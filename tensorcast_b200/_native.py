@@ -99,13 +99,16 @@ class FileStage(ctypes.Structure):
                 ("ring_slots", _c.c_int), ("slot_bytes", _c.c_uint64)]
 
 
+KV_COUNTERS = 2048
+
+
 class KvAttentionArgs(ctypes.Structure):
     _fields_ = [(n, _c.c_double if n == "scale" else _c.c_void_p if n.startswith("d_") else _c.c_uint64) for n in (
         "d_pool", "planes", "pool_pages", "page_tokens", "kv_heads", "q_heads", "head_dim", "dtype", "k_plane",
         "v_plane", "d_page_table", "d_page_offsets", "d_seq_tokens", "n_seq", "d_q_offsets", "q_tokens", "max_q",
         "total_pages", "max_pages", "d_prefix_table", "prefix_pages", "d_prefix_tokens", "window", "sinks", "scale",
         "d_q", "q_token_stride", "q_head_stride", "d_out", "out_token_stride", "out_head_stride", "d_lse",
-        "d_weights", "weights_head_stride", "d_status")]
+        "d_weights", "weights_head_stride", "d_status", "d_counters")]
 
 
 class KvEvictArgs(ctypes.Structure):

@@ -49,7 +49,8 @@ tcx_status check_sizes(const tcx_kv_attention_args& a) {
 
 tcx_status check(const tcx_kv_attention_args& a) {
   if (a.d_pool == nullptr || a.d_page_offsets == nullptr || a.d_seq_tokens == nullptr ||
-      a.d_q_offsets == nullptr || a.d_q == nullptr || a.d_out == nullptr || a.d_lse == nullptr || a.d_status == nullptr)
+      a.d_q_offsets == nullptr || a.d_q == nullptr || a.d_out == nullptr || a.d_lse == nullptr || a.d_status == nullptr ||
+      a.d_counters == nullptr)
     return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
   if (a.d_page_table == nullptr && a.total_pages != 0) return set_error(TCX_INVALID_ARGUMENT, "null device pointer");
   if (const tcx_status st = check_sizes(a); st != TCX_OK) return st;
@@ -105,6 +106,7 @@ AttnArgs device_args(const tcx_kv_attention_args& x) {
   a.weights = x.d_weights;
   a.weights_head_stride = x.weights_head_stride;
   a.status = x.d_status;
+  a.counters = x.d_counters;
   a.box_rows = std::min<uint32_t>(64, a.page_tokens & -a.page_tokens);
   a.k_row0 = x.k_plane * x.pool_pages * x.page_tokens;
   a.v_row0 = x.v_plane * x.pool_pages * x.page_tokens;

@@ -1,6 +1,8 @@
 // Arguments and lookups shared by the attention kernels over the paged KV pool.
 #pragma once
 
+#include <atomic>
+
 #include "sm100.cuh"
 #include "tcx_internal.h"
 
@@ -32,6 +34,7 @@ struct AttnArgs {
   float* weights;
   uint64_t weights_head_stride;
   uint32_t* status;
+  uint32_t* counters;  // TCX_KV_COUNTERS, all 0 between launches
   // Where there is a shared prefix: the rows' parts over it (o normalised, lse in
   // powers of two, [q token][q head]) are written to `part` and then read as `prior`.
   float *part_o, *part_lse;
@@ -147,6 +150,29 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, uint32_t t, uint32_
 __device__ __forceinline__ void store_lse(const AttnArgs& a, uint32_t t, uint32_t h, const Finish& f) {
   const uint64_t row = static_cast<uint64_t>(t) * a.kv_heads * a.group + h;
   if (a.part_o != nullptr) a.part_lse[row] = f.lse; else a.lse[row] = kLn2 * f.lse;
+}
+
+// The last of `parts` CTAs to come here, all of whose writes the others' precede;
+// it leaves the counter at 0 for the next call.
+__device__ __forceinline__ bool last_to_arrive(uint32_t* counter, uint32_t parts) {
+  __threadfence();
+  const bool last = atomicAdd(counter, 1u) + 1 == parts;
+  if (last) {
+    *counter = 0;
+    __threadfence();
+  }
+  return last;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory, once for each device.
+inline tcx_status allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  TCX_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done->load(std::memory_order_relaxed) & bit)) return TCX_OK;
+  TCX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done->fetch_or(bit, std::memory_order_relaxed);
+  return TCX_OK;
 }
 
 inline uint64_t align256(uint64_t n) { return (n + 255) / 256 * 256; }

@@ -13,8 +13,8 @@
 // maximum and sum in 32 bits, probabilities rounded to the input type (half a step,
 // as the output is) for the second product, sums in 32 bits. Where a sequence ends
 // inside a range the four warps' parts are joined in the tile's memory and written;
-// a sequence cut by a range's border leaves parts in the scratch that
-// decode_join_kernel adds up in the ranges' order. Where weights are accumulated, the
+// a sequence cut by a range's border leaves parts in the scratch, and the CTA that
+// comes last adds them up in the ranges' order. Where weights are accumulated, the
 // scores go to the scratch as well (rows x 4 bytes for a token, against its 4 D), and
 // decode_weights_kernel takes them up once the rows' sums are known.
 #include <algorithm>
@@ -36,20 +36,12 @@ enum : uint32_t { kFirst = 1, kLast = 2, kMask = 4, kWhole = 8, kSecondSlot = 16
 struct TileInfo {
   uint32_t flags, seq, q_first, queries;
   int token, len, low, sinks;  // low: first token inside the first query's window
-};
-
-// What decode_join_kernel needs to know of a range.
-struct RangeInfo {
-  uint32_t seq;     // of its last piece
-  uint32_t starts;  // that sequence starts in this range
-  uint32_t goes_on; // and continues in the next one
-  uint32_t slot;
+  uint32_t first_range, parts, first_slot;  // of a sequence that more than one range holds
 };
 
 struct DecodeArgs {
   AttnArgs a;
   uint32_t ranges;
-  RangeInfo* info;  // [ranges]
   float* part_o;    // [ranges][2][kv_heads][kRows][D], sums of 2^(z - m) v
   float2* part_ml;  // the same rows' m and sum of 2^(z - m)
   float* scores;    // [kv_heads][rows][columns], in powers of two, where weights are added up
@@ -88,13 +80,51 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnArgs& a, uint32_t s, int p
   return i;
 }
 
+// The rows of a sequence that several ranges hold: D / 4 threads to a row, the parts
+// in the ranges' order.
+template <typename T, int D>
+__device__ __forceinline__ void join_parts(const DecodeArgs& d, const TileInfo& info, uint32_t head, uint32_t rows) {
+  const AttnArgs& a = d.a;
+  constexpr uint32_t kLanes = D / 4;
+  const uint32_t lane = threadIdx.x % kLanes, e = lane * 4;
+  for (uint32_t r0 = 0; r0 < rows; r0 += 128 / kLanes) {
+    const uint32_t r = min(r0 + threadIdx.x / kLanes, rows - 1);  // all lanes take part in the shuffles
+    auto row_of = [&](uint32_t k) {
+      return (static_cast<uint64_t>((info.first_range + k) * 2 + (k == 0 ? info.first_slot : 0)) * a.kv_heads + head) *
+                 kRows + r;
+    };
+    float top = -INFINITY, sum = 0.f, x[4] = {};
+    for (uint32_t k = lane; k < info.parts; k += kLanes) top = fmaxf(top, __ldcg(&d.part_ml[row_of(k)].x));
+    for (uint32_t i = kLanes / 2; i; i /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 8
+    for (uint32_t k = 0; k < info.parts; ++k) {
+      const uint64_t row = row_of(k);
+      const float2 ml = __ldcg(&d.part_ml[row]);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(d.part_o + row * D + e));
+      const float f = exp2_approx(ml.x - ref);
+      sum += f * ml.y;
+      x[0] += f * v.x;
+      x[1] += f * v.y;
+      x[2] += f * v.z;
+      x[3] += f * v.w;
+    }
+    if (r0 + threadIdx.x / kLanes >= rows) continue;
+    const uint32_t t = info.q_first + r / a.group, h = head * a.group + r % a.group;
+    const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
+    store_row<T, D, 4>(a, t, h, e, f, x);
+    if (e == 0) store_lse(a, t, h, f);
+  }
+  __syncwarp();
+}
+
 template <typename T, int D, bool kScores>
 __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_constant__ CUtensorMap map, DecodeArgs d) {
   using L = Layout<D>;
   extern __shared__ uint8_t raw[];
   __shared__ TileInfo s_info[L::kStages];
   __shared__ uint64_t s_full[L::kStages], s_empty[L::kStages];
-  __shared__ uint32_t s_scan[kThreads / 32], s_begin[2], s_gave_up, s_drained;
+  __shared__ uint32_t s_scan[kThreads / 32], s_begin[2], s_gave_up, s_drained, s_last;
   __shared__ float2 s_ml[kWarps][kRows];
   const AttnArgs& a = d.a;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -133,11 +163,9 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     if (w < warp) before += s_scan[w];
     total += s_scan[w];
   }
-  const uint32_t ranges = min(d.ranges, total);
-  if (range >= ranges) {
-    if (head == 0 && threadIdx.x == 0) d.info[range] = RangeInfo{0, 0, 0, 0};
-    return;
-  }
+  // Three tiles are in flight at once: fewer in a range save no time, and leave more to join.
+  const uint32_t ranges = min(d.ranges, (total + 2) / 3);
+  if (range >= ranges) return;
   const uint32_t t0 = static_cast<uint32_t>(static_cast<uint64_t>(range) * total / ranges);
   const uint32_t t1 = static_cast<uint32_t>(static_cast<uint64_t>(range + 1) * total / ranges);
   if (before <= t0 && t0 < before + mine) {
@@ -164,11 +192,19 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       const uint32_t stage = i % L::kStages;
       const int tile = t < static_cast<uint32_t>(q.sink_tiles) ? t : q.first_tile + (t - q.sink_tiles);
       const int token = tile * kTile, end = min(token + kTile, q.len);
-      TileInfo info{fresh ? kFirst : 0u, s, q.q_first, q.queries, token, q.len, q.low, q.sinks};
+      TileInfo info{fresh ? kFirst : 0u, s, q.q_first, q.queries, token, q.len, q.low, q.sinks, 0, 0, 0};
       const bool seq_done = t + 1 == q.tiles;
       if (seq_done || i + 1 == count) info.flags |= kLast;
       const bool starts = s != s_begin[0] || s_begin[1] == 0;
       if (seq_done && starts) info.flags |= kWhole;
+      if ((info.flags & kLast) && !(info.flags & kWhole)) {
+        // the ranges that hold tiles [first, first + q.tiles)
+        const uint64_t first = t0 + i - t;
+        auto range_of = [&](uint64_t tile) { return static_cast<uint32_t>(((tile + 1) * ranges - 1) / total); };
+        info.first_range = range_of(first);
+        info.parts = range_of(first + q.tiles - 1) - info.first_range + 1;
+        info.first_slot = first != static_cast<uint64_t>(info.first_range) * total / ranges;
+      }
       if (pieces > 0) info.flags |= kSecondSlot;
       const int last_low = a.window ? q.low + static_cast<int>(q.queries) - 1 : 0;  // at least the last query's
       if (token + kTile - 1 > q.len - static_cast<int>(q.queries) ||
@@ -201,8 +237,6 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
                   D * 2, full);
       fresh = false;
       ++t;
-      if (i + 1 == count && head == 0 && lane == 0)
-        d.info[range] = RangeInfo{s, starts, !seq_done, pieces > 0};
       if (seq_done && i + 1 < count) {
         do q = seq_info(a, ++s, prefix); while (q.tiles == 0);
         t = 0;
@@ -382,55 +416,17 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
           if (e == 0) d.part_ml[row] = make_float2(top, sum);
         }
       }
+      if (!(info.flags & kWhole)) {  // whoever comes last adds the parts up, in the ranges' order
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (threadIdx.x == 0)
+          s_last = alive && last_to_arrive(a.counters + info.first_range * a.kv_heads + head, info.parts);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        if (s_last) join_parts<T, D>(d, info, head, rows);
+      }
       proxy_fence_smem();  // these accesses come before the copies of the next tile here
     }
     mbar_arrive_warp(smem_addr(&s_empty[stage]), lane, alive);
   }
-}
-
-// One CTA per row of the sequence that starts in a range and continues past it:
-// the parts of its ranges, in their order, two values of the row for each lane.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) decode_join_kernel(DecodeArgs d) {
-  constexpr int E = D / 32;
-  const AttnArgs& a = d.a;
-  const uint32_t range = blockIdx.x, head = blockIdx.y, r = blockIdx.z, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const RangeInfo own = d.info[range];
-  if (!own.goes_on || !own.starts) return;
-  const uint32_t q_first = a.q_offsets[own.seq], rows = (a.q_offsets[own.seq + 1] - q_first) * a.group;
-  if (r >= rows) return;
-  uint32_t end = range + 1;
-  for (;; ++end) {  // the last range of this sequence: the next one starts with another, or ends here
-    const RangeInfo next = d.info[end];
-    if (next.seq != own.seq || !next.goes_on) break;
-  }
-  auto row_of = [&](uint32_t k) {
-    return (static_cast<uint64_t>(k * 2 + (k == range ? own.slot : 0)) * a.kv_heads + head) * kRows + r;
-  };
-  float top = -INFINITY, sum = 0.f, v[E] = {};
-  for (uint32_t k = range + lane; k <= end; k += 32) top = fmaxf(top, d.part_ml[row_of(k)].x);
-  for (int x = 16; x; x /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
-  const float ref = top == -INFINITY ? 0.f : top;
-  for (uint32_t k = range + warp; k <= end; k += 4) {
-    const uint64_t row = row_of(k);
-    const float2 ml = d.part_ml[row];
-    const float f = exp2_approx(ml.x - ref);
-    sum += f * ml.y;
-    for (int e = 0; e < E; ++e) v[e] += f * d.part_o[row * D + e * 32 + lane];
-  }
-  __shared__ float s_v[4][D], s_sum[4];
-  for (int e = 0; e < E; ++e) s_v[warp][e * 32 + lane] = v[e];
-  if (lane == 0) s_sum[warp] = sum;
-  __syncthreads();
-  const uint32_t e = threadIdx.x * 4;
-  if (e >= D) return;
-  sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-  float x[4];
-  for (int i = 0; i < 4; ++i) x[i] = s_v[0][e + i] + s_v[1][e + i] + s_v[2][e + i] + s_v[3][e + i];
-  const uint32_t t = q_first + r / a.group, h = head * a.group + r % a.group;
-  const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
-  store_row<T, D, 4>(a, t, h, e, f, x);
-  if (e == 0) store_lse(a, t, h, f);
 }
 
 // A token's softmax weights, of the scores that decode_kernel left: one thread for
@@ -461,26 +457,23 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(DecodeArgs d) {
   }
 }
 
-// Two CTAs fit an SM. A range holds one tile at least.
+// Two CTAs fit an SM. Each range and head needs a counter, where there are ranges to join.
 uint32_t decode_ranges(const tcx_kv_attention_args& x) {
   const uint64_t tiles = x.total_pages * x.page_tokens / kTile + x.n_seq;
-  return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(tiles, 2ull * sm_count() / x.kv_heads)));
+  const uint64_t most = std::min<uint64_t>(2ull * sm_count(), TCX_KV_COUNTERS) / x.kv_heads;
+  return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((tiles + 2) / 3, most)));
 }
 
 template <typename T, int D, bool kScores>
-tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint32_t rows, uint64_t max_tokens,
-                  cudaStream_t stream) {
+tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint64_t max_tokens, cudaStream_t stream) {
   using L = Layout<D>;
-  TCX_CUDA_TRY(
-      cudaFuncSetAttribute(decode_kernel<T, D, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+  static std::atomic<uint64_t> allowed{0};
+  if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(decode_kernel<T, D, kScores>), L::kBytes, &allowed);
+      st != TCX_OK)
+    return st;
   decode_kernel<T, D, kScores><<<d.ranges * d.a.kv_heads, kThreads, L::kBytes, stream>>>(map, d);
   note_launches(1);
   TCX_CUDA_TRY(cudaGetLastError());
-  if (d.ranges > 1) {
-    decode_join_kernel<T, D><<<dim3(d.ranges - 1, d.a.kv_heads, rows), 128, 0, stream>>>(d);
-    note_launches(1);
-    TCX_CUDA_TRY(cudaGetLastError());
-  }
   if (kScores && max_tokens > 0) {
     const uint64_t blocks = std::min<uint64_t>((max_tokens + 255) / 256, 64);
     decode_weights_kernel<<<dim3(static_cast<unsigned>(blocks), d.a.kv_heads, d.a.n_seq), 256, 0, stream>>>(d);
@@ -491,10 +484,9 @@ tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint32_t rows, ui
 }
 
 template <typename T, int D>
-tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint32_t rows, uint64_t max_tokens,
-                  cudaStream_t stream) {
-  return d.scores != nullptr ? launch<T, D, true>(d, map, rows, max_tokens, stream)
-                             : launch<T, D, false>(d, map, rows, max_tokens, stream);
+tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint64_t max_tokens, cudaStream_t stream) {
+  return d.scores != nullptr ? launch<T, D, true>(d, map, max_tokens, stream)
+                             : launch<T, D, false>(d, map, max_tokens, stream);
 }
 
 uint64_t score_bytes(const tcx_kv_attention_args& x) {
@@ -510,7 +502,7 @@ bool decode_fits(const tcx_kv_attention_args& x) {
 
 uint64_t decode_scratch_bytes(const tcx_kv_attention_args& x) {
   const uint64_t parts = decode_ranges(x) * 2ull * x.kv_heads * kRows;
-  return align256(decode_ranges(x) * sizeof(RangeInfo)) + align256(parts * sizeof(float2)) +
+  return align256(parts * sizeof(float2)) +
          align256(parts * x.head_dim * 4) + score_bytes(x);
 }
 
@@ -521,8 +513,7 @@ tcx_status launch_decode(const tcx_kv_attention_args& x, const AttnArgs& a, cons
   d.ranges = decode_ranges(x);
   const uint64_t parts = d.ranges * 2ull * x.kv_heads * kRows;
   uint8_t* at = static_cast<uint8_t*>(scratch);
-  d.info = reinterpret_cast<RangeInfo*>(at);
-  d.part_ml = reinterpret_cast<float2*>(at += align256(d.ranges * sizeof(RangeInfo)));
+  d.part_ml = reinterpret_cast<float2*>(at);
   d.part_o = reinterpret_cast<float*>(at += align256(parts * sizeof(float2)));
   const uint32_t rows = static_cast<uint32_t>(x.max_q) * a.group;
   if (x.d_weights != nullptr) {
@@ -532,9 +523,9 @@ tcx_status launch_decode(const tcx_kv_attention_args& x, const AttnArgs& a, cons
   }
   const uint64_t max_tokens = x.max_pages * x.page_tokens;
   if (x.dtype == TCX_KV_BF16)
-    return x.head_dim == 128 ? launch<__nv_bfloat16, 128>(d, map, rows, max_tokens, stream)
-                             : launch<__nv_bfloat16, 64>(d, map, rows, max_tokens, stream);
-  return x.head_dim == 128 ? launch<__half, 128>(d, map, rows, max_tokens, stream) : launch<__half, 64>(d, map, rows, max_tokens, stream);
+    return x.head_dim == 128 ? launch<__nv_bfloat16, 128>(d, map, max_tokens, stream)
+                             : launch<__nv_bfloat16, 64>(d, map, max_tokens, stream);
+  return x.head_dim == 128 ? launch<__half, 128>(d, map, max_tokens, stream) : launch<__half, 64>(d, map, max_tokens, stream);
 }
 
 }  // namespace tcx

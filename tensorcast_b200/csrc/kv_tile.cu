@@ -17,8 +17,10 @@
 //
 // Work: the visible (row tile, kv head, token tile) units laid end to end and cut
 // into equal ranges, one CTA on every SM, whatever the prompts' lengths and masks
-// are; row tiles cut by a border leave parts that tile_join_kernel adds up in the
-// ranges' order. tile_plan_kernel lays the units out from the device's lengths.
+// are; row tiles cut by a border leave parts in the scratch, which are added up in the
+// ranges' order by tile_join_kernel, or where they are few by the CTA that comes
+// last. tile_plan_kernel lays prompts' units out
+// from the device's lengths; over a prefix all row tiles have the same ones.
 #include <algorithm>
 #include <type_traits>
 
@@ -36,6 +38,10 @@ constexpr int kPlanCache = 2048;
 // What a piece of a row tile costs beside its token tiles (its queries, its first
 // scores, its output), in token tiles: counted when the work is cut into ranges.
 constexpr uint32_t kPieceCost = 3;
+
+// Up to so many rows the CTA that comes last adds their parts up, one warp to a row
+// at a time: 256 rows took it 115 us over 18 ranges, a launch of its own takes 18.
+constexpr uint32_t kJoinHere = 32;
 
 // A tile of rows: row r is query token q_first + (row0 + r) / group.
 struct Item {
@@ -60,6 +66,7 @@ struct RangeEnd {
 struct TileArgs {
   AttnArgs a;
   uint32_t prefix;  // rows of all sequences over the shared prefix
+  uint32_t join_here;  // few rows: the CTA that comes last adds their parts up
   uint32_t max_q, max_ranges;
   uint32_t* item_first;  // [n_seq + 1]
   Item* items;
@@ -106,6 +113,11 @@ __device__ Item make_item(const TileArgs& d, uint32_t s, uint32_t index, int pre
   return it;
 }
 
+// Every range must hold more than a piece's cost to hold a tile.
+__device__ __forceinline__ uint64_t piece_cost(uint64_t units, uint64_t pieces, uint32_t ranges) {
+  return (units + kPieceCost * pieces) / ranges > kPieceCost ? kPieceCost : 0;
+}
+
 // Exclusive sum over the CTA; *total gets the sum.
 __device__ uint64_t plan_scan(uint64_t v, uint64_t* sums, uint64_t* total) {
   const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -133,9 +145,7 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(TileArgs d) {
   const int prefix = static_cast<int>(prefix_length(a));
   uint64_t total;
   uint32_t items;
-  if (d.prefix) {
-    items = static_cast<uint32_t>((static_cast<uint64_t>(a.q_tokens) * a.group + kRows - 1) / kRows);
-  } else {
+  {
     const uint32_t share = (a.n_seq + kPlanThreads - 1) / kPlanThreads, s0 = min(threadIdx.x * share, a.n_seq),
                    s1 = min(s0 + share, a.n_seq);
     uint32_t mine = 0;
@@ -153,15 +163,12 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(TileArgs d) {
     const uint32_t i = i0 + threadIdx.x;
     uint64_t mine = 0;
     if (i < items) {
-      uint32_t s = 0, first = 0;
-      if (!d.prefix) {  // the last sequence whose items begin at i or before
-        uint32_t hi = a.n_seq;
-        while (hi - s > 1) {
-          const uint32_t mid = (s + hi) / 2;
-          if ((mid < kPlanCache ? s_first[mid] : d.item_first[mid]) <= i) s = mid; else hi = mid;
-        }
-        first = s < kPlanCache ? s_first[s] : d.item_first[s];
+      uint32_t s = 0, hi = a.n_seq;  // the last sequence whose items begin at i or before
+      while (hi - s > 1) {
+        const uint32_t mid = (s + hi) / 2;
+        if ((mid < kPlanCache ? s_first[mid] : d.item_first[mid]) <= i) s = mid; else hi = mid;
       }
+      const uint32_t first = s < kPlanCache ? s_first[s] : d.item_first[s];
       const Item it = make_item(d, s, i - first, prefix);
       d.items[i] = it;
       mine = static_cast<uint64_t>(it.tiles) * a.kv_heads;
@@ -175,9 +182,7 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(TileArgs d) {
   }
   __syncthreads();
   const uint32_t ranges = static_cast<uint32_t>(min(static_cast<uint64_t>(d.max_ranges), units));
-  // Every range must hold more than a piece's cost to hold a tile.
-  const uint64_t pieces = static_cast<uint64_t>(items) * a.kv_heads;
-  const uint64_t cost = (units + kPieceCost * pieces) / ranges > kPieceCost ? kPieceCost : 0;
+  const uint64_t pieces = static_cast<uint64_t>(items) * a.kv_heads, cost = piece_cost(units, pieces, ranges);
   if (threadIdx.x == 0) {
     d.counts[0] = items;
     d.counts[1] = ranges;
@@ -198,7 +203,6 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(TileArgs d) {
     d.begin[r] = RangeBegin{lo, static_cast<uint32_t>(head), static_cast<uint32_t>(tile),
                             first_of(lo) - cost * a.kv_heads * lo + head * tiles + tile};
   }
-  for (uint32_t r = ranges + threadIdx.x; r < d.max_ranges; r += kPlanThreads) d.end[r] = RangeEnd{0, 0, 0, 0, 0};
 }
 
 template <int D>
@@ -216,13 +220,57 @@ __device__ __forceinline__ int first_token(const Item& it, uint32_t tile) {
                                                      : it.first_tile + static_cast<int>(tile) - it.sink_tiles) * kTokens;
 }
 
+// The rows of an item and head that the ranges [from, to] hold parts of, one warp of
+// eight to a row, the parts in the ranges' order.
+template <typename T, int D>
+__device__ __forceinline__ void join_rows(const TileArgs& d, const Item& it, uint32_t head, uint32_t from, uint32_t to,
+                                          uint32_t first_slot, uint32_t warp, uint32_t lane) {
+  constexpr int E = D / 32;
+  const AttnArgs& a = d.a;
+  for (uint32_t r = warp; r < it.rows; r += 8) {
+    auto row_of = [&](uint32_t k) { return static_cast<uint64_t>(k * 2 + (k == from ? first_slot : 0)) * kRows + r; };
+    float top = -INFINITY, sum = 0.f, x[E] = {};
+    for (uint32_t k = from + lane; k <= to; k += 32) top = fmaxf(top, __ldcg(&d.part_ml[row_of(k)].x));
+    for (int i = 16; i; i /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
+    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+    for (uint32_t k = from; k <= to; ++k) {
+      const uint64_t row = row_of(k);
+      const float2 ml = __ldcg(&d.part_ml[row]);
+      const float f = exp2_approx(ml.x - ref);
+      sum += f * ml.y;
+      if constexpr (E == 4) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(d.part_o + row * D) + lane);
+        x[0] += f * v.x;
+        x[1] += f * v.y;
+        x[2] += f * v.z;
+        x[3] += f * v.w;
+      } else {
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(d.part_o + row * D) + lane);
+        x[0] += f * v.x;
+        x[1] += f * v.y;
+      }
+    }
+    const uint32_t row = it.row0 + r, t = it.q_first + row / a.group, h = head * a.group + row % a.group;
+    const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
+    if constexpr (E == 4) {
+      store_row<T, D, 4>(a, t, h, lane * 4, f, x);
+    } else {  // two lanes' values in one
+      const float y[4] = {x[0], x[1], __shfl_down_sync(~0u, x[0], 1), __shfl_down_sync(~0u, x[1], 1)};
+      if (lane % 2 == 0) store_row<T, D, 4>(a, t, h, lane * 2, f, y);
+    }
+    if (lane == 0) store_lse(a, t, h, f);
+    __syncwarp();
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map, TileArgs d) {
   using L = TileLayout<D>;
   constexpr uint32_t kStages = L::kStages;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t s_bar[2 * kStages + 10];
-  __shared__ uint32_t s_tmem, s_gave_up, s_drained;
+  __shared__ uint32_t s_tmem, s_gave_up, s_drained, s_last;
   __shared__ __align__(16) int s_seen[2][8][4];
   const AttnArgs& a = d.a;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, range = blockIdx.x;
@@ -251,16 +299,39 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     s_gave_up = s_drained = 0;
     mbar_init_fence();
   }
-  const uint32_t ranges = d.counts[1];
-  if (range >= ranges) return;
+  // The work: its row tiles, where the ranges begin, and this one.
+  const int prefix = static_cast<int>(prefix_length(a));
+  uint32_t items, ranges;
+  uint64_t same_tiles = 0, cost = 0;  // over a prefix: every row tile's token tiles
+  if (d.prefix) {
+    items = static_cast<uint32_t>((static_cast<uint64_t>(a.q_tokens) * a.group + kRows - 1) / kRows);
+    same_tiles = make_item(d, 0, 0, prefix).tiles;
+    const uint64_t pieces = static_cast<uint64_t>(items) * a.kv_heads;
+    ranges = static_cast<uint32_t>(min(static_cast<uint64_t>(d.max_ranges), pieces * same_tiles));
+    cost = piece_cost(pieces * same_tiles, pieces, ranges);
+  } else {
+    items = d.counts[0];
+    ranges = d.counts[1];
+  }
+  if (range >= ranges) {
+    if (threadIdx.x == 0) d.end[range] = RangeEnd{0, 0, 0, 0, 0};
+    return;
+  }
+  auto begin_of = [&](uint32_t r) {
+    if (!d.prefix) return d.begin[r];
+    const uint64_t pieces = static_cast<uint64_t>(items) * a.kv_heads, at = pieces * (same_tiles + cost) * r / ranges;
+    const uint64_t piece = at / (same_tiles + cost), tile = max(at % (same_tiles + cost), cost) - cost;
+    return RangeBegin{static_cast<uint32_t>(piece / a.kv_heads), static_cast<uint32_t>(piece % a.kv_heads),
+                      static_cast<uint32_t>(tile), piece * same_tiles + tile};
+  };
+  auto item_of = [&](uint32_t i) { return d.prefix ? make_item(d, 0, i, prefix) : d.items[i]; };
   if (warp == 8) tmem_alloc(smem_addr(&s_tmem), L::kColumns);
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
   const uint32_t tmem = s_tmem;
-  const uint32_t items = d.counts[0];
-  const RangeBegin begin = d.begin[range];
-  const uint32_t count = static_cast<uint32_t>(d.begin[range + 1].unit - begin.unit);
+  const RangeBegin begin = begin_of(range);
+  const uint32_t count = static_cast<uint32_t>(begin_of(range + 1).unit - begin.unit);
 
   // Every role walks the range's pieces: the token tiles [at, at + n) of one item and head.
   uint32_t item = begin.item, head = begin.head, at = begin.tile;
@@ -270,7 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       const uint32_t boxes = kTokens / a.box_rows;
       const uint32_t box = lane % boxes, half = lane / boxes;
       uint32_t slot_at = 0;  // ring position
-      Item it = d.items[item];
+      Item it = item_of(item);
       if (lane == 0) mbar_arrive(full(0));  // no values before the first keys
       bool alive = true;
       for (uint32_t left = count; left > 0 && alive;) {
@@ -302,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         at = 0;
         if (++head == a.kv_heads && left > 0) {
           head = 0;
-          it = d.items[++item];
+          it = item_of(++item);
         }
       }
       const uint32_t last = slot_at / 2;
@@ -362,8 +433,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         __syncwarp();
       };
       auto uniform = [&](uint32_t x) { return __shfl_sync(~0u, x, 0); };
-      uint32_t tiles = uniform(d.items[item].tiles), rows = uniform(d.items[item].rows);
-      uint32_t next = min(item + 1, items - 1), next_tiles = d.items[next].tiles, next_rows = d.items[next].rows;
+      Item next = item_of(item);
+      uint32_t tiles = uniform(next.tiles), rows = uniform(next.rows), next_item = min(item + 1, items - 1);
+      next = item_of(next_item);
       at = uniform(at);
       head = uniform(head);
       for (uint32_t left = uniform(count); left > 0;) {
@@ -396,11 +468,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         at = 0;
         if (++head == a.kv_heads) {
           head = 0;
-          tiles = uniform(next_tiles);
-          rows = uniform(next_rows);
-          next = min(next + 1, items - 1);
-          next_tiles = d.items[next].tiles;
-          next_rows = d.items[next].rows;
+          tiles = uniform(next.tiles);
+          rows = uniform(next.rows);
+          next_item = min(next_item + 1, items - 1);
+          next = item_of(next_item);
         }
       }
     }
@@ -410,7 +481,6 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     const uint32_t h = warp / 4, r = threadIdx.x, quarter = warp % 4 * 32 << 16;
     const uint32_t scores = tmem + quarter + L::kScores + h * kTokens, sums = tmem + quarter + L::kSums + h * D;
     const uint32_t staged = base + (2 + kStages) * L::kOperand + warp * 4096;
-    const int prefix = static_cast<int>(prefix_length(a));
     uint32_t pieces = 0, done = 0, summed = 0, tiles_done = 0;
     bool alive = true;
     auto wait = [&](uint32_t b, uint32_t phase) { alive = alive && mbar_wait_warp(b, phase & 1, &s_gave_up, a.status); };
@@ -430,7 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
                      a.q + (valid ? at_row + c * 16 : 0), valid ? 16 : 0);
       }
     };
-    Item it = d.items[item];
+    Item it = item_of(item);
     if (h * kHalfRows < it.rows) fetch(it.q_first, it.row0, it.rows, head);
     for (uint32_t left = count; left > 0; ++pieces) {
       const uint32_t n = min(it.tiles - at, left);
@@ -447,9 +517,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         if (head + 1 < a.kv_heads) {
           if (active) fetch(it.q_first, it.row0, it.rows, head + 1);
         } else {
-          const Item& next = d.items[item + 1];
-          const uint32_t rows = next.rows;
-          if (h * kHalfRows < rows) fetch(next.q_first, next.row0, rows, 0);
+          const Item next = item_of(item + 1);
+          if (h * kHalfRows < next.rows) fetch(next.q_first, next.row0, next.rows, 0);
         }
       };
       if (!active) fetch_next();
@@ -691,6 +760,23 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
         tmem_fence_before();
       }
+      if (d.join_here && (at != 0 || n != it.tiles)) {
+        // Another range has parts of these rows too: whoever comes last adds them up.
+        const uint64_t first = begin.unit + tiles_done - at, last = first + it.tiles - 1;
+        uint32_t from = 0, to = 0;  // the last ranges that begin at the first and last tile, or before
+        for (uint32_t r0 = 0; r0 < ranges; r0 += 32) {
+          const uint32_t r = r0 + lane;
+          const uint64_t unit = r < ranges ? begin_of(r).unit : ~uint64_t{0};
+          from += __popc(__ballot_sync(~0u, unit <= first));
+          to += __popc(__ballot_sync(~0u, unit <= last));
+        }
+        --from;
+        --to;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (threadIdx.x == 0) s_last = alive && last_to_arrive(a.counters + from, to - from + 1);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (s_last) join_rows<T, D>(d, it, head, from, to, begin_of(from).unit != first, warp, lane);
+      }
       left -= n;
       tiles_done += n;
       if (left == 0 && threadIdx.x == 0)
@@ -698,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       at = 0;
       if (++head == a.kv_heads && left > 0) {
         head = 0;
-        it = d.items[++item];
+        it = item_of(++item);
       }
     }
   }
@@ -717,12 +803,15 @@ __global__ void __launch_bounds__(256) tile_join_kernel(TileArgs d) {
   const uint32_t range = blockIdx.x, r = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   const RangeEnd own = d.end[range];
   if (!own.goes_on || !own.starts) return;
-  const Item it = d.items[own.item];
+  const Item it = d.prefix ? make_item(d, 0, own.item, static_cast<int>(prefix_length(a))) : d.items[own.item];
   if (r >= it.rows) return;
-  uint32_t end = range + 1;
-  for (;; ++end) {
-    const RangeEnd next = d.end[end];
-    if (next.item != own.item || next.head != own.head || !next.goes_on) break;
+  uint32_t end = range + 1;  // the last range of these rows: the next one holds others, or they end here
+  for (;; end += 32) {
+    const RangeEnd next = d.end[min(end + lane, d.max_ranges - 1)];
+    const uint32_t ends = __ballot_sync(~0u, next.item != own.item || next.head != own.head || !next.goes_on);
+    if (ends == 0) continue;
+    end += __ffs(ends) - 1;
+    break;
   }
   auto row_of = [&](uint32_t k) { return static_cast<uint64_t>(k * 2 + (k == range ? own.slot : 0)) * kRows + r; };
   float top = -INFINITY, sum = 0.f, x[E] = {};
@@ -735,8 +824,18 @@ __global__ void __launch_bounds__(256) tile_join_kernel(TileArgs d) {
     const float2 ml = d.part_ml[row];
     const float f = exp2_approx(ml.x - ref);
     sum += f * ml.y;
-#pragma unroll
-    for (int e = 0; e < E; ++e) x[e] += f * d.part_o[row * D + lane * E + e];
+    const float* o = d.part_o + row * D + lane * E;
+    if constexpr (E == 4) {
+      const float4 v = *reinterpret_cast<const float4*>(o);
+      x[0] += f * v.x;
+      x[1] += f * v.y;
+      x[2] += f * v.z;
+      x[3] += f * v.w;
+    } else {
+      const float2 v = *reinterpret_cast<const float2*>(o);
+      x[0] += f * v.x;
+      x[1] += f * v.y;
+    }
   }
   const uint32_t row = it.row0 + r, t = it.q_first + row / a.group, h = own.head * a.group + row % a.group;
   const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
@@ -757,7 +856,7 @@ uint64_t max_items(const tcx_kv_attention_args& x, bool prefix) {
 uint32_t max_ranges(const tcx_kv_attention_args& x, bool prefix) {
   const uint64_t pages = prefix ? x.prefix_pages : x.max_pages;
   const uint64_t units = max_items(x, prefix) * x.kv_heads * (pages * x.page_tokens / kTokens + 2);
-  return static_cast<uint32_t>(std::min<uint64_t>(sm_count(), units));
+  return static_cast<uint32_t>(std::min<uint64_t>({static_cast<uint64_t>(sm_count()), units, TCX_KV_COUNTERS}));
 }
 
 struct Parts {
@@ -788,14 +887,19 @@ Parts parts(const tcx_kv_attention_args& x, bool prefix) {
 template <typename T, int D>
 tcx_status launch(const TileArgs& d, const CUtensorMap& map, cudaStream_t stream) {
   using L = TileLayout<D>;
-  tile_plan_kernel<<<1, kPlanThreads, 0, stream>>>(d);
-  note_launches(1);
-  TCX_CUDA_TRY(cudaGetLastError());
-  TCX_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+  static std::atomic<uint64_t> allowed{0};
+  if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(tile_kernel<T, D>), L::kBytes, &allowed);
+      st != TCX_OK)
+    return st;
+  if (!d.prefix) {
+    tile_plan_kernel<<<1, kPlanThreads, 0, stream>>>(d);
+    note_launches(1);
+    TCX_CUDA_TRY(cudaGetLastError());
+  }
   tile_kernel<T, D><<<d.max_ranges, kThreads, L::kBytes, stream>>>(map, d);
   note_launches(1);
   TCX_CUDA_TRY(cudaGetLastError());
-  if (d.max_ranges > 1) {
+  if (d.max_ranges > 1 && !d.join_here) {
     tile_join_kernel<T, D><<<dim3(d.max_ranges - 1, kRows / 8), 256, 0, stream>>>(d);
     note_launches(1);
     TCX_CUDA_TRY(cudaGetLastError());
@@ -815,6 +919,7 @@ tcx_status launch_tile(const tcx_kv_attention_args& x, const AttnArgs& a, const 
   d.a = a;
   d.prefix = prefix;
   d.max_q = static_cast<uint32_t>(x.max_q);
+  d.join_here = (prefix ? x.q_tokens : x.max_q) * a.group <= kJoinHere;
   d.max_ranges = max_ranges(x, prefix);
   d.item_first = reinterpret_cast<uint32_t*>(at + p.item_first);
   d.items = reinterpret_cast<Item*>(at + p.items);

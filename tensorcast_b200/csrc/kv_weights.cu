@@ -198,7 +198,10 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
 template <typename T, int D>
 tcx_status launch(const AttnArgs& a, const CUtensorMap& map, uint64_t max_tokens, cudaStream_t stream) {
   using L = WeightLayout<D>;
-  TCX_CUDA_TRY(cudaFuncSetAttribute(weights_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes));
+  static std::atomic<uint64_t> allowed{0};
+  if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(weights_kernel<T, D>), L::kBytes, &allowed);
+      st != TCX_OK)
+    return st;
   const dim3 grid(static_cast<unsigned>((max_tokens + kKeys - 1) / kKeys), a.kv_heads, a.n_seq);
   weights_kernel<T, D><<<grid, kThreads, L::kBytes, stream>>>(map, a);
   note_launches(1);

@@ -33,6 +33,10 @@ _STATUS = {1: "page slot outside the pool", 2: "more tokens than the sequence's 
            3: "budget past the destination pages", 4: "a copy into shared memory did not arrive"}
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # by device index, without building a Stream
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+
+
 def _refuse(message: str):
     raise _native.TcxInvalidArgument(_native.INVALID_ARGUMENT, message)
 
@@ -55,7 +59,7 @@ def _check_tables(w: KvWorkload, what: str) -> None:
 
 
 class _Tables:
-    """Device tables shared by the two classes, in one allocation."""
+    """Device tables of one object, in one allocation."""
 
     def __init__(self, device, arrays: dict):
         sizes = {k: -(-v.nbytes // 16) * 16 for k, v in arrays.items()}
@@ -65,21 +69,21 @@ class _Tables:
             host[at:at + v.nbytes] = np.ascontiguousarray(v).view(np.uint8).reshape(-1)
             at += sizes[k]
         self.buffer = torch.from_numpy(host).to(device)
-        self.stream = torch.cuda.current_stream(device).cuda_stream
         at = 0
         for k, v in arrays.items():
-            kind = torch.int64 if v.itemsize == 8 else torch.int32
-            setattr(self, k, self.buffer[at:at + v.nbytes].view(kind))
+            setattr(self, k, self.buffer[at:at + v.nbytes].view(torch.int64 if v.itemsize == 8 else torch.int32))
             at += sizes[k]
-
-    def used_on(self, stream) -> None:
-        """Keeps the memory until work queued now on a stream other than the tables' own has run."""
-        if stream.cuda_stream != self.stream and not torch.cuda.is_current_stream_capturing():
-            self.buffer.record_stream(stream)
 
 
 class _OnDevice:
     """Stream, device and status handling of a call."""
+
+    def _bind(self, w: KvWorkload, tables: dict) -> _Tables:
+        t = self._tables = _Tables(self.device, tables)
+        self._pool_bytes = w.planes * w.pool_pages * w.page_tokens * w.token_bytes
+        self._stream = _raw_stream(self.device.index)  # the stream whose order the tables' memory follows
+        self.status = t.status
+        return t
 
     def _on(self, stream, call):
         """`call` with this object's device current and, where one is given, on `stream`."""
@@ -91,17 +95,24 @@ class _OnDevice:
             with torch.cuda.stream(s):
                 return call()
 
+    def _current(self) -> int:
+        """The current stream. The tables outlive what runs on it now, also where it is not their own."""
+        raw = _raw_stream(self.device.index)
+        if raw != self._stream and not _capturing():
+            self._tables.buffer.record_stream(torch.cuda.current_stream(self.device))
+        return raw
+
     def check_status(self) -> None:
+        """Waits for the device and raises what a call has recorded."""
         code = int(self.status.item())
         if code:
             raise _native.TcxError(_native.DATA_LOSS, _STATUS.get(code, f"kv attention status {code}"))
 
     def _pool(self, pool: torch.Tensor) -> int:
-        if pool.device != self.device or not pool.is_contiguous():
+        if not pool.is_cuda or pool.get_device() != self.device.index or not pool.is_contiguous():
             _refuse(f"pool must be a contiguous tensor on {self.device}")
-        need = self.w.planes * self.w.pool_pages * self.w.page_tokens * self.w.token_bytes
-        if pool.numel() * pool.element_size() < need:
-            _refuse(f"pool has {pool.numel() * pool.element_size()} bytes, its planes need {need}")
+        if pool.nbytes < self._pool_bytes:
+            _refuse(f"pool has {pool.nbytes} bytes, its planes need {self._pool_bytes}")
         return pool.data_ptr()
 
 
@@ -148,12 +159,12 @@ class KvAttention(_OnDevice):
         self.q_offsets = np.concatenate([[0], np.cumsum(counts)])
         self.device = _cuda_device(device)
         offs = np.asarray(w.page_offsets).astype(np.uint64)
-        t = self._tables = _Tables(self.device, {
+        t = self._bind(w, {
             "page_offsets": offs, "page_table": np.asarray(w.page_table).astype(np.uint32),
             "seq_tokens": np.asarray(w.seq_tokens).astype(np.uint32), "q_offsets": self.q_offsets.astype(np.uint32),
             "prefix_table": pages, "prefix_tokens": np.array([prefix_tokens], np.uint32),
             "status": np.zeros(1, np.uint32)})
-        self.page_table, self.seq_tokens, self.status = t.page_table, t.seq_tokens, t.status
+        self.page_table, self.seq_tokens = t.page_table, t.seq_tokens
         self.prefix_tokens = None if prefix_pages is None else t.prefix_tokens
         self._args = _native.KvAttentionArgs(
             planes=w.planes, pool_pages=w.pool_pages, page_tokens=w.page_tokens, kv_heads=kv_heads, q_heads=q_heads,
@@ -165,20 +176,43 @@ class KvAttention(_OnDevice):
             d_prefix_table=None if prefix_pages is None else t.buffer.data_ptr() if not pages.size
             else t.prefix_table.data_ptr(), prefix_pages=pages.size, d_prefix_tokens=t.prefix_tokens.data_ptr(),
             window=window, sinks=sinks, scale=scale, d_status=t.status.data_ptr())
+        self._shape = (q_heads, head_dim)
+        self._scratch_bytes = {}  # with and without weights
+        self._workspaces = {}     # scratch and counters, by stream
 
     @property
     def weight_columns(self) -> int:
         """Columns of ``weights``: token j of sequence s is column page_offsets[s] * page_tokens + j."""
         return int(self.w.page_offsets[-1]) * self.w.page_tokens
 
-    def _rows(self, x: torch.Tensor, what: str) -> None:
-        if x.dtype != self.dtype or x.device != self.device:
+    def _rows(self, x: torch.Tensor, what: str):
+        """(address, token stride, head stride) of queries or outputs."""
+        if x.dtype is not self.dtype or not x.is_cuda or x.get_device() != self.device.index:
             _refuse(f"{what} must be {self.dtype} on {self.device}, got {x.dtype} on {x.device}")
-        if x.dim() != 3 or x.shape[0] < self._args.q_tokens or tuple(x.shape[1:]) != (self.q_heads, self.head_dim):
+        if x.dim() != 3 or x.shape[0] < self._args.q_tokens or x.shape[1:] != self._shape:
             _refuse(f"{what} must be [>= {self._args.q_tokens} tokens, {self.q_heads}, {self.head_dim}], "
                     f"got {list(x.shape)}")
-        if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.data_ptr() % 16:
+        tokens, heads, values = x.stride()
+        at = x.data_ptr()
+        if values != 1 or tokens % 8 or heads % 8 or at % 16:
             _refuse(f"{what} must have dense heads, strides that are multiples of 8 and 16-byte alignment")
+        return at, tokens, heads
+
+    def _workspace(self, a, stream: int):
+        """Scratch and counters: a stream's calls share them, a captured graph has its own."""
+        weighed = a.d_weights is not None
+        need = self._scratch_bytes.get(weighed)
+        if need is None:
+            need = self._scratch_bytes[weighed] = _native.lib().tcx_kv_attention_scratch_bytes(ctypes.byref(a))
+        capturing = _capturing()
+        found = None if capturing else self._workspaces.get(stream)
+        if found is None or found[0].numel() < need:
+            found = (torch.empty(need, dtype=torch.uint8, device=self.device),
+                     torch.zeros(_native.KV_COUNTERS, dtype=torch.int32, device=self.device))
+            if not capturing:
+                self._workspaces[stream] = found
+        a.d_counters = found[1].data_ptr()
+        return found[0].data_ptr(), need
 
     def run(self, pool: torch.Tensor, layer: int, q: torch.Tensor, *, weights: torch.Tensor | None = None,
             out: torch.Tensor | None = None, lse: torch.Tensor | None = None, stream=None):
@@ -189,7 +223,8 @@ class KvAttention(_OnDevice):
         which is not touched in a given ``out`` or ``lse`` and 0 in a new one. ``lse`` is float32
         [tokens, q_heads], the natural logarithm of each row's sum of exponentials. ``weights``,
         float32 [kv_heads, weight_columns], gains each token's softmax weights. ``stream`` is a
-        stream or its handle; the current one by default."""
+        stream or its handle; the current one by default. Calls of one object may run on several
+        streams at once, those of one stream from one thread at a time."""
         if stream is not None or self.device.index != torch.cuda.current_device():
             return self._on(stream, lambda: self.run(pool, layer, q, weights=weights, out=out, lse=lse))
         a = _native.KvAttentionArgs.from_buffer_copy(self._args)
@@ -197,21 +232,21 @@ class KvAttention(_OnDevice):
         if not 0 <= layer < self.w.planes // 2:
             _refuse(f"layer {layer}: the pool has {self.w.planes // 2}")
         a.k_plane, a.v_plane = 2 * layer, 2 * layer + 1
-        self._rows(q, "q")
+        a.d_q, a.q_token_stride, a.q_head_stride = self._rows(q, "q")
         if q.requires_grad and torch.is_grad_enabled():
             _refuse("KvAttention has no gradient: call it under torch.no_grad()")
-        a.d_q, a.q_token_stride, a.q_head_stride = q.data_ptr(), q.stride(0), q.stride(1)
-        padded = q.shape[0] > a.q_tokens
+        rows = q.shape[0]
+        padded = rows > a.q_tokens
         if out is None:
-            out = (torch.zeros if padded else torch.empty)(q.shape, dtype=self.dtype, device=self.device)
+            out = (torch.zeros if padded else torch.empty)((rows, *self._shape), dtype=self.dtype, device=self.device)
+            a.d_out, a.out_token_stride, a.out_head_stride = out.data_ptr(), *out.stride()[:2]
         else:
-            self._rows(out, "out")
+            a.d_out, a.out_token_stride, a.out_head_stride = self._rows(out, "out")
             if out.untyped_storage().data_ptr() in (q.untyped_storage().data_ptr(),
                                                     pool.untyped_storage().data_ptr()):
                 _refuse("out must not share memory with q or the pool")
-        a.d_out, a.out_token_stride, a.out_head_stride = out.data_ptr(), out.stride(0), out.stride(1)
         if lse is None:
-            lse = (torch.zeros if padded else torch.empty)((q.shape[0], self.q_heads), dtype=torch.float32,
+            lse = (torch.zeros if padded else torch.empty)((rows, self.q_heads), dtype=torch.float32,
                                                            device=self.device)
         elif (lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous() or lse.dim() != 2
               or lse.shape[0] < a.q_tokens or lse.shape[1] != self.q_heads):
@@ -226,15 +261,18 @@ class KvAttention(_OnDevice):
                 _refuse(f"weights must be float32 [{self.kv_heads}, {self.weight_columns}] on {self.device}, "
                         "dense in its columns")
             a.d_weights, a.weights_head_stride = weights.data_ptr(), weights.stride(0)
-        current = torch.cuda.current_stream(self.device)
-        self._tables.used_on(current)
-        L = _native.lib()
-        need = L.tcx_kv_attention_scratch_bytes(ctypes.byref(a))
-        # the scratch belongs to the call: concurrent streams and captured graphs never share it
-        scratch = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        _native.call("tcx_kv_attention", ctypes.byref(a), scratch.data_ptr() if need else None, need,
-                     current.cuda_stream)
+        if a.q_tokens:
+            current = self._current()
+            scratch, need = self._workspace(a, current)
+            _native.call("tcx_kv_attention", ctypes.byref(a), scratch, need, current)
         return out, lse
+
+    def check_status(self) -> None:
+        try:
+            super().check_status()
+        except _native.TcxError:
+            self._workspaces.clear()  # a call that gave up leaves its counters as they were
+            raise
 
 
 class KvEvict(_OnDevice):
@@ -269,11 +307,11 @@ class KvEvict(_OnDevice):
         self.w, self.dst, self.kv_heads, self.device = w, dst, kv_heads, _cuda_device(device)
         u32 = lambda x: np.asarray(x).astype(np.uint32)  # noqa: E731
         u64 = lambda x: np.asarray(x).astype(np.uint64)  # noqa: E731
-        t = self._tables = _Tables(self.device, {
+        t = self._bind(w, {
             "page_offsets": u64(w.page_offsets), "dst_page_offsets": u64(dst.page_offsets),
             "page_table": u32(w.page_table), "dst_page_table": u32(dst.page_table), "seq_tokens": u32(w.seq_tokens),
             "budgets": u32(dst.seq_tokens), "status": np.zeros(1, np.uint32)})
-        self.page_table, self.seq_tokens, self.status = t.page_table, t.seq_tokens, t.status
+        self.page_table, self.seq_tokens = t.page_table, t.seq_tokens
         self._args = _native.KvEvictArgs(
             planes=w.planes, pool_pages=w.pool_pages, page_tokens=w.page_tokens, kv_heads=kv_heads,
             head_bytes=w.token_bytes // kv_heads, d_page_table=t.page_table.data_ptr() or t.buffer.data_ptr(),
@@ -303,12 +341,10 @@ class KvEvict(_OnDevice):
             _refuse("weights must not have negative strides")
         a.d_weights = weights.data_ptr() or self._tables.buffer.data_ptr()
         a.weights_layer_stride, a.weights_head_stride = weights.stride(0), weights.stride(1)
-        current = torch.cuda.current_stream(self.device)
-        self._tables.used_on(current)
         shape = (layers, self.kv_heads, int(self.dst.page_offsets[-1]) * self.dst.page_tokens)
         keep = torch.empty(shape, dtype=torch.int32, device=self.device)
         left = torch.empty(shape, dtype=torch.float32, device=self.device)
         tokens = torch.empty(self.w.n_seq, dtype=torch.int32, device=self.device)
         a.d_keep, a.d_dst_weights, a.d_dst_tokens = keep.data_ptr(), left.data_ptr(), tokens.data_ptr()
-        _native.call("tcx_kv_evict", ctypes.byref(a), current.cuda_stream)
+        _native.call("tcx_kv_evict", ctypes.byref(a), self._current())
         return keep, left, tokens

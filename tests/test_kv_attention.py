@@ -73,7 +73,7 @@ def attention_args(**kw):
         d_pool=0x1000, planes=2, pool_pages=8, page_tokens=16, kv_heads=2, q_heads=4, head_dim=64, dtype=0, k_plane=0,
         v_plane=1, d_page_table=0x1000, d_page_offsets=0x1000, d_seq_tokens=0x1000, n_seq=1, d_q_offsets=0x1000,
         q_tokens=1, max_q=1, total_pages=4, max_pages=4, scale=1.0, d_q=0x1000, q_token_stride=256, q_head_stride=64,
-        d_out=0x2000, out_token_stride=256, out_head_stride=64, d_lse=0x1000, d_status=0x1000)
+        d_out=0x2000, out_token_stride=256, out_head_stride=64, d_lse=0x1000, d_status=0x1000, d_counters=0x1000)
     for k, v in kw.items():
         setattr(a, k, v)
     return a
@@ -81,6 +81,7 @@ def attention_args(**kw):
 
 @pytest.mark.parametrize("change,message", [
     (dict(d_pool=None), "null device pointer"), (dict(d_lse=None), "null device pointer"),
+    (dict(d_counters=None), "null device pointer"),
     (dict(d_page_table=None), "null device pointer"), (dict(planes=0), "must be > 0"),
     (dict(page_tokens=12), "multiple of 8"), (dict(head_dim=96), "head_dim"), (dict(dtype=2), "dtype"),
     (dict(q_heads=5), "multiple of kv_heads"), (dict(v_plane=2), "planes of the pool"),
@@ -95,6 +96,21 @@ def test_attention_entry_checks(change, message):
     import ctypes
     with pytest.raises(_native.TcxInvalidArgument, match=message):
         _native.call("tcx_kv_attention", ctypes.byref(attention_args(**change)), None, 0, None)
+
+
+def test_attention_entry_checks_its_scratch():
+    import ctypes
+    L = _native.lib()
+    for change in ({}, dict(d_prefix_table=0x1000, d_prefix_tokens=0x1000, prefix_pages=1), dict(max_q=9, q_tokens=9),
+                   dict(d_weights=0x1000)):
+        a = attention_args(**change)
+        need = L.tcx_kv_attention_scratch_bytes(ctypes.byref(a))
+        assert need > 0
+        for scratch, size in ((None, need), (0x1000, need - 1), (0x1010, need)):
+            with pytest.raises(_native.TcxInvalidArgument, match=f"scratch of {need} bytes"):
+                _native.call("tcx_kv_attention", ctypes.byref(a), scratch, size, None)
+    assert L.tcx_kv_attention_scratch_bytes(ctypes.byref(attention_args(head_dim=96))) == 0
+    assert L.tcx_kv_attention_scratch_bytes(None) == 0
 
 
 def test_attention_entry_without_work():
