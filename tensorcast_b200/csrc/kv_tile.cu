@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   using L = TileLayout<D>;
   constexpr uint32_t kStages = L::kStages;
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t s_bar[2 * kStages + 10];
+  __shared__ uint64_t s_bar[2 * kStages + 12];
   __shared__ uint32_t s_tmem, s_gave_up, s_drained, s_last;
   __shared__ __align__(16) int s_seen[2][8][4];
   const AttnArgs& a = d.a;
@@ -285,15 +285,16 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   auto full_phase = [&](uint32_t pair) { return pair / kPairs & 1; };
   auto empty = [&](uint32_t i) { return smem_addr(&s_bar[kPairs + i]); };
   auto bar = [&](uint32_t kind, uint32_t half) { return smem_addr(&s_bar[kPairs + kStages + kind * 2 + half]); };
-  enum : uint32_t { kQueries, kScored, kWeighed, kWeighedAll, kSummed };
+  enum : uint32_t { kQueries, kScoredLow, kScoredHigh, kHighRead, kWeighed, kSummed };
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < kPairs; ++i) mbar_init(full(i), 2);
-    for (uint32_t i = 0; i < kStages; ++i) mbar_init(empty(i), 1);
+    for (uint32_t i = 0; i < kStages; ++i) mbar_init(empty(i), 2);  // one arrival for each half
     for (uint32_t h = 0; h < 2; ++h) {
       mbar_init(bar(kQueries, h), 4);  // a warp's lane for all of them
-      mbar_init(bar(kScored, h), 1);
+      mbar_init(bar(kScoredLow, h), 1);
+      mbar_init(bar(kScoredHigh, h), 1);
+      mbar_init(bar(kHighRead, h), 4);
       mbar_init(bar(kWeighed, h), 4);
-      mbar_init(bar(kWeighedAll, h), 4);
       mbar_init(bar(kSummed, h), 1);
     }
     s_gave_up = s_drained = 0;
@@ -381,55 +382,34 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       // No copy may be in flight when the CTA ends.
       for (uint32_t p = last > kStages / 2 ? last - kStages / 2 : 0; p <= last; ++p)
         mbar_wait_warp(full(p), full_phase(p), &s_drained, a.status);
-    } else if (warp == 8) {  // ---- the products
-      constexpr uint32_t kScoreShape = mma_shape<T>(kTokens, false), kValueShape = mma_shape<T>(D, true);
-      const uint32_t tm = __shfl_sync(~0u, tmem, 0);
-      const uint64_t q_operand = smem_operand(base, 16, 1024), k_operand = smem_operand(ring, 16, 1024),
-                     v_operand = smem_operand(ring, L::kBlock, 1024);
-      uint32_t slot_at = 0, pieces[2] = {0, 0}, done[2] = {0, 0};
+    } else if (warp == 8 || warp == 10) {  // ---- the products of half `h`
+      // The tensor cores queue about two products, and a wait costs as long as two even
+      // where the barrier is there: two warps issue, one for each half.
+      constexpr uint32_t kScoreShape = mma_shape<T>(kTokens / 2, false), kValueShape = mma_shape<T>(D, true);
+      const uint32_t h = warp == 10, tm = __shfl_sync(~0u, tmem, 0);
+      const uint64_t q_operand = smem_operand(base + h * L::kOperand, 16, 1024),
+                     k_operand = smem_operand(ring, 16, 1024), v_operand = smem_operand(ring, L::kBlock, 1024);
+      const uint32_t scores = tm + L::kScores + h * kTokens, sums = tm + L::kSums + h * D;
+      uint32_t slot_at = 0, pieces = 0, done = 0;
       auto wait = [&](uint32_t b, uint32_t phase) {
         const bool there = mbar_wait_warp(b, phase & 1, &s_gave_up, a.status);
         tmem_fence_after();
         return there;
       };
-      // Scores of half h: its queries x the keys at `slot`. An operand's place is its
-      // descriptor's low bits, in 16-byte units.
-      auto score = [&](uint32_t h, uint32_t slot) {
-        const uint64_t q = q_operand + h * (L::kOperand / 16), k = k_operand + slot % kStages * (L::kOperand / 16);
+      // Scores: the half's queries x the first (high 0) or last 64 keys at `slot`, which
+      // the first ones' give back. An operand's place is its descriptor's low bits, in
+      // 16-byte units.
+      auto score = [&](uint32_t slot, uint32_t high) {
+        const uint64_t k = k_operand + slot % kStages * (L::kOperand / 16) + high * (64 * 128 / 16);
         if (elect_one()) {
 #pragma unroll
           for (int e = 0; e < D / 16; ++e) {
             const uint32_t off = e / 4 * (L::kBlock / 16) + e % 4 * 2;
-            mma_ss(tm + L::kScores + h * kTokens, q + off, k + off, kScoreShape, e > 0);
+            mma_ss(scores + high * 64, q_operand + off, k + off, kScoreShape, e > 0);
           }
-          mma_commit(bar(kScored, h));
+          mma_commit(bar(high ? kScoredHigh : kScoredLow, h));
+          if (!high) mma_commit(empty(slot % kStages));
         }
-        __syncwarp();
-      };
-      // Sums of half h: its probabilities x the values. The last quarter of the
-      // probabilities follows the others.
-      auto value = [&](uint32_t h, uint32_t slot, bool add, bool last) {
-        const uint64_t v = v_operand + slot % kStages * (L::kOperand / 16);
-        const uint32_t phase = done[h]++;
-        constexpr int kSteps = kTokens / 16, kEarly = kSteps * 3 / 4;
-        auto steps = [&](int from, int to) {
-#pragma unroll
-          for (int j = from; j < to; ++j)
-            mma_ts(tm + L::kSums + h * D, tm + L::kScores + h * kTokens + j * 8, v + j * 128, kValueShape, add || j > 0);
-        };
-        if (!wait(bar(kWeighed, h), phase)) return false;
-        if (elect_one()) steps(0, kEarly);
-        __syncwarp();
-        if (!wait(bar(kWeighedAll, h), phase)) return false;
-        if (elect_one()) {
-          steps(kEarly, kSteps);
-          if (last) mma_commit(bar(kSummed, h));
-        }
-        __syncwarp();
-        return true;
-      };
-      auto release = [&](uint32_t slot) {
-        if (elect_one()) mma_commit(empty(slot % kStages));
         __syncwarp();
       };
       auto uniform = [&](uint32_t x) { return __shfl_sync(~0u, x, 0); };
@@ -438,32 +418,43 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       next = item_of(next_item);
       at = uniform(at);
       head = uniform(head);
-      for (uint32_t left = uniform(count); left > 0;) {
+      bool alive = true;
+      for (uint32_t left = uniform(count); left > 0 && alive;) {
         const uint32_t n = min(tiles - at, left);
-        const bool two = rows > kHalfRows;
-        bool alive = wait(bar(kQueries, 0), pieces[0]++) && wait(full(slot_at / 2), full_phase(slot_at / 2));
-        if (!alive) break;
-        score(0, slot_at);
-        if (two) {
-          if (!wait(bar(kQueries, 1), pieces[1]++)) break;
-          score(1, slot_at);
-        }
-        release(slot_at);
-        for (uint32_t j = 0; j < n; ++j, slot_at += 2) {
-          const uint32_t v = slot_at + 1, k = slot_at + 2;
-          const bool more = j + 1 < n;
-          alive = wait(full(k / 2), full_phase(k / 2)) && value(0, v, j > 0, !more);  // both places are there
+        if (rows > h * kHalfRows) {
+          alive = wait(bar(kQueries, h), pieces++) && wait(full(slot_at / 2), full_phase(slot_at / 2));
           if (!alive) break;
-          if (more) score(0, k);
-          if (two) alive = value(1, v, j > 0, !more);
-          if (!alive) break;
-          release(v);
-          if (more) {
-            if (two) score(1, k);
-            release(k);
+          score(slot_at, 1);
+          score(slot_at, 0);
+          for (uint32_t j = 0; j < n; ++j, ++done, slot_at += 2) {
+            const uint32_t slot = slot_at + 1, k = slot_at + 2;
+            const bool more = j + 1 < n;
+            // The next scores of the last 64 tokens follow once these are read, those of
+            // the first 64, whose place the probabilities take, behind the sums.
+            alive = wait(full(k / 2), full_phase(k / 2));  // both places are there
+            if (alive && more) {
+              alive = wait(bar(kHighRead, h), done);
+              if (alive) score(k, 1);
+            }
+            alive = alive && wait(bar(kWeighed, h), done);
+            if (!alive) break;
+            const uint64_t v = v_operand + slot % kStages * (L::kOperand / 16);
+            if (elect_one()) {
+#pragma unroll
+              for (int i = 0; i < kTokens / 16; ++i)
+                mma_ts(sums, scores + i * 8, v + i * 128, kValueShape, j > 0 || i > 0);
+              mma_commit(empty(slot % kStages));
+              if (!more) mma_commit(bar(kSummed, h));
+            }
+            __syncwarp();
+            if (more) score(k, 0);
+          }
+        } else {  // no rows here: the tiles pass by
+          for (uint32_t i = 0; i < 2 * n && alive; ++i, ++slot_at) {
+            alive = wait(full((slot_at + 1) / 2), full_phase((slot_at + 1) / 2));
+            mbar_arrive_warp(empty(slot_at % kStages), lane, alive);
           }
         }
-        if (!alive) break;
         left -= n;
         at = 0;
         if (++head == a.kv_heads) {
@@ -565,118 +556,163 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       if (active) {
         for (uint32_t j = 0; j < n; ++j, ++done) {
           const int token = first_token(it, at + j);
-          wait(bar(kScored, h), done);
-          tmem_fence_after();
-          if (j + 1 == n) fetch_next();
-          uint32_t z[kTokens];
-          tmem_load128(z, scores);
-          bool plain = true;
-          if (token + kTokens - 1 > all_hi || (token < all_lo && token + kTokens > it.sinks)) {
-            plain = false;
-            // bits of the tile's tokens below x
-            auto below = [&](int x, int word) {
-              const int n_bits = min(max(x - token - word * 32, 0), 32);
+          const bool masked = token + kTokens - 1 > all_hi || (token < all_lo && token + kTokens > it.sinks);
+          // Scores that this row does not see become -inf: tokens from `from` on.
+          auto hide = [&](uint32_t (&z)[kTokens / 2], int from) {
+            auto below = [&](int x, int word) {  // bits of the word's tokens below x
+              const int n_bits = min(max(x - from - word * 32, 0), 32);
               return n_bits == 32 ? ~0u : (1u << n_bits) - 1;
             };
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+            for (int w = 0; w < 2; ++w) {
               const uint32_t see = below(hi + 1, w) & (~below(lo, w) | below(it.sinks, w));
 #pragma unroll
               for (int i = 0; i < 32; ++i)
                 if (!(see >> i & 1)) z[w * 32 + i] = 0xff800000u;
             }
-            // values that no row sees are cleared: 0 x NaN is not 0
-            if (h == 0 && (token + kTokens - 1 > any_hi || (token < any_lo && token + kTokens > it.sinks))) {
-              const uint32_t v = 2 * (tiles_done + j) + 1;
-              wait(full((v + 1) / 2), full_phase((v + 1) / 2));
-              const int mine = token + static_cast<int>(r);
-              if (mine > any_hi || (mine < any_lo && mine >= it.sinks)) {
-                const uint32_t to = ring + v % kStages * L::kOperand + r * 128;
-#pragma unroll
-                for (int c = 0; c < D / 8; ++c)
-                  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + c / 8 * L::kBlock +
-                                                                               ((c % 8 ^ (r & 7)) << 4)),
-                               "r"(0)
-                               : "memory");
-              }
-              proxy_fence_smem();
-              __syncwarp();
-            }
-          }
-          auto largest = [&] {
+          };
+          auto largest = [&](const uint32_t (&z)[kTokens / 2]) {
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < kTokens; i += 2)
+            for (int i = 0; i < kTokens / 2; i += 2)
               top[i / 2 % 4] = max3_nan(top[i / 2 % 4], __uint_as_float(z[i]), __uint_as_float(z[i + 1]));
             return max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
           };
           const float2 c2 = make_float2(a.scale_log2, a.scale_log2);
-          float2 sum[2];
-          // Probabilities of 32 tokens, in place of their scores. Mixed: every eighth
-          // pair's exponentials run on the FMA units, since the exponential units
-          // alone need as long as the products do.
-          auto weigh = [&](int c, auto mixed) {
-            const float ref = m == -INFINITY ? 0.f : m;
-            const float2 ref2 = make_float2(-ref, -ref);
-            uint32_t p[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int k = c * 32 + 2 * i;
-              float2 x = fma2(make_float2(__uint_as_float(z[k]), __uint_as_float(z[k + 1])), c2, ref2);
-              if (decltype(mixed)::value && i % 8 == 7) {
-                x = exp2_fma(x);
-              } else {
-                x.x = exp2_approx(x.x);
-                x.y = exp2_approx(x.y);
-              }
-              sum[i % 2] = add2(sum[i % 2], x);
-              p[i] = pack2<T>(x.x, x.y);
-            }
-            tmem_store16(scores + c * 16, p);
+          // 2^(z - m) of a pair, on the exponential units or (mixed: every eighth pair)
+          // the FMA units, since the exponential units alone need nearly as long as
+          // the products do.
+          auto weigh = [&](uint32_t z0, uint32_t z1, int i, float ref, auto mixed) {
+            float2 x = fma2(make_float2(__uint_as_float(z0), __uint_as_float(z1)), c2, make_float2(-ref, -ref));
+            if (decltype(mixed)::value && i % 8 == 7) return exp2_fma(x);
+            return make_float2(exp2_approx(x.x), exp2_approx(x.y));
           };
-          // A tile that all rows see whole is weighed by the maximum so far at once,
-          // while its own is found; it is weighed again where that has grown too far.
-          bool again = true;
-          float top;
-          if (plain && !__any_sync(~0u, m == -INFINITY)) {
-            sum[0] = sum[1] = make_float2(0.f, 0.f);
+          auto reference = [&] { return m == -INFINITY ? 0.f : m; };
+          float f = 1.f;  // what the sums so far are scaled by
+          auto grow = [&](float top) {
+            const float old = m, by = top > m + 8.f ? exp2_approx(old - top) : 1.f;
+            if (top > m + 8.f) m = top;
+            f *= by;
+            return by;
+          };
+
+          // The last 64 tokens, whose scores were there early.
+          float2 e[kTokens / 4], sum_e = make_float2(0.f, 0.f), sum_z = make_float2(0.f, 0.f);
+          bool odd;  // a score that only the exponential units take: masked, infinite or NaN
+          {
+            wait(bar(kScoredHigh, h), done);
+            tmem_fence_after();
+            uint32_t z[kTokens / 2];
+            tmem_load64(z, scores + kTokens / 2);
+            tmem_fence_before();
+            mbar_arrive_warp(bar(kHighRead, h), lane, alive);
+            if (masked) hide(z, token + kTokens / 2);
+            const float top = largest(z);
+            grow(top);
+            odd = masked || __any_sync(~0u, !(fabsf(top) < INFINITY));
+            const float ref = reference();
+            auto all = [&](auto mixed) {
 #pragma unroll
-            for (int c = 0; c < 3; ++c) weigh(c, std::true_type{});
-            top = largest();
-            again = __any_sync(~0u, !(top <= m + 8.f));
-          } else {
-            top = largest();
+              for (int i = 0; i < kTokens / 4; ++i) {
+                e[i] = weigh(z[2 * i], z[2 * i + 1], i, ref, mixed);
+                sum_e = add2(sum_e, e[i]);
+              }
+            };
+            if (odd) all(std::false_type{}); else all(std::true_type{});
           }
-          if (again) {
-            const bool grown = top > m + 8.f;
-            if (__any_sync(~0u, grown)) {
-              const float old = m;
-              if (grown) m = top;
-              const float f = grown ? exp2_approx(old - m) : 1.f;
-              l *= f;
-              if (j > 0) {  // these scores are there, so the sums before them are done
-                for (int c = 0; c < D; c += 32) {
-                  uint32_t o[32];
-                  tmem_load32(o, sums + c);
+          auto store_high = [&] {
 #pragma unroll
-                  for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                  tmem_store32(sums + c, o);
+            for (int c = 0; c < 2; ++c) {
+              uint32_t p[16];
+#pragma unroll
+              for (int i = 0; i < 16; ++i) p[i] = pack2<T>(e[c * 16 + i].x, e[c * 16 + i].y);
+              tmem_store16(scores + kTokens / 4 + c * 16, p);
+            }
+          };
+
+          // The first 64 tokens. All probabilities take the place of their scores.
+          {
+            wait(bar(kScoredLow, h), done);
+            tmem_fence_after();
+            if (j + 1 == n) fetch_next();
+            uint32_t z[kTokens / 2];
+            tmem_load64(z, scores);
+            if (masked) {
+              hide(z, token);
+              // Values that no row sees are cleared (0 x NaN is not 0), half of them by
+              // each half of the rows; both come here, and neither goes on alone.
+              if (token + kTokens - 1 > any_hi || (token < any_lo && token + kTokens > it.sinks)) {
+                const uint32_t v = 2 * (tiles_done + j) + 1, of = r % kHalfRows, halves = it.rows > kHalfRows ? 2 : 1;
+                wait(full((v + 1) / 2), full_phase((v + 1) / 2));
+                const int mine = token + static_cast<int>(of);
+                if (mine > any_hi || (mine < any_lo && mine >= it.sinks)) {
+                  const uint32_t to = ring + v % kStages * L::kOperand + of * 128;
+                  for (uint32_t c = h; c < D / 8; c += halves)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + c / 8 * L::kBlock +
+                                                                                 ((c % 8 ^ (of & 7)) << 4)),
+                                 "r"(0)
+                                 : "memory");
                 }
+                proxy_fence_smem();
+                if (halves == 2)
+                  asm volatile("bar.sync 2, 256;" ::: "memory");
+                else
+                  __syncwarp();
               }
             }
-            sum[0] = sum[1] = make_float2(0.f, 0.f);
+            store_high();
+            auto all = [&](auto mixed) {
+              const float ref = reference();
+              sum_z = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < 3; ++c) weigh(c, std::false_type{});
+              for (int c = 0; c < 2; ++c) {
+                uint32_t p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                  const int k = c * 32 + 2 * i;
+                  const float2 x = weigh(z[k], z[k + 1], i, ref, mixed);
+                  sum_z = add2(sum_z, x);
+                  p[i] = pack2<T>(x.x, x.y);
+                }
+                tmem_store16(scores + c * 16, p);
+              }
+            };
+            // Where all rows see them whole they are weighed by the maximum so far at
+            // once, while their own is found, and again where that has grown too far.
+            bool again = true;
+            float top;
+            if (!odd) {
+              all(std::true_type{});
+              top = largest(z);
+              again = __any_sync(~0u, !(top <= m + 8.f));
+            } else {
+              top = largest(z);
+            }
+            if (again) {
+              const float by = grow(top);
+              if (__any_sync(~0u, by != 1.f)) {
+#pragma unroll
+                for (int i = 0; i < kTokens / 4; ++i) e[i] = make_float2(e[i].x * by, e[i].y * by);
+                sum_e = make_float2(sum_e.x * by, sum_e.y * by);
+                store_high();
+              }
+              all(std::false_type{});
+            }
+          }
+          if (__any_sync(~0u, f != 1.f) && j > 0) {  // these scores are there, so the sums before them are done
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_load32(o, sums + c);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+              tmem_store32(sums + c, o);
+            }
           }
           tmem_wait_store();
           tmem_fence_before();
           mbar_arrive_warp(bar(kWeighed, h), lane, alive);
-          weigh(3, std::false_type{});
-          tmem_wait_store();
-          tmem_fence_before();
-          mbar_arrive_warp(bar(kWeighedAll, h), lane, alive);
-          sum[0] = add2(sum[0], sum[1]);
-          l += sum[0].x + sum[0].y;
+          sum_e = add2(sum_e, sum_z);
+          l = l * f + (sum_e.x + sum_e.y);
         }
         wait(bar(kSummed, h), summed++);
         tmem_fence_after();
