@@ -579,12 +579,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             return max3_nan(max3_nan(top[0], top[1], top[2]), top[3], top[3]) * a.scale_log2;
           };
           const float2 c2 = make_float2(a.scale_log2, a.scale_log2);
-          // 2^(z - m) of a pair, on the exponential units or (mixed: every eighth pair)
+          // 2^(z - m) of a pair, on the exponential units or (mixed: every fourth pair)
           // the FMA units, since the exponential units alone need nearly as long as
           // the products do.
           auto weigh = [&](uint32_t z0, uint32_t z1, int i, float ref, auto mixed) {
             float2 x = fma2(make_float2(__uint_as_float(z0), __uint_as_float(z1)), c2, make_float2(-ref, -ref));
-            if (decltype(mixed)::value && i % 8 == 7) return exp2_fma(x);
+            if (decltype(mixed)::value && i % 4 == 3) return exp2_fma(x);
             return make_float2(exp2_approx(x.x), exp2_approx(x.y));
           };
           auto reference = [&] { return m == -INFINITY ? 0.f : m; };
