@@ -146,8 +146,7 @@ using namespace tcx;
 extern "C" uint64_t tcx_kv_attention_scratch_bytes(const tcx_kv_attention_args* args) {
   if (args == nullptr || args->n_seq == 0 || args->q_tokens == 0 || check_sizes(*args) != TCX_OK) return 0;
   uint64_t own = decode_fits(*args) ? decode_scratch_bytes(*args) : tile_scratch_bytes(*args, false);
-  if (args->d_prefix_table != nullptr)  // the two run one after the other
-    own = std::max(own, tile_scratch_bytes(*args, true)) + prior_bytes(*args);
+  if (args->d_prefix_table != nullptr) own += tile_scratch_bytes(*args, true) + prior_bytes(*args);
   return own;
 }
 
@@ -170,6 +169,7 @@ extern "C" tcx_status tcx_kv_attention(const tcx_kv_attention_args* args, void* 
     a.part_lse = a.part_o + args->q_tokens * args->q_heads * args->head_dim;
     scratch += prior_bytes(*args);
     if (const tcx_status st = launch_tile(*args, a, map, true, scratch, s); st != TCX_OK) return st;
+    scratch += tile_scratch_bytes(*args, true);
     a.prior_o = a.part_o;
     a.prior_lse = a.part_lse;
     a.part_o = a.part_lse = nullptr;

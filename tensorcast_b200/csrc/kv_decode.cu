@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t head = blockIdx.x % a.kv_heads, range = blockIdx.x / a.kv_heads;
   const uint32_t base = (smem_addr(raw) + 1023) & ~1023u;
+  next_may_start();
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(smem_addr(&s_full[i]), 1);
@@ -369,6 +370,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       }
     }
     if (info.flags & kLast) {
+      wait_for_previous();  // the rows' parts over a shared prefix
       // The four warps' parts are joined in this tile's memory, which all have read.
       const uint32_t rows = min(info.queries * a.group, static_cast<uint32_t>(kRows));
 #pragma unroll
@@ -437,6 +439,7 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(DecodeArgs d) {
   __shared__ float s_lse[kRows];
   const uint32_t rows = min(queries * a.group, d.score_rows);
   if (rows == 0) return;
+  wait_for_previous();
   if (threadIdx.x < rows)
     s_lse[threadIdx.x] = kLog2e * a.lse[(q_first + threadIdx.x / a.group) * static_cast<uint64_t>(a.kv_heads) * a.group +
                                         head * a.group + threadIdx.x % a.group];
@@ -457,10 +460,11 @@ __global__ void __launch_bounds__(256) decode_weights_kernel(DecodeArgs d) {
   }
 }
 
-// Two CTAs fit an SM. Each range and head needs a counter, where there are ranges to join.
+// Two CTAs fit an SM. Each range and head needs a counter where there are ranges to
+// join; the other half of the counters is the tile kernel's, which may still run.
 uint32_t decode_ranges(const tcx_kv_attention_args& x) {
   const uint64_t tiles = x.total_pages * x.page_tokens / kTile + x.n_seq;
-  const uint64_t most = std::min<uint64_t>(2ull * sm_count(), TCX_KV_COUNTERS) / x.kv_heads;
+  const uint64_t most = std::min<uint64_t>(2ull * sm_count(), TCX_KV_COUNTERS / 2) / x.kv_heads;
   return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((tiles + 2) / 3, most)));
 }
 
@@ -471,16 +475,20 @@ tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint64_t max_toke
   if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(decode_kernel<T, D, kScores>), L::kBytes, &allowed);
       st != TCX_OK)
     return st;
-  decode_kernel<T, D, kScores><<<d.ranges * d.a.kv_heads, kThreads, L::kBytes, stream>>>(map, d);
-  note_launches(1);
-  TCX_CUDA_TRY(cudaGetLastError());
-  if (kScores && max_tokens > 0) {
-    const uint64_t blocks = std::min<uint64_t>((max_tokens + 255) / 256, 64);
-    decode_weights_kernel<<<dim3(static_cast<unsigned>(blocks), d.a.kv_heads, d.a.n_seq), 256, 0, stream>>>(d);
+  const dim3 grid(d.ranges * d.a.kv_heads);
+  if (d.a.prior_o != nullptr) {  // behind the shared prefix's kernels
+    if (const tcx_status st = launch_after(decode_kernel<T, D, kScores>, grid, dim3(kThreads), L::kBytes, stream, map, d);
+        st != TCX_OK)
+      return st;
+  } else {
+    decode_kernel<T, D, kScores><<<grid, kThreads, L::kBytes, stream>>>(map, d);
     note_launches(1);
     TCX_CUDA_TRY(cudaGetLastError());
   }
-  return TCX_OK;
+  if (!kScores || max_tokens == 0) return TCX_OK;
+  const uint64_t blocks = std::min<uint64_t>((max_tokens + 255) / 256, 64);
+  return launch_after(decode_weights_kernel, dim3(static_cast<unsigned>(blocks), d.a.kv_heads, d.a.n_seq), dim3(256), 0,
+                      stream, d);
 }
 
 template <typename T, int D>

@@ -12,6 +12,7 @@
 
 #include <algorithm>
 
+#include "sm100.cuh"
 #include "tcx_internal.h"
 
 namespace tcx {
@@ -87,6 +88,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
   __shared__ uint32_t bins[kBins], warp_sums[kSelectThreads / 32], s_pick[2];
   const uint32_t head = blockIdx.x, layer = blockIdx.y, s = blockIdx.z;
+  next_may_start();
   uint32_t n, kept;
   lengths(a, s, &n, &kept);
   const uint64_t base = a.page_offsets[s] * a.page_tokens, dst_base = a.dst_page_offsets[s] * a.page_tokens;
@@ -181,6 +183,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(EvictArgs a) {
   const uint64_t plane_off = plane * a.pool_pages * a.page_bytes;
   const uint32_t* table = a.page_table + a.page_offsets[lo];
   const int32_t* keep = a.keep + static_cast<uint64_t>(plane / 2) * a.kv_heads * a.dst_capacity + page * a.page_tokens;
+  wait_for_previous();  // the kept indices
   const uint32_t pieces = static_cast<uint32_t>(a.head_bytes / 16), per_token = pieces * a.kv_heads;
   for (uint32_t i = threadIdx.x; i < rows * per_token; i += blockDim.x) {
     const uint32_t r = i / per_token, head = i % per_token / pieces, piece = i % pieces;
@@ -258,9 +261,7 @@ extern "C" tcx_status tcx_kv_evict(const tcx_kv_evict_args* args, void* stream) 
   TCX_CUDA_TRY(cudaGetLastError());
   if (x.dst_total_pages != 0) {
     const dim3 copy_grid(static_cast<unsigned>(x.dst_total_pages), static_cast<unsigned>(x.planes));
-    copy_kernel<<<copy_grid, kCopyThreads, 0, s>>>(a);
-    note_launches(1);
-    TCX_CUDA_TRY(cudaGetLastError());
+    return launch_after(copy_kernel, copy_grid, dim3(kCopyThreads), 0, s, a);
   }
   return TCX_OK;
 }

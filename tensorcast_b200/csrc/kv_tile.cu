@@ -142,6 +142,8 @@ __global__ void __launch_bounds__(kPlanThreads) tile_plan_kernel(TileArgs d) {
   __shared__ uint64_t s_sums[kPlanThreads / 32], s_units[kPlanCache];
   __shared__ uint32_t s_first[kPlanCache];
   const AttnArgs& a = d.a;
+  next_may_start();
+  wait_for_previous();
   const int prefix = static_cast<int>(prefix_length(a));
   uint64_t total;
   uint32_t items;
@@ -300,6 +302,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     s_gave_up = s_drained = 0;
     mbar_init_fence();
   }
+  next_may_start();
+  wait_for_previous();
   // The work: its row tiles, where the ranges begin, and this one.
   const int prefix = static_cast<int>(prefix_length(a));
   uint32_t items, ranges;
@@ -809,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         --from;
         --to;
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (threadIdx.x == 0) s_last = alive && last_to_arrive(a.counters + from, to - from + 1);
+        if (threadIdx.x == 0) s_last = alive && last_to_arrive(a.counters + TCX_KV_COUNTERS / 2 + from, to - from + 1);
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (s_last) join_rows<T, D>(d, it, head, from, to, begin_of(from).unit != first, warp, lane);
       }
@@ -837,6 +841,8 @@ __global__ void __launch_bounds__(256) tile_join_kernel(TileArgs d) {
   constexpr int E = D / 32;
   const AttnArgs& a = d.a;
   const uint32_t range = blockIdx.x, r = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
+  next_may_start();
+  wait_for_previous();
   const RangeEnd own = d.end[range];
   if (!own.goes_on || !own.starts) return;
   const Item it = d.prefix ? make_item(d, 0, own.item, static_cast<int>(prefix_length(a))) : d.items[own.item];
@@ -892,7 +898,7 @@ uint64_t max_items(const tcx_kv_attention_args& x, bool prefix) {
 uint32_t max_ranges(const tcx_kv_attention_args& x, bool prefix) {
   const uint64_t pages = prefix ? x.prefix_pages : x.max_pages;
   const uint64_t units = max_items(x, prefix) * x.kv_heads * (pages * x.page_tokens / kTokens + 2);
-  return static_cast<uint32_t>(std::min<uint64_t>({static_cast<uint64_t>(sm_count()), units, TCX_KV_COUNTERS}));
+  return static_cast<uint32_t>(std::min<uint64_t>({static_cast<uint64_t>(sm_count()), units, TCX_KV_COUNTERS / 2}));
 }
 
 struct Parts {
@@ -927,20 +933,26 @@ tcx_status launch(const TileArgs& d, const CUtensorMap& map, cudaStream_t stream
   if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(tile_kernel<T, D>), L::kBytes, &allowed);
       st != TCX_OK)
     return st;
-  if (!d.prefix) {
-    tile_plan_kernel<<<1, kPlanThreads, 0, stream>>>(d);
+  // The first kernel of the call follows the stream's earlier work whole.
+  if (d.prefix) {
+    tile_kernel<T, D><<<d.max_ranges, kThreads, L::kBytes, stream>>>(map, d);
     note_launches(1);
     TCX_CUDA_TRY(cudaGetLastError());
+  } else {
+    if (d.a.prior_o != nullptr) {
+      if (const tcx_status st = launch_after(tile_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, d); st != TCX_OK)
+        return st;
+    } else {
+      tile_plan_kernel<<<1, kPlanThreads, 0, stream>>>(d);
+      note_launches(1);
+      TCX_CUDA_TRY(cudaGetLastError());
+    }
+    if (const tcx_status st = launch_after(tile_kernel<T, D>, dim3(d.max_ranges), dim3(kThreads), L::kBytes, stream, map, d);
+        st != TCX_OK)
+      return st;
   }
-  tile_kernel<T, D><<<d.max_ranges, kThreads, L::kBytes, stream>>>(map, d);
-  note_launches(1);
-  TCX_CUDA_TRY(cudaGetLastError());
-  if (d.max_ranges > 1 && !d.join_here) {
-    tile_join_kernel<T, D><<<dim3(d.max_ranges - 1, kRows / 8), 256, 0, stream>>>(d);
-    note_launches(1);
-    TCX_CUDA_TRY(cudaGetLastError());
-  }
-  return TCX_OK;
+  if (d.max_ranges == 1 || d.join_here) return TCX_OK;
+  return launch_after(tile_join_kernel<T, D>, dim3(d.max_ranges - 1, kRows / 8), dim3(256), 0, stream, d);
 }
 
 }  // namespace

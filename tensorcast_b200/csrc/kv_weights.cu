@@ -70,6 +70,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
     s_gave_up = s_drained = 0;
     mbar_init_fence();
   }
+  wait_for_previous();  // the rows' sums, and the tensor memory of the kernel before
   if (warp == kWorkers / 32) tmem_alloc(smem_addr(&s_tmem), 2 * kRows);
   tmem_fence_before();
   __syncthreads();
@@ -203,10 +204,7 @@ tcx_status launch(const AttnArgs& a, const CUtensorMap& map, uint64_t max_tokens
       st != TCX_OK)
     return st;
   const dim3 grid(static_cast<unsigned>((max_tokens + kKeys - 1) / kKeys), a.kv_heads, a.n_seq);
-  weights_kernel<T, D><<<grid, kThreads, L::kBytes, stream>>>(map, a);
-  note_launches(1);
-  TCX_CUDA_TRY(cudaGetLastError());
-  return TCX_OK;
+  return launch_after(weights_kernel<T, D>, grid, dim3(kThreads), L::kBytes, stream, map, a);
 }
 
 }  // namespace

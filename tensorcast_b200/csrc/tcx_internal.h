@@ -60,3 +60,29 @@ inline std::string cuda_msg(cudaError_t e) {
       return ::tcx::set_error(TCX_INTERNAL, std::string(#call " failed: ") + ::tcx::cuda_msg(tcx_e_)); \
     }                                                                                              \
   } while (0)
+
+namespace tcx {
+
+// Launches a kernel that waits for the one before it in its own code
+// (griddepcontrol.wait, in every thread that uses that one's memory or writes where it
+// may still read), so that its set-up runs beside that one's end. The first kernel of
+// a call is launched without: it follows all earlier work of the stream.
+template <typename... Params, typename... Args>
+tcx_status launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream,
+                        const Args&... args) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  TCX_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, args...));
+  note_launches(1);
+  return TCX_OK;
+}
+
+}  // namespace tcx

@@ -177,6 +177,9 @@ class KvAttention(_OnDevice):
             else t.prefix_table.data_ptr(), prefix_pages=pages.size, d_prefix_tokens=t.prefix_tokens.data_ptr(),
             window=window, sinks=sinks, scale=scale, d_status=t.status.data_ptr())
         self._shape = (q_heads, head_dim)
+        # what new outputs are like (no memory of their own: cheaper to allocate by than by a shape)
+        self._out_like = torch.empty(1, dtype=dtype, device=self.device).expand(self._args.q_tokens, *self._shape)
+        self._lse_like = torch.empty(1, device=self.device).expand(self._args.q_tokens, q_heads)
         self._scratch_bytes = {}  # with and without weights
         self._workspaces = {}     # scratch and counters, by stream
 
@@ -238,7 +241,8 @@ class KvAttention(_OnDevice):
         rows = q.shape[0]
         padded = rows > a.q_tokens
         if out is None:
-            out = (torch.zeros if padded else torch.empty)((rows, *self._shape), dtype=self.dtype, device=self.device)
+            out = torch.empty_like(self._out_like) if not padded else torch.zeros(
+                (rows, *self._shape), dtype=self.dtype, device=self.device)
             a.d_out, a.out_token_stride, a.out_head_stride = out.data_ptr(), *out.stride()[:2]
         else:
             a.d_out, a.out_token_stride, a.out_head_stride = self._rows(out, "out")
@@ -246,8 +250,8 @@ class KvAttention(_OnDevice):
                                                     pool.untyped_storage().data_ptr()):
                 _refuse("out must not share memory with q or the pool")
         if lse is None:
-            lse = (torch.zeros if padded else torch.empty)((rows, self.q_heads), dtype=torch.float32,
-                                                           device=self.device)
+            lse = torch.empty_like(self._lse_like) if not padded else torch.zeros((rows, self.q_heads),
+                                                                                  device=self.device)
         elif (lse.dtype != torch.float32 or lse.device != self.device or not lse.is_contiguous() or lse.dim() != 2
               or lse.shape[0] < a.q_tokens or lse.shape[1] != self.q_heads):
             _refuse(f"lse must be contiguous float32 [>= {a.q_tokens}, {self.q_heads}] on {self.device}")
@@ -255,10 +259,11 @@ class KvAttention(_OnDevice):
         if weights is not None:
             if self.prefix_tokens is not None:
                 _refuse("weights are not accumulated with a shared prefix")
-            if (weights.dtype != torch.float32 or weights.device != self.device
-                    or tuple(weights.shape) != (self.kv_heads, self.weight_columns)
-                    or (weights.numel() and weights.stride(1) != 1) or weights.stride(0) < self.weight_columns):
-                _refuse(f"weights must be float32 [{self.kv_heads}, {self.weight_columns}] on {self.device}, "
+            columns = self.weight_columns
+            if (weights.dtype != torch.float32 or weights.get_device() != self.device.index
+                    or weights.shape != (self.kv_heads, columns)
+                    or (columns and weights.stride(1) != 1) or weights.stride(0) < columns):
+                _refuse(f"weights must be float32 [{self.kv_heads}, {columns}] on {self.device}, "
                         "dense in its columns")
             a.d_weights, a.weights_head_stride = weights.data_ptr(), weights.stride(0)
         if a.q_tokens:
@@ -319,6 +324,12 @@ class KvEvict(_OnDevice):
             d_dst_page_table=t.dst_page_table.data_ptr() or t.buffer.data_ptr(),
             d_dst_page_offsets=t.dst_page_offsets.data_ptr(), d_budgets=t.budgets.data_ptr(), n_seq=w.n_seq,
             dst_total_pages=int(dst.page_offsets[-1]), sinks=sinks, recent=recent, d_status=t.status.data_ptr())
+        layers = w.planes // 2
+        self._weights_shape = (layers, kv_heads, int(w.page_offsets[-1]) * w.page_tokens)
+        shape = (layers, kv_heads, int(dst.page_offsets[-1]) * dst.page_tokens)
+        one = torch.zeros(1, dtype=torch.int32, device=self.device)
+        # what the outputs are like (no memory of their own)
+        self._like = one.expand(shape), one.float().expand(shape), one.expand(w.n_seq)
 
     def run(self, pool: torch.Tensor, weights: torch.Tensor, stream=None):
         """(keep, weights, tokens) after the eviction; the destination pages of ``pool`` are written.
@@ -331,20 +342,12 @@ class KvEvict(_OnDevice):
             return self._on(stream, lambda: self.run(pool, weights))
         a = _native.KvEvictArgs.from_buffer_copy(self._args)
         a.d_pool = self._pool(pool)
-        layers, columns = self.w.planes // 2, int(self.w.page_offsets[-1]) * self.w.page_tokens
-        if (weights.dtype != torch.float32 or weights.device != self.device
-                or tuple(weights.shape) != (layers, self.kv_heads, columns)
-                or (columns and weights.stride(2) != 1)):
-            _refuse(f"weights must be float32 [{layers}, {self.kv_heads}, {columns}] on {self.device}, "
-                    "dense in its columns")
-        if min(weights.stride()) < 0:
-            _refuse("weights must not have negative strides")
+        if (weights.dtype != torch.float32 or weights.get_device() != self.device.index
+                or weights.shape != self._weights_shape or (self._weights_shape[2] and weights.stride(2) != 1)):
+            _refuse(f"weights must be float32 {list(self._weights_shape)} on {self.device}, dense in its columns")
         a.d_weights = weights.data_ptr() or self._tables.buffer.data_ptr()
-        a.weights_layer_stride, a.weights_head_stride = weights.stride(0), weights.stride(1)
-        shape = (layers, self.kv_heads, int(self.dst.page_offsets[-1]) * self.dst.page_tokens)
-        keep = torch.empty(shape, dtype=torch.int32, device=self.device)
-        left = torch.empty(shape, dtype=torch.float32, device=self.device)
-        tokens = torch.empty(self.w.n_seq, dtype=torch.int32, device=self.device)
+        a.weights_layer_stride, a.weights_head_stride = weights.stride()[:2]
+        keep, left, tokens = (torch.empty_like(x) for x in self._like)
         a.d_keep, a.d_dst_weights, a.d_dst_tokens = keep.data_ptr(), left.data_ptr(), tokens.data_ptr()
         _native.call("tcx_kv_evict", ctypes.byref(a), self._current())
         return keep, left, tokens
