@@ -1,8 +1,6 @@
 // Arguments and lookups shared by the attention kernels over the paged KV pool.
 #pragma once
 
-#include <atomic>
-
 #include "sm100.cuh"
 #include "tcx_internal.h"
 
@@ -162,17 +160,6 @@ __device__ __forceinline__ bool last_to_arrive(uint32_t* counter, uint32_t parts
     __threadfence();
   }
   return last;
-}
-
-// Lets a kernel use `bytes` of dynamic shared memory, once for each device.
-inline tcx_status allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>* done) {
-  int dev = 0;
-  TCX_CUDA_TRY(cudaGetDevice(&dev));
-  const uint64_t bit = 1ull << (dev & 63);
-  if (dev < 64 && (done->load(std::memory_order_relaxed) & bit)) return TCX_OK;
-  TCX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-  if (dev < 64) done->fetch_or(bit, std::memory_order_relaxed);
-  return TCX_OK;
 }
 
 inline uint64_t align256(uint64_t n) { return (n + 255) / 256 * 256; }

@@ -166,7 +166,10 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   }
   // Three tiles are in flight at once: fewer in a range save no time, and leave more to join.
   const uint32_t ranges = min(d.ranges, (total + 2) / 3);
-  if (range >= ranges) return;
+  if (range >= ranges) {
+    wait_for_previous();
+    return;
+  }
   const uint32_t t0 = static_cast<uint32_t>(static_cast<uint64_t>(range) * total / ranges);
   const uint32_t t1 = static_cast<uint32_t>(static_cast<uint64_t>(range + 1) * total / ranges);
   if (before <= t0 && t0 < before + mine) {
@@ -431,32 +434,42 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   }
 }
 
-// A token's softmax weights, of the scores that decode_kernel left: one thread for
-// each token and kv head, the rows in their order.
-__global__ void __launch_bounds__(256) decode_weights_kernel(DecodeArgs d) {
+// The tokens' softmax weights, of the scores that decode_kernel left: a thread for
+// four tokens and a kv head, the rows in their order.
+__global__ void __launch_bounds__(128) decode_weights_kernel(DecodeArgs d) {
   const AttnArgs& a = d.a;
   const uint32_t s = blockIdx.z, head = blockIdx.y, q_first = a.q_offsets[s], queries = a.q_offsets[s + 1] - q_first;
   __shared__ float s_lse[kRows];
   const uint32_t rows = min(queries * a.group, d.score_rows);
-  if (rows == 0) return;
+  const SeqInfo q = seq_info(a, s, 0);
+  if (rows == 0 || static_cast<int>(blockIdx.x * 512) >= q.len) {
+    wait_for_previous();  // also here: this kernel's end stands for the one's before
+    return;
+  }
+  const uint64_t column = a.page_offsets[s] * a.page_tokens;
+  const float* z = d.scores + static_cast<uint64_t>(head) * d.score_rows * d.columns + column;
+  float* w = a.weights + head * a.weights_head_stride + column;
   wait_for_previous();
   if (threadIdx.x < rows)
     s_lse[threadIdx.x] = kLog2e * a.lse[(q_first + threadIdx.x / a.group) * static_cast<uint64_t>(a.kv_heads) * a.group +
                                         head * a.group + threadIdx.x % a.group];
   __syncthreads();
-  const SeqInfo q = seq_info(a, s, 0);
-  const uint64_t column = a.page_offsets[s] * a.page_tokens;
-  const float* z = d.scores + static_cast<uint64_t>(head) * d.score_rows * d.columns + column;
-  float* w = a.weights + head * a.weights_head_stride + column;
-  for (int j = static_cast<int>(blockIdx.x * 256 + threadIdx.x); j < q.len; j += static_cast<int>(gridDim.x * 256)) {
-    if (j < q.low && j >= q.sinks) continue;  // no row sees it, and no tile held it
-    float sum = 0.f;
+  for (int j = static_cast<int>(blockIdx.x * 128 + threadIdx.x) * 4; j < q.len; j += static_cast<int>(gridDim.x * 512)) {
+    float sum[4] = {};
 #pragma unroll 4
     for (uint32_t r = 0; r < rows; ++r) {
-      const float lse = s_lse[r], x = z[r * d.columns + j];
-      sum += lse == -INFINITY ? 0.f : exp2f(x - lse);
+      const float lse = s_lse[r];
+      const float4 x = *reinterpret_cast<const float4*>(z + r * d.columns + j);  // whole pages: within the scratch
+      if (lse == -INFINITY) continue;
+      sum[0] += exp2_approx(x.x - lse);
+      sum[1] += exp2_approx(x.y - lse);
+      sum[2] += exp2_approx(x.z - lse);
+      sum[3] += exp2_approx(x.w - lse);
     }
-    w[j] += sum;
+    // Tokens between the sinks and the window are seen by no row, and no tile held them.
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (j + k < q.len && (j + k >= q.low || j + k < q.sinks)) w[j + k] += sum[k];
   }
 }
 
@@ -486,8 +499,8 @@ tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint64_t max_toke
     TCX_CUDA_TRY(cudaGetLastError());
   }
   if (!kScores || max_tokens == 0) return TCX_OK;
-  const uint64_t blocks = std::min<uint64_t>((max_tokens + 255) / 256, 64);
-  return launch_after(decode_weights_kernel, dim3(static_cast<unsigned>(blocks), d.a.kv_heads, d.a.n_seq), dim3(256), 0,
+  const uint64_t blocks = std::min<uint64_t>((max_tokens + 511) / 512, 64);
+  return launch_after(decode_weights_kernel, dim3(static_cast<unsigned>(blocks), d.a.kv_heads, d.a.n_seq), dim3(128), 0,
                       stream, d);
 }
 

@@ -4,8 +4,10 @@
 //
 // Two launches: select_kernel, one CTA per (layer, kv head, sequence), finds the
 // budget's weight by radix selection over the weights' order-preserving integer
-// images and writes the kept indices; copy_kernel moves the rows, bound by HBM
-// (each kept row is read and written once). The destination pages are not the
+// images (11, 11 and 10 bits at a time, the images kept in shared memory) and writes
+// the kept indices; copy_kernel moves the rows, bound by HBM (each kept row is read
+// and written once; the sources of 256 rows are looked up first, so that a thread has
+// eight 16-byte loads under way). The destination pages are not the
 // source's: a page may be shared with other sequences, and the copy needs no
 // order between its CTAs.
 #include <cuda_runtime.h>
@@ -20,7 +22,10 @@ namespace {
 
 constexpr int kSelectThreads = 512;
 constexpr int kCopyThreads = 256;
-constexpr int kBins = 256;
+constexpr int kBins = 2048;
+constexpr int kBatch = 8;                 // tokens of a thread in a round of the last pass
+constexpr uint32_t kHeldTokens = 14336;   // images that shared memory holds: 56 KiB, three CTAs on an SM
+constexpr int kSelectShared = kHeldTokens * 4;
 
 struct EvictArgs {
   uint8_t* pool;
@@ -86,6 +91,7 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
 }
 
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
+  extern __shared__ uint32_t held[];
   __shared__ uint32_t bins[kBins], warp_sums[kSelectThreads / 32], s_pick[2];
   const uint32_t head = blockIdx.x, layer = blockIdx.y, s = blockIdx.z;
   next_may_start();
@@ -114,50 +120,66 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
   const uint32_t newest = static_cast<uint32_t>(min(a.recent, static_cast<uint64_t>(kept - first)));
   const uint32_t last = n - newest;
   uint32_t want = kept - first - newest;
-  uint32_t prefix = 0, known = 0;  // the wanted image's upper bits, and their mask
-  if (want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      for (uint32_t b = threadIdx.x; b < kBins; b += blockDim.x) bins[b] = 0;
-      __syncthreads();
-      for (uint32_t j = first + threadIdx.x; j < last; j += blockDim.x) {
-        const uint32_t x = image(w[j]);
-        if ((x & known) == prefix) atomicAdd(&bins[x >> shift & 255], 1u);
-      }
-      __syncthreads();
-      // thread b: how many lie in higher bins than 255 - b
-      uint32_t all;
-      const uint32_t mine = threadIdx.x < kBins ? bins[kBins - 1 - threadIdx.x] : 0;
-      const uint32_t above = block_scan(mine, warp_sums, &all);
-      if (threadIdx.x < kBins && above < want && above + mine >= want) {
-        s_pick[0] = kBins - 1 - threadIdx.x;
-        s_pick[1] = above;
-      }
-      __syncthreads();
-      prefix |= s_pick[0] << shift;
-      known |= 255u << shift;
-      want -= s_pick[1];
-      __syncthreads();
+  const bool any = want > 0, hold = n <= kHeldTokens;
+  uint32_t prefix = 0;  // the wanted image's upper bits
+  for (int pass = 0; any && pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    const uint32_t known = pass == 0 ? 0 : ~0u << (shift + bits);
+    for (uint32_t b = threadIdx.x; b < kBins; b += kSelectThreads) bins[b] = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t j = first + threadIdx.x; j < last; j += kSelectThreads) {
+      const uint32_t x = hold && pass > 0 ? held[j] : image(w[j]);
+      if (hold && pass == 0) held[j] = x;
+      if ((x & known) == prefix) atomicAdd(&bins[x >> shift & ((1u << bits) - 1)], 1u);
     }
+    __syncthreads();
+    // thread t: bins 2047 - 4 t down to 2044 - 4 t; how many lie above them
+    uint32_t mine[4], all = 0, total;
+    for (int k = 0; k < 4; ++k) all += mine[k] = bins[kBins - 1 - 4 * threadIdx.x - k];
+    uint32_t above = block_scan(all, warp_sums, &total);
+    if (above < want && above + all >= want) {
+      int k = 0;
+      while (above + mine[k] < want) above += mine[k++];
+      s_pick[0] = kBins - 1 - 4 * threadIdx.x - k;
+      s_pick[1] = above;
+    }
+    __syncthreads();
+    prefix |= s_pick[0] << shift;
+    want -= s_pick[1];
+    __syncthreads();
   }
-  // `want` of the tokens with exactly this image stay, the lowest indices first.
-  const bool any = kept > first + newest;
+  // `want` of the tokens with exactly this image stay, the lowest indices first. A
+  // thread takes consecutive tokens, so that one scan numbers a round of them.
   uint32_t done = 0, equal_done = 0;
-  for (uint32_t j0 = 0; j0 < n; j0 += blockDim.x) {
-    const uint32_t j = j0 + threadIdx.x;
-    const float v = j < n ? w[j] : 0.f;
-    const bool middle = j >= first && j < last, safe = j < n && !middle;
-    const uint32_t x = image(v);
-    uint32_t total;
-    const uint32_t equal = any && middle && x == prefix;
-    const uint32_t equal_before = equal_done + block_scan(equal, warp_sums, &total);
-    equal_done += total;
-    const uint32_t stay = safe || (any && middle && x > prefix) || (equal && equal_before < want);
-    const uint32_t r = done + block_scan(stay, warp_sums, &total);
-    done += total;
-    if (stay) {
-      keep[r] = static_cast<int32_t>(j);
-      left[r] = v;
+  for (uint32_t j0 = 0; j0 < n; j0 += kSelectThreads * kBatch) {
+    const uint32_t from = j0 + threadIdx.x * kBatch;
+    float v[kBatch];
+    uint32_t equal = 0, stays = 0, total;  // bits of the thread's tokens
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const uint32_t j = from + k;
+      v[k] = j < n ? w[j] : 0.f;
+      const bool middle = j >= first && j < last;
+      const uint32_t x = image(v[k]);
+      if (any && middle && x == prefix) equal |= 1u << k;
+      if ((j < n && !middle) || (any && middle && x > prefix)) stays |= 1u << k;
     }
+    // both counts in one sum: at most 512 x 8 each
+    const uint32_t before = block_scan(static_cast<uint32_t>(__popc(equal)) << 16 | __popc(stays), warp_sums, &total);
+    uint32_t equals = equal_done + (before >> 16);
+    uint32_t r = done + (before & 0xffff) + min(equals, want) - min(equal_done, want);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const bool stay = (stays >> k & 1) || ((equal >> k & 1) && equals < want);
+      equals += equal >> k & 1;
+      if (stay) {
+        keep[r] = static_cast<int32_t>(from + k);
+        left[r++] = v[k];
+      }
+    }
+    done += (total & 0xffff) + min(equal_done + (total >> 16), want) - min(equal_done, want);
+    equal_done += total >> 16;
   }
 }
 
@@ -173,30 +195,55 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(EvictArgs a) {
   uint32_t n, kept;
   lengths(a, lo, &n, &kept);
   const uint64_t r0 = (page - a.dst_page_offsets[lo]) * a.page_tokens;
-  if (r0 >= kept) return;
+  if (r0 >= kept) {
+    wait_for_previous();  // also here: this kernel's end stands for the one's before
+    return;
+  }
   const uint32_t rows = static_cast<uint32_t>(min(static_cast<uint64_t>(a.page_tokens), kept - r0));
   const uint32_t dst_slot = a.dst_page_table[page];
   if (dst_slot >= a.pool_pages) {
     if (threadIdx.x == 0) atomicCAS(a.status, 0u, 1u);
+    wait_for_previous();
     return;
   }
   const uint64_t plane_off = plane * a.pool_pages * a.page_bytes;
   const uint32_t* table = a.page_table + a.page_offsets[lo];
   const int32_t* keep = a.keep + static_cast<uint64_t>(plane / 2) * a.kv_heads * a.dst_capacity + page * a.page_tokens;
-  wait_for_previous();  // the kept indices
-  const uint32_t pieces = static_cast<uint32_t>(a.head_bytes / 16), per_token = pieces * a.kv_heads;
-  for (uint32_t i = threadIdx.x; i < rows * per_token; i += blockDim.x) {
-    const uint32_t r = i / per_token, head = i % per_token / pieces, piece = i % pieces;
-    const uint32_t j = static_cast<uint32_t>(keep[head * a.dst_capacity + r]);
-    const uint32_t slot = table[j / a.page_tokens];
-    if (slot >= a.pool_pages) {
-      atomicCAS(a.status, 0u, 1u);
-      continue;
+  const uint32_t pieces = static_cast<uint32_t>(a.head_bytes / 16), entries = rows * a.kv_heads;
+  __shared__ uint64_t s_from[kCopyThreads];
+  uint8_t* to = a.pool + plane_off + dst_slot * a.page_bytes;  // the page's rows and heads, one after the other
+  wait_for_previous();                                         // the kept indices
+  for (uint32_t e0 = 0; e0 < entries; e0 += kCopyThreads) {
+    const uint32_t e = e0 + threadIdx.x;
+    uint64_t from = ~uint64_t{0};
+    if (e < entries) {
+      const uint32_t r = e / a.kv_heads, head = e % a.kv_heads;
+      const uint32_t j = static_cast<uint32_t>(keep[head * a.dst_capacity + r]);
+      const uint32_t slot = table[j / a.page_tokens];
+      if (slot < a.pool_pages)
+        from = plane_off + slot * a.page_bytes + j % a.page_tokens * a.token_bytes + head * a.head_bytes;
+      else
+        atomicCAS(a.status, 0u, 1u);
     }
-    const uint64_t in = head * a.head_bytes + piece * 16;
-    const uint4 v = *reinterpret_cast<const uint4*>(a.pool + plane_off + slot * a.page_bytes +
-                                                    j % a.page_tokens * a.token_bytes + in);
-    *reinterpret_cast<uint4*>(a.pool + plane_off + dst_slot * a.page_bytes + r * a.token_bytes + in) = v;
+    s_from[threadIdx.x] = from;
+    __syncthreads();
+    const uint32_t moves = min(entries - e0, static_cast<uint32_t>(kCopyThreads)) * pieces;
+    for (uint32_t i0 = threadIdx.x; i0 < moves; i0 += 8 * kCopyThreads) {
+      uint4 v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t i = i0 + k * kCopyThreads;
+        if (i < moves && s_from[i / pieces] != ~uint64_t{0})
+          v[k] = __ldcs(reinterpret_cast<const uint4*>(a.pool + s_from[i / pieces]) + i % pieces);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t i = i0 + k * kCopyThreads;
+        if (i < moves && s_from[i / pieces] != ~uint64_t{0})
+          reinterpret_cast<uint4*>(to + static_cast<uint64_t>(e0) * a.head_bytes)[i] = v[k];
+      }
+    }
+    __syncthreads();
   }
 }
 
@@ -256,7 +303,10 @@ extern "C" tcx_status tcx_kv_evict(const tcx_kv_evict_args* args, void* stream) 
   a.status = x.d_status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const dim3 select_grid(a.kv_heads, static_cast<unsigned>(x.planes / 2), a.n_seq);
-  select_kernel<<<select_grid, kSelectThreads, 0, s>>>(a);
+  static std::atomic<uint64_t> allowed{0};
+  if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(select_kernel), kSelectShared, &allowed); st != TCX_OK)
+    return st;
+  select_kernel<<<select_grid, kSelectThreads, kSelectShared, s>>>(a);
   note_launches(1);
   TCX_CUDA_TRY(cudaGetLastError());
   if (x.dst_total_pages != 0) {

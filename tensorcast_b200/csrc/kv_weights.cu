@@ -42,7 +42,10 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y, s = blockIdx.z;
   const int len = static_cast<int>(seq_length(a, s)), key0 = static_cast<int>(blockIdx.x) * kKeys;
   const uint32_t q_first = a.q_offsets[s], queries = a.q_offsets[s + 1] - q_first, rows = queries * a.group;
-  if (key0 >= len || queries == 0) return;
+  if (key0 >= len || queries == 0) {
+    wait_for_previous();  // also here: this kernel's end stands for the one's before
+    return;
+  }
   const int pos0 = len - static_cast<int>(queries), key_end = min(key0 + kKeys, len);
   const int sinks = static_cast<int>(a.sinks);
   auto low_of = [&](int pos) { return a.window ? static_cast<int>(max(int64_t{0}, pos - a.window + 1)) : 0; };
@@ -51,7 +54,10 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
   const int q_begin = max(key0 - pos0, 0);
   const int64_t q_last = a.window && key0 >= sinks ? key_end - 1 + a.window - 1 - pos0 : static_cast<int64_t>(queries) - 1;
   const int q_end = static_cast<int>(min(q_last + 1, static_cast<int64_t>(queries)));
-  if (q_begin >= q_end) return;
+  if (q_begin >= q_end) {
+    wait_for_previous();
+    return;
+  }
   const uint32_t tile0 = q_begin * a.group / kRows, tile_end = (q_end * a.group + kRows - 1) / kRows;
   const uint32_t n = tile_end - tile0;
 

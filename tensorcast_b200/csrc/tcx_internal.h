@@ -4,6 +4,7 @@
 
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdint>
 #include <cstdio>
@@ -63,9 +64,20 @@ inline std::string cuda_msg(cudaError_t e) {
 
 namespace tcx {
 
+// Lets a kernel use `bytes` of dynamic shared memory, once for each device.
+inline tcx_status allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>* done) {
+  int dev = 0;
+  TCX_CUDA_TRY(cudaGetDevice(&dev));
+  const uint64_t bit = 1ull << (dev & 63);
+  if (dev < 64 && (done->load(std::memory_order_relaxed) & bit)) return TCX_OK;
+  TCX_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) done->fetch_or(bit, std::memory_order_relaxed);
+  return TCX_OK;
+}
+
 // Launches a kernel that waits for the one before it in its own code
 // (griddepcontrol.wait, in every thread that uses that one's memory or writes where it
-// may still read), so that its set-up runs beside that one's end. The first kernel of
+// may still read, and in every CTA before it ends), so that its set-up runs beside that one's end. The first kernel of
 // a call is launched without: it follows all earlier work of the stream.
 template <typename... Params, typename... Args>
 tcx_status launch_after(void (*kernel)(Params...), dim3 grid, dim3 block, size_t shared, cudaStream_t stream,
