@@ -9,6 +9,7 @@
 // Bound by the exponential units (one for each score; the product is half as long);
 // two CTAs share an SM, so that one's fetches run beside the other's exponentials.
 #include <algorithm>
+#include <type_traits>
 
 #include "kv_attention.cuh"
 
@@ -27,16 +28,14 @@ struct WeightLayout {
   static constexpr int kBytes = 3 * kOperand + 1024;  // the keys, and two tiles of queries
 };
 
-struct RowSeen {
-  float lse;  // in powers of two; infinite where the row counts for nothing
-  int hi, lo;
-};
-
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_constant__ CUtensorMap map, AttnArgs a) {
   using L = WeightLayout<D>;
   extern __shared__ uint8_t raw[];
-  __shared__ RowSeen s_rows[4][kRows];
+  // Of the tiles' rows: lse in powers of two, infinite where the row counts for nothing,
+  // and the keys that it sees, up to hi and from lo on (and the sinks).
+  __shared__ __align__(16) float s_lse[4][kRows];
+  __shared__ int2 s_sees[4][kRows];
   __shared__ uint64_t s_bar[7];
   __shared__ uint32_t s_tmem, s_gave_up, s_drained;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y, s = blockIdx.z;
@@ -76,7 +75,6 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
     s_gave_up = s_drained = 0;
     mbar_init_fence();
   }
-  wait_for_previous();  // the rows' sums, and the tensor memory of the kernel before
   if (warp == kWorkers / 32) tmem_alloc(smem_addr(&s_tmem), 2 * kRows);
   tmem_fence_before();
   __syncthreads();
@@ -125,6 +123,8 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
     const int key = key0 + static_cast<int>(threadIdx.x);
     // Starts the copies of a tile's queries (this warp: 32 of them, D / 8 lanes to a
     // row, swizzled) and notes what its rows see.
+    float of_row;
+    int2 sees;
     auto fetch = [&](uint32_t i) {
       if (i < n) {
         constexpr uint32_t kLanes = D / 8;
@@ -140,27 +140,34 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
           async_copy16(base + (1 + i % 2) * L::kOperand + c / 8 * L::kBlock + of * 128 + ((c % 8 ^ (of & 7)) << 4),
                        a.q + (valid ? from + c * 16 : 0), valid ? 16 : 0);
         }
-        RowSeen seen{INFINITY, -1, 0};
+        of_row = -INFINITY;
+        sees = make_int2(-1, 0);
         if (row < rows) {
-          seen.hi = pos0 + static_cast<int>(row / a.group);
-          seen.lo = low_of(seen.hi);
-          const float lse = a.lse[static_cast<uint64_t>(t) * a.kv_heads * a.group + h] * kLog2e;
-          if (lse != -INFINITY) seen.lse = lse;
+          sees.x = pos0 + static_cast<int>(row / a.group);
+          sees.y = low_of(sees.x);
+          of_row = a.lse[static_cast<uint64_t>(t) * a.kv_heads * a.group + h];
         }
-        s_rows[i % 4][threadIdx.x] = seen;
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto note = [&](uint32_t i) {  // what fetch found, once it is there
+      if (i >= n) return;
+      s_lse[i % 4][threadIdx.x] = of_row == -INFINITY ? INFINITY : of_row * kLog2e;
+      s_sees[i % 4][threadIdx.x] = sees;
     };
     auto ready = [&](uint32_t i) {  // tile i's copies of this warp are there
       if (i >= n) return;
       proxy_fence_smem();
       mbar_arrive_warp(queries_there(i), lane, alive);
     };
+    wait_for_previous();  // the rows' lse
     fetch(0);
+    note(0);
     fetch(1);
+    note(1);
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     ready(0);
-    float sum[2] = {0.f, 0.f};
+    float2 sum[2] = {};
     for (uint32_t i = 0; i < n; ++i) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       ready(i + 1);
@@ -171,30 +178,45 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
       const uint32_t first = (tile0 + i) * kRows, last = min(first + kRows, rows) - 1;
       const int all_hi = pos0 + static_cast<int>(first / a.group), all_lo = low_of(pos0 + static_cast<int>(last / a.group));
       const bool masked = key0 + kKeys - 1 > all_hi || (key0 < all_lo && key0 + kKeys > sinks) || last != first + kRows - 1;
-      const RowSeen* seen = s_rows[i % 4];
+      const float4* lse = reinterpret_cast<const float4*>(s_lse[i % 4]);
+      const float2 c2 = make_float2(a.scale_log2, a.scale_log2);
+      auto add_up = [&](auto some_hidden) {
 #pragma unroll
-      for (int c = 0; c < kRows; c += 32) {
-        uint32_t z[32];
-        tmem_load32(z, tmem + (warp * 32 << 16) + i % 2 * kRows + c);
-        if (masked) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const RowSeen& row = seen[c + k];
-            const float p = exp2_approx(fmaf(__uint_as_float(z[k]), a.scale_log2, -row.lse));
-            if (key <= row.hi && (key >= row.lo || key < sinks)) sum[k % 2] += p;
+        for (int c = 0; c < kRows; c += 64) {
+          uint32_t z[64];
+          tmem_load64(z, tmem + (warp * 32 << 16) + i % 2 * kRows + c);
+          if (c != 0) {
+            tmem_fence_before();
+            mbar_arrive_warp(taken(i), lane, alive);
           }
-        } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            sum[k % 2] += exp2_approx(fmaf(__uint_as_float(z[k]), a.scale_log2, -seen[c + k].lse));
+          for (int k = 0; k < 64; k += 4) {
+            const float4 x = lse[(c + k) / 4];
+            float2 p = fma2(make_float2(__uint_as_float(z[k]), __uint_as_float(z[k + 1])), c2, make_float2(-x.x, -x.y));
+            float2 q = fma2(make_float2(__uint_as_float(z[k + 2]), __uint_as_float(z[k + 3])), c2,
+                            make_float2(-x.z, -x.w));
+            p = make_float2(exp2_approx(p.x), exp2_approx(p.y));
+            q = make_float2(exp2_approx(q.x), exp2_approx(q.y));
+            if constexpr (decltype(some_hidden)::value) {
+              auto see = [&](int of, float v) {
+                const int2 row = s_sees[i % 4][c + k + of];
+                return key <= row.x && (key >= row.y || key < sinks) ? v : 0.f;
+              };
+              p = make_float2(see(0, p.x), see(1, p.y));
+              q = make_float2(see(2, q.x), see(3, q.y));
+            }
+            sum[0] = add2(sum[0], p);
+            sum[1] = add2(sum[1], q);
+          }
         }
-      }
-      tmem_fence_before();
-      mbar_arrive_warp(taken(i), lane, alive);
+      };
+      if (masked) add_up(std::true_type{}); else add_up(std::false_type{});
+      note(i + 2);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (key < len && alive)
-      a.weights[head * a.weights_head_stride + a.page_offsets[s] * a.page_tokens + key] += sum[0] + sum[1];
+      a.weights[head * a.weights_head_stride + a.page_offsets[s] * a.page_tokens + key] +=
+          (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
   }
   tmem_fence_before();
   __syncthreads();
