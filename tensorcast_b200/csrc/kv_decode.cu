@@ -41,7 +41,7 @@ struct TileInfo {
 
 struct DecodeArgs {
   AttnArgs a;
-  uint32_t ranges;
+  uint32_t ranges, rows;  // at most
   float* part_o;    // [ranges][2][kv_heads][kRows][D], sums of 2^(z - m) v
   float2* part_ml;  // the same rows' m and sum of 2^(z - m)
   float* scores;    // [kv_heads][rows][columns], in powers of two, where weights are added up
@@ -63,10 +63,17 @@ struct Layout {
 struct SeqInfo {
   int len, low, sinks, sink_tiles, first_tile;  // tiles: [0, sink_tiles) and from first_tile on
   uint32_t tiles, q_first, queries;
+  uint64_t table;  // first entry in the page table
+
+  __device__ __forceinline__ int token(uint32_t t) const {  // first token of tile t
+    return (t < static_cast<uint32_t>(sink_tiles) ? static_cast<int>(t) : first_tile + static_cast<int>(t) - sink_tiles) *
+           kTile;
+  }
 };
 
 __device__ __forceinline__ SeqInfo seq_info(const AttnArgs& a, uint32_t s, int prefix) {
   SeqInfo i;
+  i.table = a.page_offsets[s];
   i.q_first = a.q_offsets[s];
   i.queries = a.q_offsets[s + 1] - i.q_first;
   i.len = static_cast<int>(seq_length(a, s));
@@ -164,8 +171,11 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     if (w < warp) before += s_scan[w];
     total += s_scan[w];
   }
-  // Three tiles are in flight at once: fewer in a range save no time, and leave more to join.
-  const uint32_t ranges = min(d.ranges, (total + 2) / 3);
+  // A tile more in a range costs about 1400 cycles (what one SM fetches of it), a range
+  // more for a sequence 90 for every four rows when its parts are joined: few tiles are
+  // cut where the two together are least.
+  const uint32_t least = max(1u, static_cast<uint32_t>(sqrtf(static_cast<float>(total) * d.rows * (1.f / 64))));
+  const uint32_t ranges = min(d.ranges, (total + least - 1) / least);
   if (range >= ranges) {
     wait_for_previous();
     return;
@@ -187,15 +197,37 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
 
   if (warp == kWarps) {  // ---- the producer
     const uint32_t boxes = kTile / a.box_rows, halves = D / 64;
-    uint32_t s = s_begin[0], t = s_begin[1];
-    SeqInfo q = seq_info(a, s, prefix);
+    // lane: one box of the keys or values and one half of the head
+    const uint32_t box = lane % boxes, half = lane / boxes % halves, plane = lane / boxes / halves;
+    const uint64_t plane_row = plane ? a.v_row0 : a.k_row0;
+    // Page slots are looked up for 32 boxes at once, and for the next 32, or the next
+    // sequence's first, while the tiles before them are fetched.
+    const uint32_t per = 32 / boxes;  // tiles
+    auto wanted_box = [&](const SeqInfo& q, int from) {
+      const int to = from + static_cast<int>(a.box_rows);
+      return from < q.len && (to > q.low || from < q.sinks);
+    };
+    auto slots_of = [&](const SeqInfo& q, uint32_t t0) {
+      const uint32_t t = t0 + lane / boxes;
+      if (t >= q.tiles) return 0u;
+      const int from = q.token(t) + static_cast<int>(box * a.box_rows);
+      return wanted_box(q, from) ? static_cast<uint32_t>(checked_slot(a, a.page_table + q.table, from / a.page_tokens)) : 0u;
+    };
+    uint32_t s = s_begin[0], t = s_begin[1], next_s = s;
+    SeqInfo q = seq_info(a, s, prefix), next = q;
+    uint32_t slots_from = t, slots = slots_of(q, t), slots_ahead = slots_of(q, t + per), next_slots = 0;
     bool fresh = true;  // the next tile is the first of its piece
     uint32_t pieces = 0;
     uint32_t i = 0;
     for (; i < count; ++i) {
       const uint32_t stage = i % L::kStages;
-      const int tile = t < static_cast<uint32_t>(q.sink_tiles) ? t : q.first_tile + (t - q.sink_tiles);
-      const int token = tile * kTile, end = min(token + kTile, q.len);
+      const int token = q.token(t);
+      if (t == slots_from + per) {
+        slots = slots_ahead;
+        slots_from = t;
+        slots_ahead = slots_of(q, t + per);
+      }
+      const uint32_t slot = __shfl_sync(~0u, slots, (t - slots_from) * boxes + box);
       TileInfo info{fresh ? kFirst : 0u, s, q.q_first, q.queries, token, q.len, q.low, q.sinks, 0, 0, 0};
       const bool seq_done = t + 1 == q.tiles;
       if (seq_done || i + 1 == count) info.flags |= kLast;
@@ -216,16 +248,10 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
         info.flags |= kMask;
       if (!mbar_wait_warp(smem_addr(&s_empty[stage]), (i / L::kStages & 1) ^ 1, &s_gave_up, a.status)) break;
       const uint32_t full = smem_addr(&s_full[stage]), at = base + stage * L::kStage;
-      // lane: one box of the keys or values and one half of the head
-      const uint32_t box = lane % boxes, half = lane / boxes % halves, plane = lane / boxes / halves;
-      const int from = token + static_cast<int>(box * a.box_rows), to = from + static_cast<int>(a.box_rows);
-      const bool wanted = lane < 2 * halves * boxes && from < end && (to > q.low || from < q.sinks);
+      const int from = token + static_cast<int>(box * a.box_rows);
+      const bool wanted = lane < 2 * halves * boxes && wanted_box(q, from);
       const uint32_t rows = fresh ? min(q.queries * a.group, static_cast<uint32_t>(kRows)) : 0;
       const uint32_t bytes = __popc(__ballot_sync(~0u, wanted)) * a.box_rows * 128 + rows * D * 2;
-      uint64_t row = 0;
-      if (wanted)
-        row = checked_slot(a, a.page_table + a.page_offsets[s], from / a.page_tokens) * a.page_tokens +
-              from % a.page_tokens + (plane ? a.v_row0 : a.k_row0);
       if (lane == 0) {
         s_info[stage] = info;
         if (bytes) mbar_arrive_expect(full, bytes); else mbar_arrive(full);
@@ -233,17 +259,25 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       __syncwarp();
       if (wanted)
         tma_load_3d(at + plane * L::kKeys + half * L::kHalf + box * a.box_rows * 128, &map, half * 64, head,
-                    static_cast<int>(row), full);
+                    static_cast<int>(plane_row + static_cast<uint64_t>(slot) * a.page_tokens + from % a.page_tokens), full);
       if (lane < rows)
         bulk_load(at + 2 * L::kKeys + lane * L::kQueryPitch,
                   a.q + (q.q_first + lane / a.group) * a.q_token_stride +
                       (head * a.group + lane % a.group) * a.q_head_stride,
                   D * 2, full);
+      if (fresh && i + (q.tiles - t) < count) {  // the next sequence is this range's too
+        next_s = s;
+        do next = seq_info(a, ++next_s, prefix); while (next.tiles == 0);
+        next_slots = slots_of(next, 0);
+      }
       fresh = false;
       ++t;
       if (seq_done && i + 1 < count) {
-        do q = seq_info(a, ++s, prefix); while (q.tiles == 0);
-        t = 0;
+        s = next_s;
+        q = next;
+        t = slots_from = 0;
+        slots = next_slots;
+        slots_ahead = slots_of(q, per);
         fresh = true;
         ++pieces;
       }
@@ -273,23 +307,19 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       m[0] = m[1] = -INFINITY;
       l[0] = l[1] = 0.f;
     }
-    // scores: tokens 0-7 (z[0]) and 8-15 (z[1]) of this warp's 16
-    float z[2][4] = {};
+    // All of the warp's keys are loaded before the first product, and its values before
+    // the softmax, so that their latencies do not add up.
+    uint32_t kf[D / 16][4], vf[D / 16][4];
     {
       const uint32_t token = warp * 16 + lane / 16 * 8 + lane % 8, chunk = lane / 8 % 2;
       const uint32_t row = at + token * 128;
 #pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        uint32_t b[4];
-        ldmatrix4(b, row + k / 4 * L::kHalf + (((k % 4 * 2 + chunk) ^ (token & 7)) << 4));
-        mma16816<T>(z[0], qf[k], b[0], b[1]);
-        mma16816<T>(z[1], qf[k], b[2], b[3]);
-      }
+      for (int k = 0; k < D / 16; ++k)
+        ldmatrix4(kf[k], row + k / 4 * L::kHalf + (((k % 4 * 2 + chunk) ^ (token & 7)) << 4));
     }
     if (info.flags & kMask) {
-      const int first = info.token + static_cast<int>(warp) * 16;
       // values that no row sees are cleared: 0 x NaN is not 0
-      const int hidden = first + static_cast<int>(lane % 16);
+      const int hidden = info.token + static_cast<int>(warp * 16 + lane % 16);
       const bool clear = hidden >= info.len || (hidden < info.low && hidden >= info.sinks);
       if (__any_sync(~0u, clear)) {
         if (clear) {
@@ -301,6 +331,29 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
         proxy_fence_smem();
         __syncwarp();
       }
+    }
+    {
+      const uint32_t token = warp * 16 + lane % 16;
+      const uint32_t row = at + L::kKeys + token * 128;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n)
+        ldmatrix4_t(vf[n], row + n / 4 * L::kHalf + (((n % 4 * 2 + lane / 16) ^ (token & 7)) << 4));
+    }
+    // scores: tokens 0-7 (z[0]) and 8-15 (z[1]) of this warp's 16, in two sums each
+    float z[2][4] = {}, z2[2][4] = {};
+#pragma unroll
+    for (int k = 0; k < D / 16; k += 2) {
+      mma16816<T>(z[0], qf[k], kf[k][0], kf[k][1]);
+      mma16816<T>(z[1], qf[k], kf[k][2], kf[k][3]);
+      mma16816<T>(z2[0], qf[k + 1], kf[k + 1][0], kf[k + 1][1]);
+      mma16816<T>(z2[1], qf[k + 1], kf[k + 1][2], kf[k + 1][3]);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[n][e] += z2[n][e];
+    if (info.flags & kMask) {
+      const int first = info.token + static_cast<int>(warp) * 16;
       const uint32_t r = lane / 4;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
@@ -361,16 +414,10 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] *= scale[e / 2];
     }
-    {
-      const uint32_t token = warp * 16 + lane % 16;
-      const uint32_t row = at + L::kKeys + token * 128;
 #pragma unroll
-      for (int n = 0; n < D / 16; ++n) {
-        uint32_t b[4];
-        ldmatrix4_t(b, row + n / 4 * L::kHalf + (((n % 4 * 2 + lane / 16) ^ (token & 7)) << 4));
-        mma16816<T>(o[2 * n], p, b[0], b[1]);
-        mma16816<T>(o[2 * n + 1], p, b[2], b[3]);
-      }
+    for (int n = 0; n < D / 16; ++n) {
+      mma16816<T>(o[2 * n], p, vf[n][0], vf[n][1]);
+      mma16816<T>(o[2 * n + 1], p, vf[n][2], vf[n][3]);
     }
     if (info.flags & kLast) {
       wait_for_previous();  // the rows' parts over a shared prefix
@@ -478,7 +525,7 @@ __global__ void __launch_bounds__(128) decode_weights_kernel(DecodeArgs d) {
 uint32_t decode_ranges(const tcx_kv_attention_args& x) {
   const uint64_t tiles = x.total_pages * x.page_tokens / kTile + x.n_seq;
   const uint64_t most = std::min<uint64_t>(2ull * sm_count(), TCX_KV_COUNTERS / 2) / x.kv_heads;
-  return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>((tiles + 2) / 3, most)));
+  return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(tiles, most)));
 }
 
 template <typename T, int D, bool kScores>
@@ -532,6 +579,7 @@ tcx_status launch_decode(const tcx_kv_attention_args& x, const AttnArgs& a, cons
   DecodeArgs d{};
   d.a = a;
   d.ranges = decode_ranges(x);
+  d.rows = static_cast<uint32_t>(x.max_q) * a.group;
   const uint64_t parts = d.ranges * 2ull * x.kv_heads * kRows;
   uint8_t* at = static_cast<uint8_t*>(scratch);
   d.part_ml = reinterpret_cast<float2*>(at);
