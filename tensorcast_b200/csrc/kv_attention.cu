@@ -38,7 +38,7 @@ tcx_status check_sizes(const tcx_kv_attention_args& a) {
   if (a.n_seq > 65535) return set_error(TCX_INVALID_ARGUMENT, "more than 65535 sequences");
   if (a.q_tokens > 0x7fffffffull / a.q_heads) return set_error(TCX_INVALID_ARGUMENT, "2^31 query rows or more");
   if (a.max_q > a.q_tokens || a.total_pages > 0x7fffffffull || a.max_pages > a.total_pages ||
-      a.max_pages > 0x7fffffffull / a.page_tokens || a.prefix_pages > 0x3fffffffull / a.page_tokens)
+      a.max_pages > 0x3fffffffull / a.page_tokens || a.prefix_pages > 0x3fffffffull / a.page_tokens)
     return set_error(TCX_INVALID_ARGUMENT, "inconsistent size bounds");
   if (a.window > 0x3fffffffull || a.sinks > 0x3fffffffull)
     return set_error(TCX_INVALID_ARGUMENT, "window and sinks must be below 2^30");

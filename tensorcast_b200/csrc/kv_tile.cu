@@ -3,24 +3,33 @@
 // tokens.
 //
 // A kv head's rows are its query tokens x its group of q heads, in tiles of 256. A
-// CTA takes a tile of rows through tiles of 128 tokens: two products of 128 x 128
-// scores on the tensor cores (one for each half of the rows, so that one half's
-// softmax runs beside the other half's products), a softmax with a running maximum
-// and sum in 32 bits, one thread for each row, and two products with the values.
-// Scores, probabilities (rounded to the input type in place of the scores, half a
-// step, as the output is) and the output's sums (32 bits) stay in tensor memory; a
-// row's sums are scaled to a new maximum only where it has grown by more than 2^8,
-// which the 32-bit sums carry exactly as well.
+// CTA takes a tile of rows through tiles of 128 tokens: for each half of the rows two
+// products of 128 x 64 scores on the tensor cores, a softmax with a running maximum
+// and sum in 32 bits, one thread for each row, and a product of the probabilities with
+// the values. Scores, probabilities and the output's sums (32 bits) stay in tensor
+// memory. The probabilities are rounded to the input type (half a step, as the output
+// is) and take the place of the first 64 tokens' scores; the other 64 tokens' place is
+// free as soon as its scores are read, so the next tile's are computed there while this
+// one's first 64 are weighed. A row's sums are scaled to a new maximum only where it
+// has grown by more than 2^8, which the 32-bit sums carry exactly as well.
 //
-// Roles: warps 0-3 and 4-7 the halves' softmax, warp 8 issues the products, warp 9
-// loads keys and values with TMA into a ring (a box for each run of rows in a page).
+// Roles: warps 0-3 and 4-7 the halves' softmax, warps 8 and 10 issue the halves'
+// products, warp 9 loads keys and values with TMA into a ring (a box for each run of
+// rows in a page).
 //
 // Work: the visible (row tile, kv head, token tile) units laid end to end and cut
 // into equal ranges, one CTA on every SM, whatever the prompts' lengths and masks
 // are; row tiles cut by a border leave parts in the scratch, which are added up in the
 // ranges' order by tile_join_kernel, or where they are few by the CTA that comes
-// last. tile_plan_kernel lays prompts' units out
-// from the device's lengths; over a prefix all row tiles have the same ones.
+// last. tile_plan_kernel lays prompts' units out from the device's lengths; over a
+// prefix all row tiles have the same ones.
+//
+// Bound by the softmax: a unit's products take 2560 cycles, its exponentials 1536 on
+// the exponential units (a fourth of them runs on the FMA units), and the two warps of
+// a scheduler take about 3500 for all of it; tensor cores 0.46 to 0.6 busy. Measured on
+// B200: 2048 queries at the end of 40011 tokens, 32 / 8 heads of 128, 1.23 ms in a
+// burst (1060 TFLOP/s, 0.63 of the measured burst rate), 1.44 ms back to back under the
+// power cap (0.65 of the sustained rate).
 #include <algorithm>
 #include <type_traits>
 

@@ -8,6 +8,9 @@
 // that is a third more, where keeping them would take rows x tokens x 4 bytes.
 // Bound by the exponential units (one for each score; the product is half as long);
 // two CTAs share an SM, so that one's fetches run beside the other's exponentials.
+// Measured on B200: 256 queries at the ends of two sequences of 5000-6100 tokens, 32 / 8
+// heads of 128, 69 us beside 80 us for their attention (90 million exponentials: 20 us
+// of the exponential units).
 #include <algorithm>
 #include <type_traits>
 

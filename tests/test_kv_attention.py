@@ -418,6 +418,107 @@ def test_streams(cuda_device):
         assert (out == want[0]).all() and (lse == want[1]).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("counts", [[1, 1, 1], [40, 1, 70]])
+def test_pool_beyond_32_bit_offsets(cuda_device, counts):
+    """Pages at the end of planes of 5.2 GB each, the second of two layers."""
+    kv_heads, dim, page, pages = 8, 128, 16, 80_000
+    tokens = [100, 33, 71]
+    need = [-(-n // page) for n in tokens]
+    slots = np.arange(pages - 40, pages, dtype=np.uint32)[::-1].copy()
+    offs = np.concatenate([[0], np.cumsum(need)]).astype(np.uint64)
+    w = KvWorkload(4, pages, page, kv_heads * dim * 2, np.array(tokens, np.uint32), offs, slots[: sum(need)])
+    pool = torch.zeros((4, pages * page, kv_heads, dim), dtype=BF16, device="cuda")
+    pool[:, -40 * page:] = torch.randn((4, 40 * page, kv_heads, dim), device="cuda").to(BF16)
+    q = queries(sum(counts), 16, dim, BF16, 0)
+    att = KvAttention(w, 16, kv_heads, query_tokens=counts)
+    weights = torch.zeros((2, kv_heads, att.weight_columns), device="cuda")
+    ref = kvtools.attention(w, pool, 1, q, counts)
+    check(att.run(pool, 1, q, weights=weights[1]), ref, BF16, 100)
+    for s, n in enumerate(tokens):
+        c = int(offs[s]) * page
+        assert (weights[1, :, c:c + n].double() - ref[2][s]).abs().max() < 1e-3
+    dst = KvWorkload(4, pages, page, w.token_bytes, np.full(3, 20, np.uint32), np.array([0, 2, 4, 6], np.uint64),
+                     slots[-6:].copy())
+    keep, _, _ = KvEvict(w, dst, kv_heads).run(pool, weights)
+    for s in range(3):
+        idx = keep[1, 3, 32 * s: 32 * s + 20].cpu().numpy()
+        want = pool[2:, torch.from_numpy(kvtools.token_rows(w, s)[idx]).cuda(), 3]
+        assert (pool[2:, torch.from_numpy(kvtools.token_rows(dst, s)).cuda(), 3] == want).all()
+
+
+@pytest.mark.gpu
+def test_many_sequences(cuda_device):
+    """More sequences than threads; most of them without queries or tokens."""
+    rng = np.random.default_rng(0)
+    tokens = rng.integers(0, 40, 3000).tolist()
+    counts = rng.integers(0, 2, 3000).tolist()
+    run(tokens, counts, kv_heads=1, group=2, dim=64)
+    counts = [c * 9 for c in counts[:300]]
+    run(tokens[:300], counts, kv_heads=1, group=2, dim=64)
+
+
+@pytest.mark.gpu
+def test_nothing_to_do(cuda_device):
+    w, free = kvtools.tables([20, 30], taken=4)
+    pool = kvtools.make_pool(w, 2, 64, BF16).cuda()
+    out, lse = KvAttention(w, 4, 2, query_tokens=[0, 0]).run(pool, 0, queries(0, 4, 64, BF16, 0))
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    none = KvWorkload(2, w.pool_pages, 16, w.token_bytes, np.zeros(0, np.uint32), np.zeros(1, np.uint64),
+                      np.zeros(0, np.uint32))
+    out, lse = KvAttention(none, 4, 2).run(pool, 0, queries(0, 4, 64, BF16, 0))
+    assert out.shape == (0, 4, 64)
+    keep, left, tokens = KvEvict(none, none, 2).run(pool, torch.zeros((1, 2, 0), device="cuda"))
+    assert keep.shape == left.shape == (1, 2, 0) and tokens.shape == (0,)
+    # sequences with queries and without a page
+    empty = KvWorkload(2, w.pool_pages, 16, w.token_bytes, np.zeros(2, np.uint32), np.zeros(3, np.uint64),
+                       np.zeros(0, np.uint32))
+    for counts in ([1, 2], [40, 2]):
+        n = sum(counts)
+        att = KvAttention(empty, 4, 2, query_tokens=counts)
+        out, lse = att.run(pool, 0, queries(n, 4, 64, BF16, 0), weights=torch.zeros((2, 0), device="cuda"))
+        att.check_status()
+        assert (out == 0).all() and (lse == -math.inf).all()
+
+
+@pytest.mark.gpu
+def test_first_call_of_a_process_may_be_captured(cuda_device):
+    import subprocess
+    import sys
+    code = """
+import torch, kvtools
+from tensorcast_b200.kvattention import KvAttention, KvEvict
+from tensorcast_b200.kvcache import KvWorkload
+import numpy as np
+w, free = kvtools.tables([100, 30], taken=8)
+pool = kvtools.make_pool(w, 2, 64, torch.bfloat16).cuda()
+dst = KvWorkload(w.planes, w.pool_pages, 16, w.token_bytes, np.full(2, 20, np.uint32), np.array([0, 2, 4], np.uint64), free[:4])
+for counts, more in (([1, 1], {}), ([60, 20], {}), ([1, 1], dict(prefix_pages=free[4:8], prefix_tokens=60))):
+    q = torch.randn((sum(counts), 4, 64), device="cuda").bfloat16()
+    att = KvAttention(w, 4, 2, query_tokens=counts, **more)
+    weights = None if more else torch.zeros((2, att.weight_columns), device="cuda")
+    ev = KvEvict(w, dst, 2)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, lse = att.run(pool, 0, q, weights=weights)
+        if weights is not None:
+            keep, _, _ = ev.run(pool, weights[None])
+    g.replay()
+    torch.cuda.synchronize()
+    want, _ = att.run(pool, 0, q)
+    assert (out == want).all()
+    if weights is not None:
+        again, _, _ = ev.run(pool, weights[None])
+        assert (keep == again).all()
+print("done")
+"""
+    import os
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.pathsep.join([here, os.path.dirname(here)]))
+    r = subprocess.run([sys.executable, "-c", code], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
+
+
 # ---------------------------------------------------------------- accumulated weights (GPU)
 
 @pytest.mark.gpu
@@ -537,6 +638,14 @@ def test_evict_ties_and_special_weights(cuda_device):
 def test_evict_zero_budget_and_everything_kept(cuda_device):
     evict_case([40, 50, 0], [0, 50, 0])
     evict_case([40, 50], [25, 25], sinks=20, recent=5)   # nothing is left to rank
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [14335, 14336, 14337, 30000])
+def test_evict_around_what_shared_memory_holds(cuda_device, n):
+    g = torch.Generator().manual_seed(n)
+    weights = torch.randint(0, 50, (1, 1, -(-n // 16) * 16), generator=g).float()
+    evict_case([n], [4099], kv_heads=1, layers=1, dim=8, sinks=3, recent=17, weights=weights)
 
 
 @pytest.mark.gpu
