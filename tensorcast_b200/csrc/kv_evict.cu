@@ -2,28 +2,26 @@
 // attention weight of every (sequence, layer, kv head) stay, and their rows are
 // copied in their old order to the sequence's destination pages.
 //
-// Two launches: select_kernel, one CTA per (layer, kv head, sequence), finds the
-// budget's weight by radix selection over the weights' order-preserving integer
-// images (11, 11 and 10 bits at a time, the images kept in shared memory) and writes
-// the kept indices; copy_kernel moves the rows, bound by HBM (each kept row is read
-// and written once; the sources of 256 rows are looked up first, so that a thread has
-// eight 16-byte loads under way). The destination pages are not the
-// source's: a page may be shared with other sequences, and the copy needs no
-// order between its CTAs. Measured on B200: 24 sequences of 500-8192 tokens, 4 layers,
-// budget 2048, 1.28 GB in 256 us (30 us for the selection; the copy 6.1 TB/s, 0.94 of
-// the measured copy rate).
+// One launch, one CTA per (layer, kv head, sequence), or some where those are few: it finds the budget's weight by
+// radix selection over the weights' order-preserving integer images (11, 11 and 10 bits
+// at a time, the images kept in shared memory), writes its share of the kept indices
+// and moves those rows of its head in both planes, so that one list's selection runs beside others' copies.
+// Bound by HBM: each kept row is read and written once; the places of 512 rows are
+// looked up first, so that a thread has eight 16-byte loads under way. The destination
+// pages are not the source's: a page may be shared with other sequences, and the copy
+// needs no order between its CTAs. Measured on B200: 24 sequences of 500-8192 tokens, 4
+// layers, budget 2048, 1.28 GB in @@ us (@@ TB/s, @@ of the measured copy rate; with
+// the copy as a second launch 256 us).
 #include <cuda_runtime.h>
 
 #include <algorithm>
 
-#include "sm100.cuh"
 #include "tcx_internal.h"
 
 namespace tcx {
 namespace {
 
-constexpr int kSelectThreads = 512;
-constexpr int kCopyThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kBins = 2048;
 constexpr int kBatch = 8;                 // tokens of a thread in a round of the last pass
 constexpr uint32_t kHeldTokens = 14336;   // images that shared memory holds: 56 KiB, three CTAs on an SM
@@ -92,31 +90,11 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* warp_sums, 
   return before + inc - v;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
-  extern __shared__ uint32_t held[];
-  __shared__ uint32_t bins[kBins], warp_sums[kSelectThreads / 32], s_pick[2];
-  const uint32_t head = blockIdx.x, layer = blockIdx.y, s = blockIdx.z;
-  next_may_start();
-  uint32_t n, kept;
-  lengths(a, s, &n, &kept);
-  const uint64_t base = a.page_offsets[s] * a.page_tokens, dst_base = a.dst_page_offsets[s] * a.page_tokens;
-  const uint64_t dst_cap = a.dst_page_offsets[s + 1] * a.page_tokens - dst_base;
-  const float* w = a.weights + layer * a.weights_layer_stride + head * a.weights_head_stride + base;
-  const uint64_t plane = (static_cast<uint64_t>(layer) * a.kv_heads + head) * a.dst_capacity + dst_base;
-  int32_t* keep = a.keep + plane;
-  float* left = a.dst_weights + plane;
-  if (layer == 0 && head == 0 && threadIdx.x == 0) a.dst_tokens[s] = kept;
-  for (uint64_t r = kept + threadIdx.x; r < dst_cap; r += blockDim.x) {
-    keep[r] = -1;
-    left[r] = 0.f;
-  }
-  if (n == kept) {
-    for (uint32_t j = threadIdx.x; j < n; j += blockDim.x) {
-      keep[j] = static_cast<int32_t>(j);
-      left[j] = w[j];
-    }
-    return;
-  }
+// The indices (in order) and weights of the `kept` of n tokens that stay.
+// Those from index r_begin to r_end are written.
+__device__ void select_tokens(const EvictArgs& a, const float* w, uint32_t n, uint32_t kept, uint32_t r_begin,
+                              uint32_t r_end, int32_t* keep, float* left, uint32_t* held) {
+  __shared__ uint32_t bins[kBins], warp_sums[kThreads / 32], s_pick[2];
   // The first `first` and the tokens from `last` on stay; `want` more of those between.
   const uint32_t first = static_cast<uint32_t>(min(a.sinks, static_cast<uint64_t>(kept)));
   const uint32_t newest = static_cast<uint32_t>(min(a.recent, static_cast<uint64_t>(kept - first)));
@@ -127,10 +105,10 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
   for (int pass = 0; any && pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
     const uint32_t known = pass == 0 ? 0 : ~0u << (shift + bits);
-    for (uint32_t b = threadIdx.x; b < kBins; b += kSelectThreads) bins[b] = 0;
+    for (uint32_t b = threadIdx.x; b < kBins; b += kThreads) bins[b] = 0;
     __syncthreads();
 #pragma unroll 4
-    for (uint32_t j = first + threadIdx.x; j < last; j += kSelectThreads) {
+    for (uint32_t j = first + threadIdx.x; j < last; j += kThreads) {
       const uint32_t x = hold && pass > 0 ? held[j] : image(w[j]);
       if (hold && pass == 0) held[j] = x;
       if ((x & known) == prefix) atomicAdd(&bins[x >> shift & ((1u << bits) - 1)], 1u);
@@ -154,7 +132,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
   // `want` of the tokens with exactly this image stay, the lowest indices first. A
   // thread takes consecutive tokens, so that one scan numbers a round of them.
   uint32_t done = 0, equal_done = 0;
-  for (uint32_t j0 = 0; j0 < n; j0 += kSelectThreads * kBatch) {
+  for (uint32_t j0 = 0; j0 < n; j0 += kThreads * kBatch) {
     const uint32_t from = j0 + threadIdx.x * kBatch;
     float v[kBatch];
     uint32_t equal = 0, stays = 0, total;  // bits of the thread's tokens
@@ -175,74 +153,82 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictArgs a) {
     for (int k = 0; k < kBatch; ++k) {
       const bool stay = (stays >> k & 1) || ((equal >> k & 1) && equals < want);
       equals += equal >> k & 1;
-      if (stay) {
+      if (stay && r >= r_begin && r < r_end) {
         keep[r] = static_cast<int32_t>(from + k);
-        left[r++] = v[k];
+        left[r] = v[k];
       }
+      r += stay;
     }
     done += (total & 0xffff) + min(equal_done + (total >> 16), want) - min(equal_done, want);
     equal_done += total >> 16;
   }
 }
 
-// One CTA moves one destination page of one plane, in 16-byte pieces.
-__global__ void __launch_bounds__(kCopyThreads) copy_kernel(EvictArgs a) {
-  const uint64_t page = blockIdx.x;
-  const uint32_t plane = blockIdx.y;
-  uint32_t lo = 0, hi = a.n_seq;  // dst_page_offsets[lo] <= page < dst_page_offsets[lo + 1]
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (a.dst_page_offsets[mid] <= page) lo = mid; else hi = mid;
-  }
+__global__ void __launch_bounds__(kThreads, 2) evict_kernel(EvictArgs a) {
+  extern __shared__ uint32_t held[];
+  __shared__ uint64_t s_from[kThreads], s_to[kThreads];
+  const uint32_t shares = gridDim.x / a.kv_heads, share = blockIdx.x % shares;
+  const uint32_t head = blockIdx.x / shares, layer = blockIdx.y, s = blockIdx.z;
   uint32_t n, kept;
-  lengths(a, lo, &n, &kept);
-  const uint64_t r0 = (page - a.dst_page_offsets[lo]) * a.page_tokens;
-  if (r0 >= kept) {
-    wait_for_previous();  // also here: this kernel's end stands for the one's before
-    return;
-  }
-  const uint32_t rows = static_cast<uint32_t>(min(static_cast<uint64_t>(a.page_tokens), kept - r0));
-  const uint32_t dst_slot = a.dst_page_table[page];
-  if (dst_slot >= a.pool_pages) {
-    if (threadIdx.x == 0) atomicCAS(a.status, 0u, 1u);
-    wait_for_previous();
-    return;
-  }
-  const uint64_t plane_off = plane * a.pool_pages * a.page_bytes;
-  const uint32_t* table = a.page_table + a.page_offsets[lo];
-  const int32_t* keep = a.keep + static_cast<uint64_t>(plane / 2) * a.kv_heads * a.dst_capacity + page * a.page_tokens;
-  const uint32_t pieces = static_cast<uint32_t>(a.head_bytes / 16), entries = rows * a.kv_heads;
-  __shared__ uint64_t s_from[kCopyThreads];
-  uint8_t* to = a.pool + plane_off + dst_slot * a.page_bytes;  // the page's rows and heads, one after the other
-  wait_for_previous();                                         // the kept indices
-  for (uint32_t e0 = 0; e0 < entries; e0 += kCopyThreads) {
-    const uint32_t e = e0 + threadIdx.x;
-    uint64_t from = ~uint64_t{0};
-    if (e < entries) {
-      const uint32_t r = e / a.kv_heads, head = e % a.kv_heads;
-      const uint32_t j = static_cast<uint32_t>(keep[head * a.dst_capacity + r]);
-      const uint32_t slot = table[j / a.page_tokens];
-      if (slot < a.pool_pages)
-        from = plane_off + slot * a.page_bytes + j % a.page_tokens * a.token_bytes + head * a.head_bytes;
-      else
-        atomicCAS(a.status, 0u, 1u);
+  lengths(a, s, &n, &kept);
+  const uint64_t base = a.page_offsets[s] * a.page_tokens, dst_base = a.dst_page_offsets[s] * a.page_tokens;
+  const uint64_t dst_cap = a.dst_page_offsets[s + 1] * a.page_tokens - dst_base;
+  const float* w = a.weights + layer * a.weights_layer_stride + head * a.weights_head_stride + base;
+  const uint64_t plane = (static_cast<uint64_t>(layer) * a.kv_heads + head) * a.dst_capacity + dst_base;
+  int32_t* keep = a.keep + plane;
+  float* left = a.dst_weights + plane;
+  const uint32_t r_begin = static_cast<uint32_t>(static_cast<uint64_t>(kept) * share / shares);
+  const uint32_t r_end = static_cast<uint32_t>(static_cast<uint64_t>(kept) * (share + 1) / shares);
+  if (share == 0) {
+    if (layer == 0 && head == 0 && threadIdx.x == 0) a.dst_tokens[s] = kept;
+    for (uint64_t r = kept + threadIdx.x; r < dst_cap; r += blockDim.x) {
+      keep[r] = -1;
+      left[r] = 0.f;
     }
-    s_from[threadIdx.x] = from;
+  }
+  if (n == kept) {
+    for (uint32_t j = r_begin + threadIdx.x; j < r_end; j += blockDim.x) {
+      keep[j] = static_cast<int32_t>(j);
+      left[j] = w[j];
+    }
+  } else {
+    select_tokens(a, w, n, kept, r_begin, r_end, keep, left, held);
+  }
+  __syncthreads();
+  // The kept rows of this head, 512 at a time.
+  constexpr uint64_t kNone = ~uint64_t{0};
+  const uint32_t* table = a.page_table + a.page_offsets[s];
+  const uint32_t* dst_table = a.dst_page_table + a.dst_page_offsets[s];
+  const uint32_t pieces = static_cast<uint32_t>(a.head_bytes / 16);
+  for (uint32_t r0 = r_begin; r0 < r_end; r0 += kThreads) {
+    const uint32_t r = r0 + threadIdx.x;
+    if (r < r_end) {
+      const uint32_t j = static_cast<uint32_t>(keep[r]);
+      const uint32_t slot = table[j / a.page_tokens], dst_slot = dst_table[r / a.page_tokens];
+      const bool good = slot < a.pool_pages && dst_slot < a.pool_pages;
+      if (!good) atomicCAS(a.status, 0u, 1u);
+      s_from[threadIdx.x] =
+          good ? slot * a.page_bytes + j % a.page_tokens * a.token_bytes + head * a.head_bytes : kNone;
+      s_to[threadIdx.x] = dst_slot * a.page_bytes + r % a.page_tokens * a.token_bytes + head * a.head_bytes;
+    }
     __syncthreads();
-    const uint32_t moves = min(entries - e0, static_cast<uint32_t>(kCopyThreads)) * pieces;
-    for (uint32_t i0 = threadIdx.x; i0 < moves; i0 += 8 * kCopyThreads) {
-      uint4 v[8];
+    const uint32_t moves = min(r_end - r0, static_cast<uint32_t>(kThreads)) * pieces;
+    for (uint32_t plane = 2 * layer; plane < 2 * layer + 2; ++plane) {
+      uint8_t* rows = a.pool + plane * a.pool_pages * a.page_bytes;
+      for (uint32_t i0 = threadIdx.x; i0 < moves; i0 += 8 * kThreads) {
+        uint4 v[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t i = i0 + k * kCopyThreads;
-        if (i < moves && s_from[i / pieces] != ~uint64_t{0})
-          v[k] = __ldcs(reinterpret_cast<const uint4*>(a.pool + s_from[i / pieces]) + i % pieces);
-      }
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t i = i0 + k * kThreads;
+          if (i < moves && s_from[i / pieces] != kNone)
+            v[k] = __ldcs(reinterpret_cast<const uint4*>(rows + s_from[i / pieces]) + i % pieces);
+        }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t i = i0 + k * kCopyThreads;
-        if (i < moves && s_from[i / pieces] != ~uint64_t{0})
-          reinterpret_cast<uint4*>(to + static_cast<uint64_t>(e0) * a.head_bytes)[i] = v[k];
+        for (int k = 0; k < 8; ++k) {
+          const uint32_t i = i0 + k * kThreads;
+          if (i < moves && s_from[i / pieces] != kNone)
+            *(reinterpret_cast<uint4*>(rows + s_to[i / pieces]) + i % pieces) = v[k];
+        }
       }
     }
     __syncthreads();
@@ -303,17 +289,15 @@ extern "C" tcx_status tcx_kv_evict(const tcx_kv_evict_args* args, void* stream) 
   a.dst_weights = x.d_dst_weights;
   a.dst_tokens = x.d_dst_tokens;
   a.status = x.d_status;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const dim3 select_grid(a.kv_heads, static_cast<unsigned>(x.planes / 2), a.n_seq);
   static std::atomic<uint64_t> allowed{0};
-  if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(select_kernel), kSelectShared, &allowed); st != TCX_OK)
+  if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(evict_kernel), kSelectShared, &allowed); st != TCX_OK)
     return st;
-  select_kernel<<<select_grid, kSelectThreads, kSelectShared, s>>>(a);
+  // Few lists: several CTAs select the same one, and each moves a share of its rows.
+  const uint64_t lists = static_cast<uint64_t>(a.kv_heads) * (x.planes / 2) * a.n_seq;
+  const uint64_t shares = std::max<uint64_t>(1, std::min<uint64_t>(16, 2ull * sm_count() / lists));
+  const dim3 grid(static_cast<unsigned>(a.kv_heads * shares), static_cast<unsigned>(x.planes / 2), a.n_seq);
+  evict_kernel<<<grid, kThreads, kSelectShared, static_cast<cudaStream_t>(stream)>>>(a);
   note_launches(1);
   TCX_CUDA_TRY(cudaGetLastError());
-  if (x.dst_total_pages != 0) {
-    const dim3 copy_grid(static_cast<unsigned>(x.dst_total_pages), static_cast<unsigned>(x.planes));
-    return launch_after(copy_kernel, copy_grid, dim3(kCopyThreads), 0, s, a);
-  }
   return TCX_OK;
 }

@@ -532,7 +532,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       auto low_of = [&](int pos) {
         return a.window ? static_cast<int>(max(int64_t{0}, pos - a.window + 1)) : 0;
       };
-      if (d.prefix) {
+      if (d.prefix && d.max_q == 1 && a.window == 0) {
+        // one query each stands behind the whole prefix, and sees it
+        hi = r < it.rows ? prefix - 1 : -1;
+        all_hi = any_hi = prefix - 1;
+        all_lo = any_lo = 0;
+      } else if (d.prefix) {
         if (r < it.rows) {
           const uint32_t t = it.q_first + row / a.group, s = seq_of(a, t);
           const int nq = static_cast<int>(a.q_offsets[s + 1] - a.q_offsets[s]);

@@ -269,7 +269,9 @@ class KvAttention(_OnDevice):
         if a.q_tokens:
             current = self._current()
             scratch, need = self._workspace(a, current)
-            _native.call("tcx_kv_attention", ctypes.byref(a), scratch, need, current)
+            rc = _native.lib().tcx_kv_attention(ctypes.byref(a), scratch, need, current)
+            if rc:
+                _native._raise(rc)
         return out, lse
 
     def check_status(self) -> None:
