@@ -185,8 +185,8 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     wait_for_previous();
     return;
   }
-  const uint32_t t0 = static_cast<uint32_t>(static_cast<uint64_t>(range) * total / ranges);
-  const uint32_t t1 = static_cast<uint32_t>(static_cast<uint64_t>(range + 1) * total / ranges);
+  const uint32_t t0 = static_cast<uint32_t>(scaled(range, total, ranges));
+  const uint32_t t1 = static_cast<uint32_t>(scaled(range + 1, total, ranges));
   if (before <= t0 && t0 < before + mine) {
     uint32_t s = s0, at = before;
     for (;; ++s) {
@@ -220,7 +220,8 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     };
     uint32_t s = s_begin[0], t = s_begin[1], next_s = s;
     SeqInfo q = seq_info(a, s, prefix), next = q;
-    uint32_t slots_from = t, slots = slots_of(q, t), slots_ahead = slots_of(q, t + per), next_slots = 0;
+    uint32_t slots_from = t, slots = slots_of(q, t), next_slots = 0;
+    uint32_t slots_ahead = count > per ? slots_of(q, t + per) : 0;
     bool fresh = true;  // the next tile is the first of its piece
     uint32_t pieces = 0;
     uint32_t i = 0;
@@ -233,34 +234,13 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
         slots_ahead = slots_of(q, t + per);
       }
       const uint32_t slot = __shfl_sync(~0u, slots, (t - slots_from) * boxes + box);
-      TileInfo info{fresh ? kFirst : 0u, s, q.q_first, q.queries, token, q.len, q.low, q.sinks, 0, 0, 0};
-      const bool seq_done = t + 1 == q.tiles;
-      if (seq_done || i + 1 == count) info.flags |= kLast;
-      const bool starts = s != s_begin[0] || s_begin[1] == 0;
-      if (seq_done && starts) info.flags |= kWhole;
-      if ((info.flags & kLast) && !(info.flags & kWhole)) {
-        // the ranges that hold tiles [first, first + q.tiles)
-        const uint64_t first = t0 + i - t;
-        auto range_of = [&](uint64_t tile) { return static_cast<uint32_t>(((tile + 1) * ranges - 1) / total); };
-        info.first_range = range_of(first);
-        info.parts = range_of(first + q.tiles - 1) - info.first_range + 1;
-        info.first_slot = first != static_cast<uint64_t>(info.first_range) * total / ranges;
-      }
-      if (pieces > 0) info.flags |= kSecondSlot;
-      const int last_low = a.window ? q.low + static_cast<int>(q.queries) - 1 : 0;  // at least the last query's
-      if (token + kTile - 1 > q.len - static_cast<int>(q.queries) ||
-          (token < last_low && token + kTile > q.sinks))
-        info.flags |= kMask;
       if (!mbar_wait_warp(smem_addr(&s_empty[stage]), (i / L::kStages & 1) ^ 1, &s_gave_up, a.status)) break;
       const uint32_t full = smem_addr(&s_full[stage]), at = base + stage * L::kStage;
       const int from = token + static_cast<int>(box * a.box_rows);
       const bool wanted = lane < 2 * halves * boxes && wanted_box(q, from);
       const uint32_t rows = fresh ? min(q.queries * a.group, static_cast<uint32_t>(kRows)) : 0;
       const uint32_t bytes = __popc(__ballot_sync(~0u, wanted)) * a.box_rows * 128 + rows * D * 2;
-      if (lane == 0) {
-        s_info[stage] = info;
-        if (bytes) mbar_arrive_expect(full, bytes); else mbar_arrive(full);
-      }
+      if (lane == 0) mbar_expect(full, bytes);
       __syncwarp();
       if (wanted)
         tma_load_3d(at + plane * L::kKeys + half * L::kHalf + box * a.box_rows * 128, &map, half * 64, head,
@@ -270,6 +250,30 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
                   a.q + (q.q_first + lane / a.group) * a.q_token_stride +
                       (head * a.group + lane % a.group) * a.q_head_stride,
                   D * 2, full);
+      // What the consumers need is worked out while the copies run; they wait for both.
+      TileInfo info{fresh ? kFirst : 0u, s, q.q_first, q.queries, token, q.len, q.low, q.sinks, 0, 0, 0};
+      const bool seq_done = t + 1 == q.tiles;
+      if (seq_done || i + 1 == count) info.flags |= kLast;
+      const bool starts = s != s_begin[0] || s_begin[1] == 0;
+      if (seq_done && starts) info.flags |= kWhole;
+      if ((info.flags & kLast) && !(info.flags & kWhole)) {
+        // the ranges that hold tiles [first, first + q.tiles)
+        const uint64_t first = t0 + i - t;
+        // the last range that begins at a tile or before: ((tile + 1) ranges - 1) / total
+        auto range_of = [&](uint64_t tile) { return static_cast<uint32_t>(scaled((tile + 1) * ranges - 1, 1, total)); };
+        info.first_range = range_of(first);
+        info.parts = range_of(first + q.tiles - 1) - info.first_range + 1;
+        info.first_slot = first != scaled(info.first_range, total, ranges);
+      }
+      if (pieces > 0) info.flags |= kSecondSlot;
+      const int last_low = a.window ? q.low + static_cast<int>(q.queries) - 1 : 0;  // at least the last query's
+      if (token + kTile - 1 > q.len - static_cast<int>(q.queries) ||
+          (token < last_low && token + kTile > q.sinks))
+        info.flags |= kMask;
+      if (lane == 0) {
+        s_info[stage] = info;
+        mbar_arrive(full);
+      }
       if (fresh && i + (q.tiles - t) < count) {  // the next sequence is this range's too
         next_s = s;
         do next = seq_info(a, ++next_s, prefix); while (next.tiles == 0);

@@ -124,7 +124,7 @@ __device__ Item make_item(const TileArgs& d, uint32_t s, uint32_t index, int pre
 
 // Every range must hold more than a piece's cost to hold a tile.
 __device__ __forceinline__ uint64_t piece_cost(uint64_t units, uint64_t pieces, uint32_t ranges) {
-  return (units + kPieceCost * pieces) / ranges > kPieceCost ? kPieceCost : 0;
+  return scaled(units + kPieceCost * pieces, 1, ranges) > kPieceCost ? kPieceCost : 0;
 }
 
 // Exclusive sum over the CTA; *total gets the sum.
@@ -333,9 +333,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   }
   auto begin_of = [&](uint32_t r) {
     if (!d.prefix) return d.begin[r];
-    const uint64_t pieces = static_cast<uint64_t>(items) * a.kv_heads, at = pieces * (same_tiles + cost) * r / ranges;
-    const uint64_t piece = at / (same_tiles + cost), tile = max(at % (same_tiles + cost), cost) - cost;
-    return RangeBegin{static_cast<uint32_t>(piece / a.kv_heads), static_cast<uint32_t>(piece % a.kv_heads),
+    const uint64_t pieces = static_cast<uint64_t>(items) * a.kv_heads, each = same_tiles + cost;
+    const uint64_t at = scaled(pieces * each, r, ranges), piece = scaled(at, 1, each);
+    const uint64_t tile = max(at - piece * each, cost) - cost, first = scaled(piece, 1, a.kv_heads);
+    return RangeBegin{static_cast<uint32_t>(first), static_cast<uint32_t>(piece - first * a.kv_heads),
                       static_cast<uint32_t>(tile), piece * same_tiles + tile};
   };
   auto item_of = [&](uint32_t i) { return d.prefix ? make_item(d, 0, i, prefix) : d.items[i]; };

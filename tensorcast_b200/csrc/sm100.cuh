@@ -42,6 +42,17 @@ __device__ __forceinline__ void mbar_arrive_expect(uint32_t bar, uint32_t bytes)
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+// a b / c; 32-bit division where that holds the product (a 64-bit one takes some
+// hundred cycles at the start of a small call).
+__device__ __forceinline__ uint64_t scaled(uint64_t a, uint64_t b, uint64_t c) {
+  const uint64_t product = a * b;
+  return (product | c) >> 32 ? product / c : static_cast<uint32_t>(product) / static_cast<uint32_t>(c);
+}
+
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
