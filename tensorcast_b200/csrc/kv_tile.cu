@@ -26,10 +26,12 @@
 //
 // Bound by the softmax: a unit's products take 2560 cycles, its exponentials 1536 on
 // the exponential units (a fourth of them runs on the FMA units), and the two warps of
-// a scheduler take about 3500 for all of it; tensor cores 0.46 to 0.6 busy. Measured on
-// B200: 2048 queries at the end of 40011 tokens, 32 / 8 heads of 128, 1.23 ms in a
-// burst (1060 TFLOP/s, 0.63 of the measured burst rate), 1.44 ms back to back under the
-// power cap (0.65 of the sustained rate).
+// a scheduler take about 3700 for all of it (loads from tensor memory, waits and the
+// exponentials of both at once); a piece of a row tile costs some 10000 more for its
+// first scores, its masked tile and its output. Measured on B200: 2048 queries at the end
+// of 40011 tokens, 32 / 8 heads of 128, 1.23 to 1.30 ms in a burst (up to 1060 TFLOP/s,
+// 0.63 of the measured burst rate), 1.44 to 1.48 ms back to back under the power cap (0.63
+// to 0.65 of the sustained rate).
 #include <algorithm>
 #include <type_traits>
 

@@ -78,6 +78,8 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
     s_gave_up = s_drained = 0;
     mbar_init_fence();
   }
+  // The kernel before may still hold tensor memory, but on no SM of this CTA's: its
+  // registers and shared memory leave no room beside it.
   if (warp == kWorkers / 32) tmem_alloc(smem_addr(&s_tmem), 2 * kRows);
   tmem_fence_before();
   __syncthreads();

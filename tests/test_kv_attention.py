@@ -253,6 +253,33 @@ def test_shared_prefix_batches(cuda_device, group, dim, batch, window, sinks):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 4), (350, 310), (1, 0)])
+@pytest.mark.parametrize("group,dim", [(4, 64), (1, 128)])
+def test_shared_prefix_with_prompts(cuda_device, window, sinks, group, dim):
+    """Many queries behind a prefix, some standing inside it, the windows reaching back across its end."""
+    run([0, 50, 130, 7, 260], [3, 50, 70, 12, 260], kv_heads=2, group=group, dim=dim, prefix=301, window=window,
+        sinks=sinks)
+
+
+@pytest.mark.gpu
+def test_lengths_of_the_prefix_and_the_sequences_may_change(cuda_device):
+    w, free = kvtools.tables([40, 5], spare=2, taken=12)
+    pool = kvtools.make_pool(w, 2, 64, BF16).cuda()
+    q = queries(2, 8, 64, BF16, 0)
+    att = KvAttention(w, 8, 2, prefix_pages=free[:12], prefix_tokens=100)
+    for prefix, tokens in ((100, [40, 5]), (0, [0, 21]), (1, [1, 0]), (192, [70, 33])):
+        att.prefix_tokens.fill_(prefix)
+        att.seq_tokens.copy_(torch.tensor(tokens, dtype=torch.int32))
+        rows = free[:12][np.arange(prefix) // 16].astype(np.int64) * 16 + np.arange(prefix) % 16
+        check(att.run(pool, 0, q), kvtools.attention(w, pool, 0, q, [1, 1], prefix_rows=rows, tokens=tokens), BF16, 300)
+    att.check_status()
+    att.prefix_tokens.fill_(193)
+    att.run(pool, 0, q)
+    with pytest.raises(_native.TcxError, match="more tokens"):
+        att.check_status()
+
+
+@pytest.mark.gpu
 def test_large_scores_and_small_scale(cuda_device):
     run(LENGTHS, [1] * len(LENGTHS), scale=3.0)
     run([300], [300], kv_heads=1, scale=3.0)
