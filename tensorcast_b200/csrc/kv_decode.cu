@@ -137,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   __shared__ TileInfo s_info[L::kStages];
   __shared__ uint64_t s_full[L::kStages], s_empty[L::kStages];
   __shared__ uint32_t s_scan[kThreads / 32], s_begin[2], s_gave_up, s_drained, s_last;
-  __shared__ float2 s_ml[kWarps][kRows];
+  __shared__ float2 s_ml[2][kWarps][kRows];  // by turns: a warp may be a sequence ahead of the others
   const AttnArgs& a = d.a;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t head = blockIdx.x % a.kv_heads, range = blockIdx.x / a.kv_heads;
@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   uint32_t qf[D / 16][4];
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   bool alive = true;
+  uint32_t turn = 0;
   for (uint32_t i = 0; i < count; ++i) {
     const uint32_t stage = i % L::kStages, at = base + stage * L::kStage;
     alive = alive && mbar_wait_warp(smem_addr(&s_full[stage]), i / L::kStages & 1, &s_gave_up, a.status);
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       for (int r = 0; r < 2; ++r) {
         l[r] += __shfl_xor_sync(~0u, l[r], 1);
         l[r] += __shfl_xor_sync(~0u, l[r], 2);
-        if (lane % 4 == 0) s_ml[warp][lane / 4 + 8 * r] = make_float2(m[r], l[r]);
+        if (lane % 4 == 0) s_ml[turn][warp][lane / 4 + 8 * r] = make_float2(m[r], l[r]);
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
       float* join = reinterpret_cast<float*>(raw + (at - smem_addr(raw)));  // [warp][row][D]
@@ -452,12 +453,12 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       for (uint32_t r = threadIdx.x / kLanes; r < rows; r += 128 / kLanes) {
         const uint32_t e = threadIdx.x % kLanes * 4;
         float top = -INFINITY, sum = 0.f;
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[w][r].x);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[turn][w][r].x);
         const float ref = top == -INFINITY ? 0.f : top;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int w = 0; w < kWarps; ++w) {
-          const float f = exp2_approx(s_ml[w][r].x - ref);
-          sum += f * s_ml[w][r].y;
+          const float f = exp2_approx(s_ml[turn][w][r].x - ref);
+          sum += f * s_ml[turn][w][r].y;
           const float4 x = *reinterpret_cast<const float4*>(join + (w * kRows + r) * D + e);
           v.x += f * x.x;
           v.y += f * x.y;
@@ -477,6 +478,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
           if (e == 0) d.part_ml[row] = make_float2(top, sum);
         }
       }
+      turn ^= 1;
       if (!(info.flags & kWhole)) {  // whoever comes last adds the parts up, in the ranges' order
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (threadIdx.x == 0)
