@@ -169,7 +169,7 @@ inline uint64_t align256(uint64_t n) { return (n + 255) / 256 * 256; }
 tcx_status encode_pool_map(const tcx_kv_attention_args& x, uint32_t box_rows, CUtensorMap* map);
 
 // Decode: few rows for each sequence and kv head (kv_decode.cu).
-constexpr uint32_t kDecodeRows = 16;
+constexpr uint32_t kDecodeRows = 32;
 bool decode_fits(const tcx_kv_attention_args& x);
 uint64_t decode_scratch_bytes(const tcx_kv_attention_args& x);
 tcx_status launch_decode(const tcx_kv_attention_args& x, const AttnArgs& a, const CUtensorMap& map, void* scratch,

@@ -1,6 +1,6 @@
 // Attention of few query rows over long paged sequences (decode).
 //
-// A kv head's rows (query tokens x the head's group of q heads, up to 16) share
+// A kv head's rows (query tokens x the head's group of q heads, up to 32) share
 // the keys and values, so the call is bound by reading every visible key and value
 // once from HBM. The visible tokens of all sequences are laid end to end in tiles
 // of 64, and that axis is cut into equal ranges, one CTA for each range and kv
@@ -9,11 +9,11 @@
 // token's heads are fetched at about the same time.
 //
 // In a CTA one warp fills a ring of tiles with TMA (a box for each run of rows
-// within a page), four warps take 16 tokens of a tile each: scores by mma, a running
-// maximum and sum in 32 bits, probabilities rounded to the input type (half a step,
-// as the output is: the two roundings together leave 1.1 to 1.2 times the output's own
-// error) for the second product, sums in 32 bits. Where a sequence ends
-// inside a range the four warps' parts are joined in the tile's memory and written;
+// within a page). Of four warps (of each four, with more than 16 rows) each takes 16
+// tokens of a tile: scores by mma, a running maximum and sum in 32 bits, probabilities
+// rounded to the input type (half a step, as the output is: the two roundings together
+// leave 1.1 to 1.2 times the output's own error) for the second product, sums in 32
+// bits. Where a sequence ends inside a range the warps' parts are joined and written;
 // a sequence cut by a range's border leaves parts in the scratch, and the CTA that
 // comes last adds them up in the ranges' order. Where weights are accumulated, the
 // scores go to the scratch as well (rows x 4 bytes for a token, against its 4 D), and
@@ -31,9 +31,8 @@ namespace tcx {
 namespace {
 
 constexpr int kTile = 64;
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * (kWarps + 1);
-constexpr int kRows = kDecodeRows;
+constexpr int kWarps = 4;       // for each 16 rows: 16 tokens of a tile each
+constexpr int kWarpRows = 16;
 
 enum : uint32_t { kFirst = 1, kLast = 2, kMask = 4, kWhole = 8, kSecondSlot = 16 };
 
@@ -47,21 +46,24 @@ struct TileInfo {
 struct DecodeArgs {
   AttnArgs a;
   uint32_t ranges, rows;  // at most
-  float* part_o;    // [ranges][2][kv_heads][kRows][D], sums of 2^(z - m) v
+  uint32_t part_rows;     // 16 or 32
+  float* part_o;    // [ranges][2][kv_heads][part_rows][D], sums of 2^(z - m) v
   float2* part_ml;  // the same rows' m and sum of 2^(z - m)
   float* scores;    // [kv_heads][rows][columns], in powers of two, where weights are added up
   uint32_t score_rows;
   uint64_t columns;
 };
 
-template <int D>
+template <int D, int G>
 struct Layout {
+  static constexpr int kRows = kWarpRows * G;
   static constexpr int kHalf = kTile * 128;              // 64 values of each token: 128-byte rows, swizzled
   static constexpr int kKeys = kHalf * (D / 64);
   static constexpr int kQueryPitch = D * 2 + 16;          // 16 bytes more: rows in different banks
   static constexpr int kQueries = kRows * kQueryPitch;
   static constexpr int kStage = 2 * kKeys + (kQueries + 1023) / 1024 * 1024;
-  static constexpr int kStages = D == 128 ? 3 : 5;
+  // two CTAs fit an SM with 16 rows, one with 32
+  static constexpr int kStages = (D == 128 ? 3 : 5) + (G == 1 ? 0 : D == 128 ? 2 : 3);
   static constexpr int kBytes = kStages * kStage + 1024;  // the first tile starts on a 1 KiB border
 };
 
@@ -94,16 +96,16 @@ __device__ __forceinline__ SeqInfo seq_info(const AttnArgs& a, uint32_t s, int p
 
 // The rows of a sequence that several ranges hold: D / 4 threads to a row, the parts
 // in the ranges' order.
-template <typename T, int D>
+template <typename T, int D, int G>
 __device__ __forceinline__ void join_parts(const DecodeArgs& d, const TileInfo& info, uint32_t head, uint32_t rows) {
   const AttnArgs& a = d.a;
   constexpr uint32_t kLanes = D / 4;
   const uint32_t lane = threadIdx.x % kLanes, e = lane * 4;
-  for (uint32_t r0 = 0; r0 < rows; r0 += 128 / kLanes) {
+  for (uint32_t r0 = 0; r0 < rows; r0 += 128 * G / kLanes) {
     const uint32_t r = min(r0 + threadIdx.x / kLanes, rows - 1);  // all lanes take part in the shuffles
     auto row_of = [&](uint32_t k) {
       return (static_cast<uint64_t>((info.first_range + k) * 2 + (k == 0 ? info.first_slot : 0)) * a.kv_heads + head) *
-                 kRows + r;
+                 (kWarpRows * G) + r;
     };
     float top = -INFINITY, sum = 0.f, x[4] = {};
     for (uint32_t k = lane; k < info.parts; k += kLanes) top = fmaxf(top, __ldcg(&d.part_ml[row_of(k)].x));
@@ -130,14 +132,16 @@ __device__ __forceinline__ void join_parts(const DecodeArgs& d, const TileInfo& 
   __syncwarp();
 }
 
-template <typename T, int D, bool kScores>
-__global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_constant__ CUtensorMap map, DecodeArgs d) {
-  using L = Layout<D>;
+template <typename T, int D, bool kScores, int G>
+__global__ void __launch_bounds__(32 * (kWarps * G + 1), G == 1 ? 2 : 1)
+    decode_kernel(const __grid_constant__ CUtensorMap map, DecodeArgs d) {
+  using L = Layout<D, G>;
+  constexpr int kThreads = 32 * (kWarps * G + 1), kRows = L::kRows;
   extern __shared__ uint8_t raw[];
   __shared__ TileInfo s_info[L::kStages];
   __shared__ uint64_t s_full[L::kStages], s_empty[L::kStages];
   __shared__ uint32_t s_scan[kThreads / 32], s_begin[2], s_gave_up, s_drained, s_last;
-  __shared__ float2 s_ml[2][kWarps][kRows];  // by turns: a warp may be a sequence ahead of the others
+  __shared__ float2 s_ml[kWarps * G][kWarpRows];
   const AttnArgs& a = d.a;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t head = blockIdx.x % a.kv_heads, range = blockIdx.x / a.kv_heads;
@@ -146,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   if (threadIdx.x == 0) {
     for (int i = 0; i < L::kStages; ++i) {
       mbar_init(smem_addr(&s_full[i]), 1);
-      mbar_init(smem_addr(&s_empty[i]), kWarps);
+      mbar_init(smem_addr(&s_empty[i]), kWarps * G);
     }
     s_gave_up = s_drained = 0;
     mbar_init_fence();
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
   __syncthreads();
   const uint32_t count = t1 - t0;
 
-  if (warp == kWarps) {  // ---- the producer
+  if (warp == kWarps * G) {  // ---- the producer
     const uint32_t boxes = kTile / a.box_rows, halves = D / 64;
     // lane: one box of the keys or values and one half of the head
     const uint32_t box = lane % boxes, half = lane / boxes % halves, plane = lane / boxes / halves;
@@ -297,11 +301,12 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     return;
   }
 
-  // ---- the consumers: rows lane / 4 and lane / 4 + 8, tokens 16 warp .. 16 warp + 15 of each tile
+  // ---- the consumers: rows row0 + lane / 4 and 8 more, tokens 16 part .. 16 part + 15 of each tile
+  const uint32_t part = warp % kWarps, row0 = warp / kWarps * kWarpRows;
+  auto meet = [&] { asm volatile("bar.sync 1, %0;" ::"n"(128 * G) : "memory"); };
   uint32_t qf[D / 16][4];
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
   bool alive = true;
-  uint32_t turn = 0;
   for (uint32_t i = 0; i < count; ++i) {
     const uint32_t stage = i % L::kStages, at = base + stage * L::kStage;
     alive = alive && mbar_wait_warp(smem_addr(&s_full[stage]), i / L::kStages & 1, &s_gave_up, a.status);
@@ -309,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     if (info.flags & kFirst) {
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
-        ldmatrix4(qf[k], at + 2 * L::kKeys + lane % 16 * L::kQueryPitch + k * 32 + lane / 16 * 16);
+        ldmatrix4(qf[k], at + 2 * L::kKeys + (row0 + lane % 16) * L::kQueryPitch + k * 32 + lane / 16 * 16);
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -321,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     // the softmax, so that their latencies do not add up.
     uint32_t kf[D / 16][4], vf[D / 16][4];
     {
-      const uint32_t token = warp * 16 + lane / 16 * 8 + lane % 8, chunk = lane / 8 % 2;
+      const uint32_t token = part * 16 + lane / 16 * 8 + lane % 8, chunk = lane / 8 % 2;
       const uint32_t row = at + token * 128;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
@@ -329,11 +334,11 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
     }
     if (info.flags & kMask) {
       // values that no row sees are cleared: 0 x NaN is not 0
-      const int hidden = info.token + static_cast<int>(warp * 16 + lane % 16);
+      const int hidden = info.token + static_cast<int>(part * 16 + lane % 16);
       const bool clear = hidden >= info.len || (hidden < info.low && hidden >= info.sinks);
       if (__any_sync(~0u, clear)) {
         if (clear) {
-          const uint32_t row = at + L::kKeys + lane / 16 * (L::kHalf * (D / 128)) + (warp * 16 + lane % 16) * 128;
+          const uint32_t row = at + L::kKeys + lane / 16 * (L::kHalf * (D / 128)) + (part * 16 + lane % 16) * 128;
           if (lane < 16 || D == 128)
             for (int c = 0; c < 8; ++c)
               asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(row + c * 16), "r"(0) : "memory");
@@ -343,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       }
     }
     {
-      const uint32_t token = warp * 16 + lane % 16;
+      const uint32_t token = part * 16 + lane % 16;
       const uint32_t row = at + L::kKeys + token * 128;
 #pragma unroll
       for (int n = 0; n < D / 16; ++n)
@@ -363,8 +368,8 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[n][e] += z2[n][e];
     if (info.flags & kMask) {
-      const int first = info.token + static_cast<int>(warp) * 16;
-      const uint32_t r = lane / 4;
+      const int first = info.token + static_cast<int>(part) * 16;
+      const uint32_t r = row0 + lane / 4;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -380,12 +385,12 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       const uint64_t column = a.page_offsets[info.seq] * a.page_tokens;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const uint32_t row = lane / 4 + 8 * r;
+        const uint32_t row = row0 + lane / 4 + 8 * r;
         if (row < info.queries * a.group && row < d.score_rows && alive) {
           float* to = d.scores + (static_cast<uint64_t>(head) * d.score_rows + row) * d.columns + column;
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            const int j = info.token + static_cast<int>(warp * 16 + n * 8 + lane % 4 * 2);
+            const int j = info.token + static_cast<int>(part * 16 + n * 8 + lane % 4 * 2);
             if (j < info.len)  // an even place: the pair's second is within the page
               *reinterpret_cast<float2*>(to + j) = make_float2(z[n][2 * r] * a.scale_log2, z[n][2 * r + 1] * a.scale_log2);
           }
@@ -437,54 +442,61 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
       for (int r = 0; r < 2; ++r) {
         l[r] += __shfl_xor_sync(~0u, l[r], 1);
         l[r] += __shfl_xor_sync(~0u, l[r], 2);
-        if (lane % 4 == 0) s_ml[turn][warp][lane / 4 + 8 * r] = make_float2(m[r], l[r]);
+        if (lane % 4 == 0) s_ml[warp][lane / 4 + 8 * r] = make_float2(m[r], l[r]);
       }
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      float* join = reinterpret_cast<float*>(raw + (at - smem_addr(raw)));  // [warp][row][D]
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        if (lane / 4 + 8 * r < rows)
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n)
-            *reinterpret_cast<float2*>(join + (warp * kRows + lane / 4 + 8 * r) * D + n * 8 + lane % 4 * 2) =
-                make_float2(o[n][2 * r], o[n][2 * r + 1]);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      meet();
+      float* join = reinterpret_cast<float*>(raw + (at - smem_addr(raw)));  // [part][row][D]
       constexpr uint32_t kLanes = D / 4;  // threads of a row: 4 values each
-      for (uint32_t r = threadIdx.x / kLanes; r < rows; r += 128 / kLanes) {
-        const uint32_t e = threadIdx.x % kLanes * 4;
-        float top = -INFINITY, sum = 0.f;
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_ml[turn][w][r].x);
-        const float ref = top == -INFINITY ? 0.f : top;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = 0; w < kWarps; ++w) {
-          const float f = exp2_approx(s_ml[turn][w][r].x - ref);
-          sum += f * s_ml[turn][w][r].y;
-          const float4 x = *reinterpret_cast<const float4*>(join + (w * kRows + r) * D + e);
-          v.x += f * x.x;
-          v.y += f * x.y;
-          v.z += f * x.z;
-          v.w += f * x.w;
+#pragma unroll
+      for (uint32_t g = 0; g < G; ++g) {  // 16 rows at a time: that is what the tile's memory holds
+        if (g > 0) meet();
+        if (row0 == g * kWarpRows) {
+#pragma unroll
+          for (int r = 0; r < 2; ++r)
+            if (row0 + lane / 4 + 8 * r < rows)
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n)
+                *reinterpret_cast<float2*>(join + (part * kWarpRows + lane / 4 + 8 * r) * D + n * 8 + lane % 4 * 2) =
+                    make_float2(o[n][2 * r], o[n][2 * r + 1]);
         }
-        if (!alive) continue;
-        if (info.flags & kWhole) {
-          const uint32_t t = info.q_first + r / a.group, h = head * a.group + r % a.group;
-          const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
-          store_row<T, D, 4>(a, t, h, e, f, {v.x, v.y, v.z, v.w});
-          if (e == 0) store_lse(a, t, h, f);
-        } else {
-          const uint64_t row = (static_cast<uint64_t>(range * 2 + (info.flags & kSecondSlot ? 1 : 0)) * a.kv_heads + head) *
-                                   kRows + r;
-          *reinterpret_cast<float4*>(d.part_o + row * D + e) = v;
-          if (e == 0) d.part_ml[row] = make_float2(top, sum);
+        meet();
+        const uint32_t here = min(rows - min(rows, g * kWarpRows), static_cast<uint32_t>(kWarpRows));
+        for (uint32_t in = threadIdx.x / kLanes; in < here; in += 128 * G / kLanes) {
+          const uint32_t e = threadIdx.x % kLanes * 4, r = g * kWarpRows + in;
+          const float2(*ml)[kWarpRows] = s_ml + g * kWarps;
+          float top = -INFINITY, sum = 0.f;
+          for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml[w][in].x);
+          const float ref = top == -INFINITY ? 0.f : top;
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int w = 0; w < kWarps; ++w) {
+            const float f = exp2_approx(ml[w][in].x - ref);
+            sum += f * ml[w][in].y;
+            const float4 x = *reinterpret_cast<const float4*>(join + (w * kWarpRows + in) * D + e);
+            v.x += f * x.x;
+            v.y += f * x.y;
+            v.z += f * x.z;
+            v.w += f * x.w;
+          }
+          if (!alive) continue;
+          if (info.flags & kWhole) {
+            const uint32_t t = info.q_first + r / a.group, h = head * a.group + r % a.group;
+            const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
+            store_row<T, D, 4>(a, t, h, e, f, {v.x, v.y, v.z, v.w});
+            if (e == 0) store_lse(a, t, h, f);
+          } else {
+            const uint64_t row =
+                (static_cast<uint64_t>(range * 2 + (info.flags & kSecondSlot ? 1 : 0)) * a.kv_heads + head) * kRows + r;
+            *reinterpret_cast<float4*>(d.part_o + row * D + e) = v;
+            if (e == 0) d.part_ml[row] = make_float2(top, sum);
+          }
         }
       }
-      turn ^= 1;
+      meet();  // all have read s_ml: the next sequence's come there
       if (!(info.flags & kWhole)) {  // whoever comes last adds the parts up, in the ranges' order
-        asm volatile("bar.sync 1, 128;" ::: "memory");
         if (threadIdx.x == 0)
           s_last = alive && last_to_arrive(a.counters + info.first_range * a.kv_heads + head, info.parts);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (s_last) join_parts<T, D>(d, info, head, rows);
+        meet();
+        if (s_last) join_parts<T, D, G>(d, info, head, rows);
       }
       proxy_fence_smem();  // these accesses come before the copies of the next tile here
     }
@@ -497,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 2) decode_kernel(const __grid_consta
 __global__ void __launch_bounds__(128) decode_weights_kernel(DecodeArgs d) {
   const AttnArgs& a = d.a;
   const uint32_t s = blockIdx.z, head = blockIdx.y, q_first = a.q_offsets[s], queries = a.q_offsets[s + 1] - q_first;
-  __shared__ float s_lse[kRows];
+  __shared__ float s_lse[kDecodeRows];
   const uint32_t rows = min(queries * a.group, d.score_rows);
   const SeqInfo q = seq_info(a, s, 0);
   if (rows == 0 || static_cast<int>(blockIdx.x * 512) >= q.len) {
@@ -531,28 +543,34 @@ __global__ void __launch_bounds__(128) decode_weights_kernel(DecodeArgs d) {
   }
 }
 
-// Two CTAs fit an SM. Each range and head needs a counter where there are ranges to
-// join; the other half of the counters is the tile kernel's, which may still run.
+uint32_t part_rows(const tcx_kv_attention_args& x) {
+  return x.max_q * (x.q_heads / x.kv_heads) <= kWarpRows ? kWarpRows : 2 * kWarpRows;
+}
+
+// Two CTAs fit an SM (one with 32 rows). Each range and head needs a counter where
+// there are ranges to join; the other half of the counters is the tile kernel's, which
+// may still run.
 uint32_t decode_ranges(const tcx_kv_attention_args& x) {
   const uint64_t tiles = x.total_pages * x.page_tokens / kTile + x.n_seq;
-  const uint64_t most = std::min<uint64_t>(2ull * sm_count(), TCX_KV_COUNTERS / 2) / x.kv_heads;
+  const uint64_t most = std::min<uint64_t>((part_rows(x) == kWarpRows ? 2ull : 1ull) * sm_count(), TCX_KV_COUNTERS / 2) / x.kv_heads;
   return static_cast<uint32_t>(std::max<uint64_t>(1, std::min<uint64_t>(tiles, most)));
 }
 
-template <typename T, int D, bool kScores>
+template <typename T, int D, bool kScores, int G>
 tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint64_t max_tokens, cudaStream_t stream) {
-  using L = Layout<D>;
+  using L = Layout<D, G>;
+  constexpr int kThreads = 32 * (kWarps * G + 1);
   static std::atomic<uint64_t> allowed{0};
-  if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(decode_kernel<T, D, kScores>), L::kBytes, &allowed);
+  if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(decode_kernel<T, D, kScores, G>), L::kBytes, &allowed);
       st != TCX_OK)
     return st;
   const dim3 grid(d.ranges * d.a.kv_heads);
   if (d.a.prior_o != nullptr) {  // behind the shared prefix's kernels
-    if (const tcx_status st = launch_after(decode_kernel<T, D, kScores>, grid, dim3(kThreads), L::kBytes, stream, map, d);
+    if (const tcx_status st = launch_after(decode_kernel<T, D, kScores, G>, grid, dim3(kThreads), L::kBytes, stream, map, d);
         st != TCX_OK)
       return st;
   } else {
-    decode_kernel<T, D, kScores><<<grid, kThreads, L::kBytes, stream>>>(map, d);
+    decode_kernel<T, D, kScores, G><<<grid, kThreads, L::kBytes, stream>>>(map, d);
     note_launches(1);
     TCX_CUDA_TRY(cudaGetLastError());
   }
@@ -564,8 +582,11 @@ tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint64_t max_toke
 
 template <typename T, int D>
 tcx_status launch(const DecodeArgs& d, const CUtensorMap& map, uint64_t max_tokens, cudaStream_t stream) {
-  return d.scores != nullptr ? launch<T, D, true>(d, map, max_tokens, stream)
-                             : launch<T, D, false>(d, map, max_tokens, stream);
+  if (d.part_rows == kWarpRows)
+    return d.scores != nullptr ? launch<T, D, true, 1>(d, map, max_tokens, stream)
+                               : launch<T, D, false, 1>(d, map, max_tokens, stream);
+  return d.scores != nullptr ? launch<T, D, true, 2>(d, map, max_tokens, stream)
+                             : launch<T, D, false, 2>(d, map, max_tokens, stream);
 }
 
 uint64_t score_bytes(const tcx_kv_attention_args& x) {
@@ -575,12 +596,15 @@ uint64_t score_bytes(const tcx_kv_attention_args& x) {
 
 }  // namespace
 
+// Up to 16 rows fill one tile of the products, up to 32 two, in warps of their own and one
+// CTA on an SM; from there on the tile kernel. At 20 rows of one 500-token sequence the
+// two take 18.6 and 23.6 us, at 32 rows of 96 sequences of 64-4096 tokens 165 and 156.
 bool decode_fits(const tcx_kv_attention_args& x) {
   return x.max_q * (x.q_heads / x.kv_heads) <= kDecodeRows;
 }
 
 uint64_t decode_scratch_bytes(const tcx_kv_attention_args& x) {
-  const uint64_t parts = decode_ranges(x) * 2ull * x.kv_heads * kRows;
+  const uint64_t parts = decode_ranges(x) * 2ull * x.kv_heads * part_rows(x);
   return align256(parts * sizeof(float2)) +
          align256(parts * x.head_dim * 4) + score_bytes(x);
 }
@@ -591,7 +615,8 @@ tcx_status launch_decode(const tcx_kv_attention_args& x, const AttnArgs& a, cons
   d.a = a;
   d.ranges = decode_ranges(x);
   d.rows = static_cast<uint32_t>(x.max_q) * a.group;
-  const uint64_t parts = d.ranges * 2ull * x.kv_heads * kRows;
+  d.part_rows = part_rows(x);
+  const uint64_t parts = d.ranges * 2ull * x.kv_heads * part_rows(x);
   uint8_t* at = static_cast<uint8_t*>(scratch);
   d.part_ml = reinterpret_cast<float2*>(at);
   d.part_o = reinterpret_cast<float*>(at += align256(parts * sizeof(float2)));

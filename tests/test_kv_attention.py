@@ -201,6 +201,22 @@ def test_decode_window_and_sinks(cuda_device, window, sinks, dim):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("group,count", [(16, 1), (17, 1), (5, 4), (8, 4), (31, 1), (32, 1), (11, 3)])
+def test_decode_around_the_rows_of_a_tile(cuda_device, dim, group, count):
+    """Up to and beyond 16 and 32 rows, several short sequences to a range of work, parts to join, weights."""
+    tokens = [1, 70, 0, 300, 5, 64, 129, 2000, 33, 12]
+    att, pool, q, _, ref = run(tokens, [count] * len(tokens), kv_heads=2, group=group, dim=dim)
+    run(tokens, [count] * len(tokens), kv_heads=1, group=group, dim=dim, window=90, sinks=7, dtype=FP16)
+    weights = torch.zeros((2, att.weight_columns), device="cuda")
+    att.run(pool, 0, q, weights=weights)
+    relative = float(kvtools.bounds(ref, BF16, 2000)[2].max()) + 32 * 2.0 ** -24
+    for s, n in enumerate(tokens):
+        c = int(att.w.page_offsets[s]) * 16
+        assert ((weights[:, c:c + n].double() - ref[2][s]).abs() <= relative * ref[2][s] + 2.0 ** -126).all(), s
+
+
+@pytest.mark.gpu
 def test_decode_one_long_sequence(cuda_device):
     run([20011], [1], kv_heads=1)
     run([20011, 3], [1, 1], kv_heads=1, window=9000, sinks=5, dtype=FP16)
