@@ -2,10 +2,11 @@
 // attention weight of every (sequence, layer, kv head) stay, and their rows are
 // copied in their old order to the sequence's destination pages.
 //
-// One launch, one CTA per (layer, kv head, sequence), or some where those are few: it finds the budget's weight by
-// radix selection over the weights' order-preserving integer images (11, 11 and 10 bits
-// at a time, the images kept in shared memory), writes its share of the kept indices
-// and moves those rows of its head in both planes, so that one list's selection runs beside others' copies.
+// One launch, one CTA per (layer, kv head, sequence), or some where those are few: it
+// finds the budget's weight by radix selection over the weights' order-preserving
+// integer images (11, 11 and 10 bits at a time, the images kept in shared memory),
+// writes its share of the kept indices and moves those rows of its head in both planes,
+// so that one list's selection runs beside others' copies.
 // Bound by HBM: each kept row is read and written once; the places of 512 rows are
 // looked up first, so that a thread has eight 16-byte loads under way. The destination
 // pages are not the source's: a page may be shared with other sequences, and the copy
