@@ -3,14 +3,16 @@
 //
 // A CTA holds a tile of 128 keys and takes all rows that see one of them through it,
 // 128 at a time: scores with the keys as the product's rows, so that a thread owns
-// one key and adds up its row of 128 scores without exchanging anything, in the
-// rows' order. The scores are recomputed from the keys: beside a prompt's products
-// that is a third more, where keeping them would take rows x tokens x 4 bytes.
-// Bound by the exponential units (one for each score; the product is half as long);
-// two CTAs share an SM, so that one's fetches run beside the other's exponentials.
+// one key and half of the rows, adds up its 64 scores without exchanging anything, in
+// the rows' order, and the key's two halves meet once at the end. The scores are
+// recomputed from the keys: beside a prompt's products that is a third more, where
+// keeping them would take rows x tokens x 4 bytes. Two CTAs share an SM, so that one's
+// fetches run beside the other's exponentials. The exponential units bound it, at 0.45
+// of their rate while an SM has work (a fourth of the exponentials as polynomials
+// changed less than 1 %); over the whole call 0.34, because 657 CTAs are 2.2 rounds.
 // Measured on B200: 256 queries at the ends of two sequences of 5000-6100 tokens, 32 / 8
-// heads of 128, 69 us beside 80 us for their attention (90 million exponentials: 20 us
-// of the exponential units).
+// heads of 128, 65 us beside 75 us for their attention (69 us with one thread for all
+// 128 rows of a key).
 #include <algorithm>
 #include <type_traits>
 
@@ -21,7 +23,8 @@ namespace {
 
 constexpr int kKeys = 128;
 constexpr int kRows = 128;
-constexpr int kWorkers = 128;
+constexpr int kWorkers = 2 * kKeys;  // a thread for each key and half of the rows
+constexpr int kWarpRows = kRows * 32 / kWorkers;  // that a warp fetches
 constexpr int kThreads = kWorkers + 32;
 
 template <int D>
@@ -39,6 +42,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
   // and the keys that it sees, up to hi and from lo on (and the sinks).
   __shared__ __align__(16) float s_lse[4][kRows];
   __shared__ int2 s_sees[4][kRows];
+  __shared__ float s_other[kKeys];
   __shared__ uint64_t s_bar[7];
   __shared__ uint32_t s_tmem, s_gave_up, s_drained;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y, s = blockIdx.z;
@@ -123,23 +127,24 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
       __syncwarp();
     }
     if (!alive) mbar_wait_warp(keys_there, 0, &s_drained, a.status);  // no copy may be in flight at the end
-  } else {  // ---- one key for each thread; the queries' copies
+  } else {  // ---- one key and half of a tile's rows for each thread; the queries' copies
     bool alive = true;
-    const int key = key0 + static_cast<int>(threadIdx.x);
-    // Starts the copies of a tile's queries (this warp: 32 of them, D / 8 lanes to a
+    const uint32_t part = threadIdx.x / kKeys, mine = warp * kWarpRows + lane % kWarpRows;  // the row that it looks up
+    const int key = key0 + static_cast<int>(threadIdx.x % kKeys);
+    // Starts the copies of a tile's queries (this warp: 16 of them, D / 8 lanes to a
     // row, swizzled) and notes what its rows see.
     float of_row;
     int2 sees;
     auto fetch = [&](uint32_t i) {
       if (i < n) {
         constexpr uint32_t kLanes = D / 8;
-        const uint32_t row = (tile0 + i) * kRows + threadIdx.x, t = q_first + row / a.group,
+        const uint32_t row = (tile0 + i) * kRows + mine, t = q_first + row / a.group,
                        h = head * a.group + row % a.group;
         const uint64_t at = t * a.q_token_stride + h * a.q_head_stride;
-        const uint32_t first = (tile0 + i) * kRows + warp * 32;
+        const uint32_t first = (tile0 + i) * kRows + warp * kWarpRows;
 #pragma unroll
-        for (uint32_t k = 0; k < kLanes; ++k) {
-          const uint32_t src = k * (32 / kLanes) + lane / kLanes, c = lane % kLanes, of = warp * 32 + src;
+        for (uint32_t k = 0; k < kWarpRows * kLanes / 32; ++k) {
+          const uint32_t src = k * (32 / kLanes) + lane / kLanes, c = lane % kLanes, of = warp * kWarpRows + src;
           const bool valid = first + src < rows;
           const uint64_t from = __shfl_sync(~0u, at, src);
           async_copy16(base + (1 + i % 2) * L::kOperand + c / 8 * L::kBlock + of * 128 + ((c % 8 ^ (of & 7)) << 4),
@@ -156,9 +161,9 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
     auto note = [&](uint32_t i) {  // what fetch found, once it is there
-      if (i >= n) return;
-      s_lse[i % 4][threadIdx.x] = of_row == -INFINITY ? INFINITY : of_row * kLog2e;
-      s_sees[i % 4][threadIdx.x] = sees;
+      if (i >= n || lane >= kWarpRows) return;
+      s_lse[i % 4][mine] = of_row == -INFINITY ? INFINITY : of_row * kLog2e;
+      s_sees[i % 4][mine] = sees;
     };
     auto ready = [&](uint32_t i) {  // tile i's copies of this warp are there
       if (i >= n) return;
@@ -176,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
     for (uint32_t i = 0; i < n; ++i) {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       ready(i + 1);
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // the rows' notes are there, and those of tile i - 2 are read
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the rows' notes are there, and those of tile i - 2 are read
       alive = alive && mbar_wait_warp(scored(i), i / 2 & 1, &s_gave_up, a.status);
       tmem_fence_after();
       fetch(i + 2);  // in place of tile i, which the product has read
@@ -187,15 +192,16 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
       const float2 c2 = make_float2(a.scale_log2, a.scale_log2);
       auto add_up = [&](auto some_hidden) {
 #pragma unroll
-        for (int c = 0; c < kRows; c += 64) {
-          uint32_t z[64];
-          tmem_load64(z, tmem + (warp * 32 << 16) + i % 2 * kRows + c);
-          if (c != 0) {
+        for (int half = 0; half < 2; ++half) {
+          const int c = static_cast<int>(part) * (kRows / 2) + half * (kRows / 4);
+          uint32_t z[kRows / 4];
+          tmem_load32(z, tmem + (warp % 4 * 32 << 16) + i % 2 * kRows + c);
+          if (half == 1) {
             tmem_fence_before();
             mbar_arrive_warp(taken(i), lane, alive);
           }
 #pragma unroll
-          for (int k = 0; k < 64; k += 4) {
+          for (int k = 0; k < kRows / 4; k += 4) {
             const float4 x = lse[(c + k) / 4];
             float2 p = fma2(make_float2(__uint_as_float(z[k]), __uint_as_float(z[k + 1])), c2, make_float2(-x.x, -x.y));
             float2 q = fma2(make_float2(__uint_as_float(z[k + 2]), __uint_as_float(z[k + 3])), c2,
@@ -219,9 +225,11 @@ __global__ void __launch_bounds__(kThreads, 2) weights_kernel(const __grid_const
       note(i + 2);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (key < len && alive)
-      a.weights[head * a.weights_head_stride + a.page_offsets[s] * a.page_tokens + key] +=
-          (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+    const float total = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+    if (part == 1) s_other[threadIdx.x % kKeys] = total;
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (part == 0 && key < len && *static_cast<volatile uint32_t*>(&s_gave_up) == 0)
+      a.weights[head * a.weights_head_stride + a.page_offsets[s] * a.page_tokens + key] += total + s_other[threadIdx.x];
   }
   tmem_fence_before();
   __syncthreads();
