@@ -287,7 +287,8 @@ class KvEvict(_OnDevice):
     the newest ``recent`` and, of the rest, the heaviest (equal weights by lower index, NaN lowest).
 
     ``dst`` holds the pages that the kept rows are copied to, in their old order, and the budgets as
-    its ``seq_tokens``; its pages must be distinct and none of ``w``'s. The source pages are only
+    its ``seq_tokens``; its pages must be distinct and none of ``w``'s. A budget must hold ``sinks +
+    recent`` tokens, or the whole sequence where that is shorter. The source pages are only
     read: other sequences may share them. Rows are copied whole, so the element type does not matter.
     """
 
@@ -304,8 +305,10 @@ class KvEvict(_OnDevice):
             _refuse("sinks and recent must not be negative")
         _check_tables(w, "sequences")
         _check_tables(dst, "destination")
-        if (np.asarray(dst.seq_tokens).astype(np.int64) < sinks + recent).any():
-            _refuse(f"a budget is below sinks + recent ({sinks + recent})")
+        # a sequence that its budget holds whole keeps everything
+        stays = np.minimum(np.asarray(w.seq_tokens).astype(np.int64), min(sinks + recent, 1 << 32))
+        if (np.asarray(dst.seq_tokens).astype(np.int64) < stays).any():
+            _refuse(f"a budget is below sinks + recent ({sinks + recent}) and below its sequence")
         to = np.asarray(dst.page_table)
         if np.unique(to).size != to.size:
             _refuse("a destination page is listed twice")

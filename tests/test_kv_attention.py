@@ -59,7 +59,7 @@ def test_evict_refuses_what_it_cannot_run():
     make = lambda dst, k=2, **kw: (lambda: KvEvict(w, dst, k, **kw))  # noqa: E731
     refused("listed twice", make(page(free[0], free[1], free[0])))
     refused("is a source page", make(page(free[0], free[1], w.page_table[2])))
-    refused("below sinks", make(good, sinks=3, recent=3))
+    refused("below sinks", make(good, sinks=3, recent=18))   # 21 of 40 tokens; 5 of 5 would stay
     refused("negative", make(good, sinks=-1))
     refused("same pool", make(kvtools.tables([5], taken=4)[0]))
     refused("multiple of 16", make(good, k=7))
@@ -681,6 +681,15 @@ def test_evict_ties_and_special_weights(cuda_device):
 def test_evict_zero_budget_and_everything_kept(cuda_device):
     evict_case([40, 50, 0], [0, 50, 0])
     evict_case([40, 50], [25, 25], sinks=20, recent=5)   # nothing is left to rank
+
+
+@pytest.mark.gpu
+def test_evict_sequences_shorter_than_what_always_stays(cuda_device):
+    """A budget of the whole sequence holds it, also below sinks + recent; the same budget behind it does not."""
+    evict_case([2, 5, 0, 43, 44, 700], [2, 5, 0, 43, 43, 100], sinks=7, recent=36)
+    evict_case([2, 5, 700], [2, 60, 100], layers=1, sinks=7, recent=36)
+    with pytest.raises(Exception, match="below sinks"):
+        evict_case([2, 44], [2, 42], sinks=7, recent=36)
 
 
 @pytest.mark.gpu
