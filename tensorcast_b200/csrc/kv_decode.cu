@@ -24,6 +24,7 @@
 // loads' and the last joins' latencies); one sequence of 777 tokens 12 us.
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "kv_attention.cuh"
 
@@ -305,7 +306,8 @@ __global__ void __launch_bounds__(32 * (kWarps * G + 1), G == 1 ? 2 : 1)
   const uint32_t part = warp % kWarps, row0 = warp / kWarps * kWarpRows;
   auto meet = [&] { asm volatile("bar.sync 1, %0;" ::"n"(128 * G) : "memory"); };
   uint32_t qf[D / 16][4];
-  float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  constexpr bool kIsHalf = std::is_same<T, __half>::value;
+  float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, peak[2] = {-INFINITY, -INFINITY};
   bool alive = true;
   for (uint32_t i = 0; i < count; ++i) {
     const uint32_t stage = i % L::kStages, at = base + stage * L::kStage;
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(32 * (kWarps * G + 1), G == 1 ? 2 : 1)
       for (int n = 0; n < D / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
-      m[0] = m[1] = -INFINITY;
+      m[0] = m[1] = peak[0] = peak[1] = -INFINITY;
       l[0] = l[1] = 0.f;
     }
     // All of the warp's keys are loaded before the first product, and its values before
@@ -404,7 +406,12 @@ __global__ void __launch_bounds__(32 * (kWarps * G + 1), G == 1 ? 2 : 1)
       float top = fmaxf(fmaxf(z[0][2 * r], z[0][2 * r + 1]), fmaxf(z[1][2 * r], z[1][2 * r + 1]));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
       top = fmaxf(top, __shfl_xor_sync(~0u, top, 2)) * a.scale_log2;
-      top = fmaxf(top, m[r]);
+      if constexpr (kIsHalf) {
+        top = half_reference(m[r], top, peak[r], true);
+        peak[r] = fmaxf(peak[r], top);
+      } else {
+        top = fmaxf(top, m[r]);
+      }
       const float ref = top == -INFINITY ? 0.f : top;
       scale[r] = exp2_approx(m[r] - ref);
       m[r] = top;

@@ -10,8 +10,9 @@
 // memory. The probabilities are rounded to the input type (half a step, as the output
 // is) and take the place of the first 64 tokens' scores; the other 64 tokens' place is
 // free as soon as its scores are read, so the next tile's are computed there while this
-// one's first 64 are weighed. A row's sums are scaled to a new maximum only where it
-// has grown by more than 2^8, which the 32-bit sums carry exactly as well.
+// one's first 64 are weighed. A row's sums are scaled to a new reference only where its
+// maximum has grown by more than 2^8 (fp16: where a tile's leaves what the type holds),
+// which the 32-bit sums carry exactly as well.
 //
 // Roles: warps 0-3 and 4-7 the halves' softmax, warps 8 and 10 issue the halves'
 // products, warp 9 loads keys and values with TMA into a ring (a box for each run of
@@ -573,7 +574,9 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         any_hi = it.limit - 1;
         any_lo = it.low;
       }
-      float m = -INFINITY, l = 0.f;
+      constexpr bool kIsHalf = std::is_same<T, __half>::value;
+      constexpr float kTop = kIsHalf ? kHalfTop : 8.f;  // the largest exponent before m rises
+      float m = -INFINITY, l = 0.f, peak = -INFINITY;
       if (active) {
         for (uint32_t j = 0; j < n; ++j, ++done) {
           const int token = first_token(it, at + j);
@@ -610,9 +613,15 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           };
           auto reference = [&] { return m == -INFINITY ? 0.f : m; };
           float f = 1.f;  // what the sums so far are scaled by
-          auto grow = [&](float top) {
-            const float old = m, by = top > m + 8.f ? exp2_approx(old - top) : 1.f;
-            if (top > m + 8.f) m = top;
+          auto move = [&](float top, bool down) {
+            const float old = m;
+            if constexpr (kIsHalf) {
+              m = half_reference(old, top, peak, down);
+              peak = fmaxf(peak, m);
+            } else if (top > m + kTop) {
+              m = top;
+            }
+            const float by = m == old ? 1.f : exp2_approx(old - m);
             f *= by;
             return by;
           };
@@ -629,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             mbar_arrive_warp(bar(kHighRead, h), lane, alive);
             if (masked) hide(z, token + kTokens / 2);
             const float top = largest(z);
-            grow(top);
+            move(top, true);
             odd = masked || __any_sync(~0u, !(fabsf(top) < INFINITY));
             const float ref = reference();
             auto all = [&](auto mixed) {
@@ -705,12 +714,12 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             if (!odd) {
               all(std::true_type{});
               top = largest(z);
-              again = __any_sync(~0u, !(top <= m + 8.f));
+              again = __any_sync(~0u, !(top <= m + kTop));
             } else {
               top = largest(z);
             }
             if (again) {
-              const float by = grow(top);
+              const float by = move(top, false);
               if (__any_sync(~0u, by != 1.f)) {
 #pragma unroll
                 for (int i = 0; i < kTokens / 4; ++i) e[i] = make_float2(e[i].x * by, e[i].y * by);

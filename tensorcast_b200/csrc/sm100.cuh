@@ -282,7 +282,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// 2^x for finite x <= 8, two at once, without the exponential unit: x = n + r with
+// 2^x for finite x <= 15, two at once, without the exponential unit: x = n + r with
 // n the nearest whole number, 2^r by the polynomial of degree 5 with the smallest
 // relative error on [-1/2, 1/2] (7.5e-8, found by Remez exchange; 2.2e-7 evaluated
 // in 32 bits), n added to the exponent. Below -126 the result is that of -126.

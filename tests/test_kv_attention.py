@@ -562,6 +562,86 @@ print("done")
     assert r.returncode == 0 and "done" in r.stdout, r.stderr[-2000:]
 
 
+# ---------------------------------------------------------------- the range of the probabilities (GPU)
+
+def steered(scores, values, count, group, dim=64, seed=0):
+    """A sequence of len(scores) fp16 tokens of one kv head whose scaled scores are about `scores` for every row
+    (plus normal ones of size 0.1), its values, and its `count` queries."""
+    n = len(scores)
+    w, _ = kvtools.tables([n], kv_heads=1, dim=dim)
+    pool = kvtools.make_pool(w, 1, dim, FP16)
+    rows = torch.from_numpy(kvtools.token_rows(w, 0))
+    g = torch.Generator().manual_seed(seed)
+    k = torch.randn((n, dim), generator=g) * 0.1
+    k[:, 0] = scores.float() * dim ** 0.5 / 4
+    q = torch.randn((count, group, dim), generator=g)
+    q[:, :, 0] = 4
+    pool[0, rows, 0], pool[1, rows, 0] = k.half(), values.half()
+    return w, pool.cuda(), q.half().cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 40])
+@pytest.mark.parametrize("gap", [17.0, 19.0, 25.0])
+@pytest.mark.parametrize("sink", [0.0, 2.0 ** -9, 1.0])
+def test_fp16_tokens_far_below_a_strong_first_one_count(cuda_device, count, gap, sink):
+    """A first token that takes nearly all of the softmax, and whose value may be small or 0: the 40000 others
+    make up much of the output, though each weighs 2^-25 to 2^-36 of it."""
+    g = torch.Generator().manual_seed(1)
+    scores = torch.zeros(40000)
+    scores[0] = gap
+    values = torch.randn((40000, 64), generator=g).abs() * 8
+    values[0] *= sink
+    w, pool, q = steered(scores, values, count, 4)
+    got = KvAttention(w, 4, 1, FP16, query_tokens=[count]).run(pool, 0, q)
+    check(got, kvtools.attention(w, pool, 0, q, [count]), FP16, 40000)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 40])
+@pytest.mark.parametrize("order", ["up", "down", "zigzag", "steps", "mixed"])
+def test_fp16_scores_that_rise_and_fall_along_the_row(cuda_device, count, order):
+    """Scores over a range of 2^26 in weight, with values that make every token count alike. A probability below
+    2^-14 is off by 2^-25 where the largest of its 128 tokens has 2^-1 at least: by 2^-24 of that one's weight."""
+    n = 3000
+    at = torch.arange(n, dtype=torch.float64)
+    z = {"up": at / n * 18, "down": 18 - at / n * 18, "zigzag": (at % 500 - 250).abs() / 250 * 18,
+         "steps": (at // 128 % 2) * 18, "mixed": torch.rand(n, generator=torch.Generator().manual_seed(2)) * 18}[order]
+    values = (torch.rand((n, 64), generator=torch.Generator().manual_seed(3)) + 0.5) * torch.exp(9 - z)[:, None]
+    w, pool, q = steered(z - 9, values, count, 4)
+    out, lse = KvAttention(w, 4, 1, FP16, query_tokens=[count]).run(pool, 0, q)
+    ref = kvtools.attention(w, pool, 0, q, [count])
+    tol, tol_lse, _ = kvtools.bounds(ref, FP16, n)
+    rows = torch.from_numpy(kvtools.token_rows(w, 0)).cuda()
+    k, v = pool[0, rows, 0].double(), pool[1, rows, 0].double()
+    p = torch.exp((q.double() @ k.t()) / 8 - ref[1][..., None])
+    see = torch.arange(n, device="cuda") <= n - count + torch.arange(count, device="cuda")[:, None]
+    p = torch.nn.functional.pad(p * see[:, None], (0, -n % 128)).unflatten(-1, (-1, 128))
+    size = torch.nn.functional.pad(v.abs(), (0, 0, 0, -n % 128)).unflatten(0, (-1, 128)).sum(1)
+    tol = tol + 2.0 ** -24 * p.amax(-1) @ size
+    assert ((out.double() - ref[0]).abs() <= tol).all(), float(((out.double() - ref[0]).abs() / tol).max())
+    assert ((lse.double() - ref[1]).abs() <= tol_lse).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [17.0, 19.0, 25.0])
+def test_fp16_tail_of_a_decode_batch(cuda_device, gap):
+    """The same for one query token, in sequences that share their pages: a warp goes through many tiles of each."""
+    n, batch = 20000, 60
+    values = torch.randn((n, 64), generator=torch.Generator().manual_seed(1)).abs() * 8
+    values[0] = 0
+    scores = torch.zeros(n)
+    scores[0] = gap
+    one, pool, q = steered(scores, values, 1, 4)
+    pages = len(one.page_table)
+    w = KvWorkload(2, one.pool_pages, 16, one.token_bytes, np.full(batch, n, np.uint32),
+                   (np.arange(batch + 1) * pages).astype(np.uint64), np.tile(one.page_table, batch))
+    out, lse = KvAttention(w, 4, 1, FP16).run(pool, 0, q.expand(batch, 4, 64))
+    ref = kvtools.attention(one, pool, 0, q, [1])
+    for s in range(batch):
+        check((out[s:s + 1], lse[s:s + 1]), ref, FP16, n)
+
+
 # ---------------------------------------------------------------- accumulated weights (GPU)
 
 @pytest.mark.gpu
