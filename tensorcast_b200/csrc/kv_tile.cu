@@ -234,6 +234,15 @@ __device__ __forceinline__ int first_token(const Item& it, uint32_t tile) {
                                                      : it.first_tile + static_cast<int>(tile) - it.sink_tiles) * kTokens;
 }
 
+// The finite ones of two 16-bit values; 0 in place of the others.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_only(uint32_t pair) {
+  constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c00 : 0x7f80;
+  if ((pair & kExponent) == kExponent) pair &= 0xffff0000u;
+  if ((pair >> 16 & kExponent) == kExponent) pair &= 0xffffu;
+  return pair;
+}
+
 // The rows of an item and head that the ranges [from, to] hold parts of, one warp of
 // eight to a row, the parts in the ranges' order.
 template <typename T, int D>
@@ -278,13 +287,14 @@ __device__ __forceinline__ void join_rows(const TileArgs& d, const Item& it, uin
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kPrefix>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map, TileArgs d) {
   using L = TileLayout<D>;
   constexpr uint32_t kStages = L::kStages;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t s_bar[2 * kStages + 12];
   __shared__ uint32_t s_tmem, s_gave_up, s_drained, s_last;
+  __shared__ uint32_t s_left_out[2];  // piece + 1 where values were kept from its products
   __shared__ __align__(16) int s_seen[2][8][4];
   const AttnArgs& a = d.a;
   const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, range = blockIdx.x;
@@ -311,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       mbar_init(bar(kWeighed, h), 4);
       mbar_init(bar(kSummed, h), 1);
     }
-    s_gave_up = s_drained = 0;
+    s_gave_up = s_drained = s_left_out[0] = s_left_out[1] = 0;
     mbar_init_fence();
   }
   next_may_start();
@@ -320,7 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
   const int prefix = static_cast<int>(prefix_length(a));
   uint32_t items, ranges;
   uint64_t same_tiles = 0, cost = 0;  // over a prefix: every row tile's token tiles
-  if (d.prefix) {
+  if (kPrefix) {
     items = static_cast<uint32_t>((static_cast<uint64_t>(a.q_tokens) * a.group + kRows - 1) / kRows);
     same_tiles = make_item(d, 0, 0, prefix).tiles;
     const uint64_t pieces = static_cast<uint64_t>(items) * a.kv_heads;
@@ -335,14 +345,14 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
     return;
   }
   auto begin_of = [&](uint32_t r) {
-    if (!d.prefix) return d.begin[r];
+    if (!kPrefix) return d.begin[r];
     const uint64_t pieces = static_cast<uint64_t>(items) * a.kv_heads, each = same_tiles + cost;
     const uint64_t at = scaled(pieces * each, r, ranges), piece = scaled(at, 1, each);
     const uint64_t tile = max(at - piece * each, cost) - cost, first = scaled(piece, 1, a.kv_heads);
     return RangeBegin{static_cast<uint32_t>(first), static_cast<uint32_t>(piece - first * a.kv_heads),
                       static_cast<uint32_t>(tile), piece * same_tiles + tile};
   };
-  auto item_of = [&](uint32_t i) { return d.prefix ? make_item(d, 0, i, prefix) : d.items[i]; };
+  auto item_of = [&](uint32_t i) { return kPrefix ? make_item(d, 0, i, prefix) : d.items[i]; };
   if (warp == 8) tmem_alloc(smem_addr(&s_tmem), L::kColumns);
   tmem_fence_before();
   __syncthreads();
@@ -364,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       bool alive = true;
       for (uint32_t left = count; left > 0 && alive;) {
         const uint32_t n = min(it.tiles - at, left);
-        const uint32_t* table = (d.prefix ? a.prefix_table : a.page_table) + it.table;
+        const uint32_t* table = (kPrefix ? a.prefix_table : a.page_table) + it.table;
         for (uint32_t j = 0; j < n && alive; ++j) {
           const int from = first_token(it, at + j) + static_cast<int>(box * a.box_rows),
                     to = from + static_cast<int>(a.box_rows);
@@ -531,17 +541,18 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
       };
       if (!active) fetch_next();
       // What this row sees: [0, hi] from lo on, and the sinks. What all rows of this
-      // half see (all_*), and what any row of the item sees (any_*).
-      int hi = -1, lo = 0, all_hi, all_lo, any_hi, any_lo;
+      // half see (all_*), and what any row of the item sees (any_*). Over a prefix, where
+      // the rows are those of several sequences: what all rows of the item see (every_*).
+      int hi = -1, lo = 0, all_hi, all_lo, any_hi, any_lo, every_hi, every_lo;
       auto low_of = [&](int pos) {
         return a.window ? static_cast<int>(max(int64_t{0}, pos - a.window + 1)) : 0;
       };
-      if (d.prefix && d.max_q == 1 && a.window == 0) {
+      if (kPrefix && d.max_q == 1 && a.window == 0) {
         // one query each stands behind the whole prefix, and sees it
         hi = r < it.rows ? prefix - 1 : -1;
-        all_hi = any_hi = prefix - 1;
-        all_lo = any_lo = 0;
-      } else if (d.prefix) {
+        all_hi = any_hi = every_hi = prefix - 1;
+        all_lo = any_lo = every_lo = 0;
+      } else if (kPrefix) {
         if (r < it.rows) {
           const uint32_t t = it.q_first + row / a.group, s = seq_of(a, t);
           const int nq = static_cast<int>(a.q_offsets[s + 1] - a.q_offsets[s]);
@@ -556,9 +567,13 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         any_lo = __reduce_min_sync(~0u, valid ? lo : 0x7fffffff);
         if (lane == 0) *reinterpret_cast<int4*>(s_seen[pieces & 1][warp]) = make_int4(all_hi, all_lo, any_hi, any_lo);
         asm volatile("bar.sync 1, 256;" ::: "memory");
+        every_hi = 0x7fffffff;
+        every_lo = 0;
 #pragma unroll
         for (int w = 0; w < 8; ++w) {
           const int* v = s_seen[pieces & 1][w];
+          every_hi = min(every_hi, v[0]);
+          every_lo = max(every_lo, v[1]);
           if (static_cast<uint32_t>(w) / 4 == h) {
             all_hi = min(all_hi, v[0]);
             all_lo = max(all_lo, v[1]);
@@ -571,9 +586,13 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         lo = low_of(hi);
         all_hi = it.pos0 + static_cast<int>((it.row0 + h * kHalfRows) / a.group);
         all_lo = low_of(it.pos0 + static_cast<int>((it.row0 + it.rows - 1) / a.group));
-        any_hi = it.limit - 1;
-        any_lo = it.low;
+        any_hi = every_hi = it.limit - 1;
+        any_lo = every_lo = it.low;
       }
+      // Does the tile hold tokens that not every row sees (every: of the item)?
+      auto partly_seen = [&](int token) {
+        return token + kTokens - 1 > every_hi || (token < every_lo && token + kTokens > it.sinks);
+      };
       constexpr bool kIsHalf = std::is_same<T, __half>::value;
       constexpr float kTop = kIsHalf ? kHalfTop : 8.f;  // the largest exponent before m rises
       float m = -INFINITY, l = 0.f, peak = -INFINITY;
@@ -667,28 +686,45 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             if (j + 1 == n) fetch_next();
             uint32_t z[kTokens / 2];
             tmem_load64(z, scores);
-            if (masked) {
-              hide(z, token);
-              // Values that no row sees are cleared (0 x NaN is not 0), half of them by
-              // each half of the rows; both come here, and neither goes on alone.
-              if (token + kTokens - 1 > any_hi || (token < any_lo && token + kTokens > it.sinks)) {
-                const uint32_t v = 2 * (tiles_done + j) + 1, of = r % kHalfRows, halves = it.rows > kHalfRows ? 2 : 1;
-                wait(full((v + 1) / 2), full_phase((v + 1) / 2));
-                const int mine = token + static_cast<int>(of);
-                if (mine > any_hi || (mine < any_lo && mine >= it.sinks)) {
-                  const uint32_t to = ring + v % kStages * L::kOperand + of * 128;
-                  for (uint32_t c = h; c < D / 8; c += halves)
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(to + c / 8 * L::kBlock +
-                                                                                 ((c % 8 ^ (of & 7)) << 4)),
-                                 "r"(0)
-                                 : "memory");
+            if (masked) hide(z, token);
+            // Values that no row sees are cleared (0 x NaN is not 0), half of them by each
+            // half of the rows; both come here, and neither goes on alone. One that some
+            // sequences' rows see must not reach the others': where it is not finite it is
+            // kept from the product, and added to its rows' sums behind the last one.
+            if ((kPrefix || masked) && partly_seen(token)) {
+              const uint32_t v = 2 * (tiles_done + j) + 1, of = r % kHalfRows, halves = it.rows > kHalfRows ? 2 : 1;
+              wait(full((v + 1) / 2), full_phase((v + 1) / 2));
+              const int mine = token + static_cast<int>(of);
+              const uint32_t to = ring + v % kStages * L::kOperand + of * 128;
+              auto place_of = [&](uint32_t c) { return to + c / 8 * L::kBlock + ((c % 8 ^ (of & 7)) << 4); };
+              auto put = [](uint32_t at, const uint32_t (&x)[4]) {
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3])
+                             : "memory");
+              };
+              if (mine > any_hi || (mine < any_lo && mine >= it.sinks)) {
+                for (uint32_t c = h; c < D / 8; c += halves) put(place_of(c), {0, 0, 0, 0});
+              } else if (kPrefix && (mine > every_hi || (mine < every_lo && mine >= it.sinks))) {
+#pragma unroll 1
+                for (uint32_t c = h; c < D / 8; c += halves) {
+                  uint32_t x[4], y[4];
+                  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                               : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                               : "r"(place_of(c))
+                               : "memory");
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) y[i] = finite_only<T>(x[i]);
+                  if (((x[0] ^ y[0]) | (x[1] ^ y[1]) | (x[2] ^ y[2]) | (x[3] ^ y[3])) == 0) continue;
+                  *static_cast<volatile uint32_t*>(&s_left_out[pieces & 1]) = pieces + 1;
+                  put(place_of(c), y);
                 }
-                proxy_fence_smem();
-                if (halves == 2)
-                  asm volatile("bar.sync 2, 256;" ::: "memory");
-                else
-                  __syncwarp();
               }
+              proxy_fence_smem();
+              if (halves == 2)
+                asm volatile("bar.sync 2, 256;" ::: "memory");
+              else if (kPrefix)  // half 1 is here no more: rows of half 0 alone are the last item's
+                asm volatile("bar.sync 2, 128;" ::: "memory");
+              else
+                __syncwarp();
             }
             store_high();
             auto all = [&](auto mixed) {
@@ -746,6 +782,43 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
         wait(bar(kSummed, h), summed++);
         tmem_fence_after();
+        if (kPrefix && *static_cast<volatile uint32_t*>(&s_left_out[pieces & 1]) == pieces + 1) {
+          // The values that were kept from this piece's products, read again: an infinity
+          // or NaN is one whatever its weight.
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_load32(o, sums + c);
+#pragma unroll 1
+            for (uint32_t j = 0; j < n; ++j) {
+              const int token = first_token(it, at + j);
+              if (!partly_seen(token)) continue;
+#pragma unroll 1
+              for (int k = token; k < token + kTokens; ++k) {
+                const bool every = k <= every_hi && (k >= every_lo || k < it.sinks);
+                if (every || k > hi || (k < lo && k >= it.sinks)) continue;
+                const uint64_t row = checked_slot(a, a.prefix_table, k / a.page_tokens) * a.page_tokens + k % a.page_tokens;
+                const uint4* values = reinterpret_cast<const uint4*>(a.pool + (a.v_row0 + row) * a.token_bytes +
+                                                                     head * a.row_bytes + c * 2);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const uint4 v = values[i];
+                  const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                  for (int w = 0; w < 4; ++w) {
+                    const float2 y = unpack2<T>(x[w] ^ finite_only<T>(x[w]));
+                    uint32_t* to = o + i * 8 + w * 2;
+                    to[0] = __float_as_uint(__uint_as_float(to[0]) + y.x);
+                    to[1] = __float_as_uint(__uint_as_float(to[1]) + y.y);
+                  }
+                }
+              }
+            }
+            __syncwarp();
+            tmem_store32(sums + c, o);
+          }
+          tmem_wait_store();
+        }
         const bool whole = at == 0 && n == it.tiles, final = whole && a.part_o == nullptr;
         const bool write = r < it.rows && alive;
         const uint32_t t = it.q_first + row / a.group, q_head = head * a.group + row % a.group;
@@ -952,16 +1025,16 @@ Parts parts(const tcx_kv_attention_args& x, bool prefix) {
   return p;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool kPrefix>
 tcx_status launch(const TileArgs& d, const CUtensorMap& map, cudaStream_t stream) {
   using L = TileLayout<D>;
   static std::atomic<uint64_t> allowed{0};
-  if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(tile_kernel<T, D>), L::kBytes, &allowed);
+  if (const tcx_status st = allow_shared(reinterpret_cast<const void*>(tile_kernel<T, D, kPrefix>), L::kBytes, &allowed);
       st != TCX_OK)
     return st;
   // The first kernel of the call follows the stream's earlier work whole.
-  if (d.prefix) {
-    tile_kernel<T, D><<<d.max_ranges, kThreads, L::kBytes, stream>>>(map, d);
+  if (kPrefix) {
+    tile_kernel<T, D, kPrefix><<<d.max_ranges, kThreads, L::kBytes, stream>>>(map, d);
     note_launches(1);
     TCX_CUDA_TRY(cudaGetLastError());
   } else {
@@ -973,12 +1046,17 @@ tcx_status launch(const TileArgs& d, const CUtensorMap& map, cudaStream_t stream
       note_launches(1);
       TCX_CUDA_TRY(cudaGetLastError());
     }
-    if (const tcx_status st = launch_after(tile_kernel<T, D>, dim3(d.max_ranges), dim3(kThreads), L::kBytes, stream, map, d);
+    if (const tcx_status st = launch_after(tile_kernel<T, D, kPrefix>, dim3(d.max_ranges), dim3(kThreads), L::kBytes, stream, map, d);
         st != TCX_OK)
       return st;
   }
   if (d.max_ranges == 1 || d.join_here) return TCX_OK;
   return launch_after(tile_join_kernel<T, D>, dim3(d.max_ranges - 1, kRows / 8), dim3(256), 0, stream, d);
+}
+
+template <typename T, int D>
+tcx_status launch(const TileArgs& d, const CUtensorMap& map, cudaStream_t stream) {
+  return d.prefix ? launch<T, D, true>(d, map, stream) : launch<T, D, false>(d, map, stream);
 }
 
 }  // namespace

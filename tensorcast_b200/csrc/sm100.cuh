@@ -158,6 +158,12 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   }
 }
 
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t pair) {
+  if constexpr (__is_same(T, __nv_bfloat16)) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&pair));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&pair));
+}
+
 // ---- tensor memory and the fifth-generation tensor cores
 
 // `columns` of tensor memory for the CTA, by one whole warp; the address goes to shared memory.

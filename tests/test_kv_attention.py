@@ -642,6 +642,40 @@ def test_fp16_tail_of_a_decode_batch(cuda_device, gap):
         check((out[s:s + 1], lse[s:s + 1]), ref, FP16, n)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("group,dim,batch", [(4, 64, 4), (8, 128, 40), (5, 128, 70), (8, 64, 64)])
+def test_prefix_values_that_one_sequence_sees_stay_out_of_the_others(cuda_device, dtype, group, dim, batch):
+    """Windows that reach back into a shared prefix from different places, and queries that stand inside it: an
+    infinite or NaN value in the prefix shows in the rows that see it, in its column, and nowhere else."""
+    prefix, window, sinks, page = 515, 150, 4, 16
+    tokens = [(37 * i) % 190 + 10 * (i % 3) for i in range(batch)]
+    counts = [1 if i % 5 else 1 + 7 * i % 33 for i in range(batch)] if batch > 4 else [1] * batch
+    taken = -(-prefix // page)
+    w, free = kvtools.tables(tokens, page, 2, dim, taken=taken)
+    pool = kvtools.make_pool(w, 2, dim, dtype)
+    rows = free[:taken][np.arange(prefix) // page].astype(np.int64) * page + np.arange(prefix) % page
+    g = torch.Generator().manual_seed(7)
+    pool[:, torch.from_numpy(rows)] = torch.randn((2, prefix, 2, dim), generator=g).to(dtype)
+    for token, column, value in ((2, 1, math.inf), (380, 3, math.nan), (400, 4, -math.inf), (430, 5, math.inf),
+                                 (440, 6, math.inf), (441, 6, -math.inf), (500, 7, math.inf), (511, 8, math.nan),
+                                 (512, 9, -math.inf), (514, 10, math.inf), (300, 11, math.nan)):
+        pool[1, int(rows[token]), token % 2, column] = value
+    pool, q = pool.cuda(), queries(sum(counts), 2 * group, dim, dtype, 0)
+    att = KvAttention(w, 2 * group, 2, dtype, query_tokens=counts, window=window, sinks=sinks,
+                      prefix_pages=free[:taken], prefix_tokens=prefix)
+    out, lse = att.run(pool, 0, q)
+    att.check_status()
+    ref = kvtools.attention(w, pool, 0, q, counts, window, sinks, prefix_rows=rows)
+    finite = torch.isfinite(ref[0])
+    assert finite.any() and not finite.all()
+    assert (torch.isnan(out) == torch.isnan(ref[0])).all()
+    assert (out[torch.isinf(ref[0])].double() == ref[0][torch.isinf(ref[0])]).all()
+    tol, tol_lse, _ = kvtools.bounds(ref, dtype, 800)
+    assert ((out.double() - ref[0]).abs() <= tol)[finite].all()
+    assert ((lse.double() - ref[1]).abs() <= tol_lse)[ref[1] > -math.inf].all()
+
+
 # ---------------------------------------------------------------- accumulated weights (GPU)
 
 @pytest.mark.gpu
