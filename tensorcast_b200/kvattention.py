@@ -103,9 +103,12 @@ class _OnDevice:
         return raw
 
     def check_status(self) -> None:
-        """Waits for the device and raises what a call has recorded."""
+        """Waits for the device, all its streams, and raises what a call has recorded since the last check."""
+        torch.cuda.synchronize(self.device)
         code = int(self.status.item())
         if code:
+            self.status.zero_()
+            torch.cuda.synchronize(self.device)  # calls on other streams that follow record anew
             raise _native.TcxError(_native.DATA_LOSS, _STATUS.get(code, f"kv attention status {code}"))
 
     def _pool(self, pool: torch.Tensor) -> int:

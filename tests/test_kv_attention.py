@@ -676,6 +676,38 @@ def test_prefix_values_that_one_sequence_sees_stay_out_of_the_others(cuda_device
     assert ((lse.double() - ref[1]).abs() <= tol_lse)[ref[1] > -math.inf].all()
 
 
+@pytest.mark.gpu
+def test_check_status_waits_for_every_stream_and_starts_anew(cuda_device):
+    """The error of a call that another stream still holds back is found; once it is raised, it is forgotten."""
+    w, free = kvtools.tables([100, 90], taken=4)
+    pool = kvtools.make_pool(w, 2, 64, BF16).cuda()
+    q = queries(2, 4, 64, BF16, 0)
+    dst = KvWorkload(w.planes, w.pool_pages, 16, w.token_bytes, np.array([20, 20], np.uint32),
+                     np.array([0, 2, 4], np.uint64), free[:4].copy())
+    weights = torch.ones((1, 2, int(w.page_offsets[-1]) * 16), device="cuda")
+    side = torch.cuda.Stream()
+    for handle, call in ((KvAttention(w, 4, 2), lambda h, s: h.run(pool, 0, q, stream=s)),
+                         (KvEvict(w, dst, 2), lambda h, s: h.run(pool, weights, stream=s))):
+        good = handle.page_table.clone()
+        call(handle, side)
+        handle.check_status()
+        handle.page_table[1] = 10_000_000
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(300_000_000)
+        call(handle, side)
+        with pytest.raises(_native.TcxError, match="outside the pool"):
+            handle.check_status()
+        handle.page_table.copy_(good)
+        handle.check_status()
+        call(handle, None)
+        handle.check_status()
+        handle.seq_tokens[1] = 1000
+        call(handle, None)
+        with pytest.raises(_native.TcxError, match="more tokens"):
+            handle.check_status()
+
+
 # ---------------------------------------------------------------- accumulated weights (GPU)
 
 @pytest.mark.gpu
