@@ -48,12 +48,22 @@ def _cuda_device(device) -> torch.device:
     return d if d.index is not None else torch.device("cuda", torch.cuda.current_device())
 
 
+def _slots(table, what: str) -> np.ndarray:
+    """Page slots in 32 bits; -1, a usual mark of an unused entry, becomes one outside of every pool."""
+    t = np.asarray(table)
+    for slot in (int(t.min()), int(t.max())) if t.size else ():
+        if not -(1 << 31) <= slot < 1 << 32:
+            _refuse(f"{what}: page slot {slot} does not fit 32 bits")
+    return t.astype(np.uint32)
+
+
 def _check_tables(w: KvWorkload, what: str) -> None:
     offs = np.asarray(w.page_offsets).astype(np.int64)
     if offs.size != w.n_seq + 1 or offs[0] != 0 or (np.diff(offs) < 0).any():
         _refuse(f"{what}: page_offsets must start at 0 and not decrease")
     if int(offs[-1]) != np.asarray(w.page_table).size:
         _refuse(f"{what}: page_offsets end at {int(offs[-1])}, the page table has {np.asarray(w.page_table).size}")
+    _slots(w.page_table, what)
     if (np.asarray(w.seq_tokens).astype(np.int64) > np.diff(offs) * w.page_tokens).any():
         _refuse(f"{what}: a sequence has more tokens than its pages hold")
 
@@ -155,7 +165,7 @@ class KvAttention(_OnDevice):
             _refuse(f"query_tokens must be {w.n_seq} counts, none negative")
         if prefix_pages is None and prefix_tokens:
             _refuse("prefix_tokens without prefix_pages")
-        pages = np.zeros(0, np.uint32) if prefix_pages is None else np.asarray(prefix_pages).astype(np.uint32)
+        pages = np.zeros(0, np.uint32) if prefix_pages is None else _slots(prefix_pages, "prefix")
         if prefix_tokens < 0 or prefix_tokens > pages.size * w.page_tokens:
             _refuse(f"prefix_tokens {prefix_tokens}: the prefix pages hold {pages.size * w.page_tokens}")
         self.w, self.q_heads, self.kv_heads, self.head_dim, self.dtype = w, q_heads, kv_heads, head_dim, dtype
@@ -163,7 +173,7 @@ class KvAttention(_OnDevice):
         self.device = _cuda_device(device)
         offs = np.asarray(w.page_offsets).astype(np.uint64)
         t = self._bind(w, {
-            "page_offsets": offs, "page_table": np.asarray(w.page_table).astype(np.uint32),
+            "page_offsets": offs, "page_table": _slots(w.page_table, "sequences"),
             "seq_tokens": np.asarray(w.seq_tokens).astype(np.uint32), "q_offsets": self.q_offsets.astype(np.uint32),
             "prefix_table": pages, "prefix_tokens": np.array([prefix_tokens], np.uint32),
             "status": np.zeros(1, np.uint32)})
@@ -312,17 +322,17 @@ class KvEvict(_OnDevice):
         stays = np.minimum(np.asarray(w.seq_tokens).astype(np.int64), min(sinks + recent, 1 << 32))
         if (np.asarray(dst.seq_tokens).astype(np.int64) < stays).any():
             _refuse(f"a budget is below sinks + recent ({sinks + recent}) and below its sequence")
-        to = np.asarray(dst.page_table)
+        table, to = _slots(w.page_table, "sequences"), _slots(dst.page_table, "destination")
         if np.unique(to).size != to.size:
             _refuse("a destination page is listed twice")
-        if np.isin(to, np.asarray(w.page_table)).any():
+        if np.isin(to, table).any():
             _refuse("a destination page is a source page")
         self.w, self.dst, self.kv_heads, self.device = w, dst, kv_heads, _cuda_device(device)
         u32 = lambda x: np.asarray(x).astype(np.uint32)  # noqa: E731
         u64 = lambda x: np.asarray(x).astype(np.uint64)  # noqa: E731
         t = self._bind(w, {
             "page_offsets": u64(w.page_offsets), "dst_page_offsets": u64(dst.page_offsets),
-            "page_table": u32(w.page_table), "dst_page_table": u32(dst.page_table), "seq_tokens": u32(w.seq_tokens),
+            "page_table": table, "dst_page_table": to, "seq_tokens": u32(w.seq_tokens),
             "budgets": u32(dst.seq_tokens), "status": np.zeros(1, np.uint32)})
         self.page_table, self.seq_tokens = t.page_table, t.seq_tokens
         self._args = _native.KvEvictArgs(

@@ -67,6 +67,19 @@ def test_evict_refuses_what_it_cannot_run():
     refused("CUDA device", make(good, device="cpu"))
 
 
+def test_page_slots_that_32_bits_do_not_hold_are_refused():
+    """A slot of 2^32 + 3 is not slot 3. (-1 is a usual mark of an unused entry and stays outside of every pool.)"""
+    w, free = kvtools.tables([5, 40], taken=3)
+    wide = lambda slot: KvWorkload(**{**w.__dict__, "page_table": np.concatenate(  # noqa: E731
+        [[slot], w.page_table[1:].astype(np.int64)])})
+    for slot in (1 << 32, (1 << 32) + 3, -(1 << 32) + 3, -(1 << 31) - 1):
+        refused("slot .* 32 bits", lambda: KvAttention(wide(slot), 4, 2, device="cpu"))
+        refused("slot .* 32 bits", lambda: KvAttention(w, 4, 2, prefix_pages=[1, slot], prefix_tokens=3, device="cpu"))
+        refused("slot .* 32 bits", lambda: KvEvict(wide(slot), w, 2, device="cpu"))
+        refused("slot .* 32 bits", lambda: KvEvict(w, wide(slot), 2, device="cpu"))
+    refused("CUDA device", lambda: KvAttention(wide(-1), 4, 2, device="cpu"))
+
+
 def attention_args(**kw):
     """Arguments that pass the checks of the C entry, made-up pointers among them, with `kw` changed."""
     a = _native.KvAttentionArgs(
