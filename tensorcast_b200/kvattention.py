@@ -214,6 +214,14 @@ class KvAttention(_OnDevice):
             _refuse(f"{what} must have dense heads, strides that are multiples of 8 and 16-byte alignment")
         return at, tokens, heads
 
+    def _check_apart(self, tokens: int, heads: int) -> None:
+        """Rows of an output with these strides must lie apart, whichever axis is the outer one."""
+        n, m, dim = self._args.q_tokens, self.q_heads, self.head_dim
+        outer = lambda n, tokens, m, heads: ((m < 2 or heads >= dim) and  # noqa: E731
+                                             (n < 2 or tokens >= (m - 1) * heads + dim))
+        if not outer(n, tokens, m, heads) and not outer(m, heads, n, tokens):
+            _refuse(f"out's rows overlap: strides of {tokens} (tokens) and {heads} (heads)")
+
     def _workspace(self, a, stream: int):
         """Scratch and counters: a stream's calls share them, a captured graph has its own."""
         weighed = a.d_weights is not None
@@ -262,6 +270,7 @@ class KvAttention(_OnDevice):
             if out.untyped_storage().data_ptr() in (q.untyped_storage().data_ptr(),
                                                     pool.untyped_storage().data_ptr()):
                 _refuse("out must not share memory with q or the pool")
+            self._check_apart(a.out_token_stride, a.out_head_stride)
         if lse is None:
             lse = torch.empty_like(self._lse_like) if not padded else torch.zeros((rows, self.q_heads),
                                                                                   device=self.device)

@@ -721,6 +721,20 @@ def test_check_status_waits_for_every_stream_and_starts_anew(cuda_device):
             handle.check_status()
 
 
+@pytest.mark.gpu
+def test_outputs_whose_rows_overlap_are_refused(cuda_device):
+    w, _ = kvtools.tables([20, 30])
+    pool = kvtools.make_pool(w, 2, 64, BF16).cuda()
+    q = queries(2, 4, 64, BF16, 0)
+    att = KvAttention(w, 4, 2)
+    flat = torch.zeros(4096, dtype=BF16, device="cuda")
+    for strides in ((0, 64, 1), (256, 0, 1), (256, 32, 1), (64, 64, 1), (192, 64, 1), (64, 120, 1)):
+        refused("rows overlap", lambda: att.run(pool, 0, q, out=flat.as_strided((2, 4, 64), strides)))
+    want = att.run(pool, 0, q)[0]
+    for strides in ((256, 64, 1), (64, 128, 1), (320, 72, 1), (264, 64, 1)):
+        assert (att.run(pool, 0, q, out=flat.as_strided((2, 4, 64), strides))[0] == want).all()
+
+
 # ---------------------------------------------------------------- accumulated weights (GPU)
 
 @pytest.mark.gpu
