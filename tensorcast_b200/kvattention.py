@@ -210,6 +210,8 @@ class KvAttention(_OnDevice):
                     f"got {list(x.shape)}")
         tokens, heads, values = x.stride()
         at = x.data_ptr()
+        if tokens % 8 or heads % 8:  # the stride of an axis of one entry is never used
+            tokens, heads = tokens if x.shape[0] > 1 else 0, heads if self.q_heads > 1 else 0
         if values != 1 or tokens % 8 or heads % 8 or at % 16:
             _refuse(f"{what} must have dense heads, strides that are multiples of 8 and 16-byte alignment")
         return at, tokens, heads
@@ -284,7 +286,8 @@ class KvAttention(_OnDevice):
             columns = self.weight_columns
             if (weights.dtype != torch.float32 or weights.get_device() != self.device.index
                     or weights.shape != (self.kv_heads, columns)
-                    or (columns and weights.stride(1) != 1) or weights.stride(0) < columns):
+                    or (columns and weights.stride(1) != 1)
+                    or (self.kv_heads > 1 and weights.stride(0) < columns)):
                 _refuse(f"weights must be float32 [{self.kv_heads}, {columns}] on {self.device}, "
                         "dense in its columns")
             a.d_weights, a.weights_head_stride = weights.data_ptr(), weights.stride(0)

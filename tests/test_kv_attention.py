@@ -735,6 +735,22 @@ def test_outputs_whose_rows_overlap_are_refused(cuda_device):
         assert (att.run(pool, 0, q, out=flat.as_strided((2, 4, 64), strides))[0] == want).all()
 
 
+@pytest.mark.gpu
+def test_strides_of_single_tokens_and_heads_do_not_matter(cuda_device):
+    """The stride of an axis of one entry can be anything: a lone query row, one head, one kv head's weights."""
+    w, _ = kvtools.tables([70], kv_heads=1)
+    pool = kvtools.make_pool(w, 1, 64, BF16).cuda()
+    q = queries(1, 1, 64, BF16, 0)
+    att = KvAttention(w, 1, 1)
+    columns = att.weight_columns
+    want, got = torch.zeros((1, columns), device="cuda"), torch.zeros((columns, 1), device="cuda").t()
+    assert got.stride() == (1, 1)
+    out, lse = att.run(pool, 0, q, weights=want)
+    odd = att.run(pool, 0, q.as_strided((1, 1, 64), (3, 5, 1)), weights=got,
+                  out=torch.zeros(64, dtype=BF16, device="cuda").as_strided((1, 1, 64), (1, 1, 1)))
+    assert (odd[0] == out).all() and (odd[1] == lse).all() and (got == want).all()
+
+
 # ---------------------------------------------------------------- accumulated weights (GPU)
 
 @pytest.mark.gpu
