@@ -27,6 +27,7 @@
 #include <type_traits>
 
 #include "kv_attention.cuh"
+#include "kv_pieces.h"
 
 namespace tcx {
 namespace {
@@ -312,7 +313,16 @@ __global__ void __launch_bounds__(32 * (kWarps * G + 1), G == 1 ? 2 : 1)
   for (uint32_t i = 0; i < count; ++i) {
     const uint32_t stage = i % L::kStages, at = base + stage * L::kStage;
     alive = alive && mbar_wait_warp(smem_addr(&s_full[stage]), i / L::kStages & 1, &s_gave_up, a.status);
-    const TileInfo info = s_info[stage];
+    TileInfo info{};
+    if (alive) {
+      info = s_info[stage];
+    } else {
+      // The notes may be another lap's, and the copies may still arrive for other warps: a
+      // warp whose wait ran out meets them as often as they do, by the lengths alone, and
+      // has no rows, so that it reads and stores nothing.
+      const TileEnd end = tile_end(s_begin[0], s_begin[1], count, i, [&](uint32_t s) { return seq_info(a, s, prefix).tiles; });
+      info.flags = (end.last ? kLast : 0u) | (end.whole ? kWhole : 0u);
+    }
     if (info.flags & kFirst) {
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)

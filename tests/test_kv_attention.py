@@ -80,6 +80,36 @@ def test_page_slots_that_32_bits_do_not_hold_are_refused():
     refused("CUDA device", lambda: KvAttention(wide(-1), 4, 2, device="cpu"))
 
 
+def test_pieces_of_a_range_follow_from_the_lengths(tmp_path):
+    """Warps that meet at a piece's end count the pieces by this where they cannot read the notes: it must say what
+    the notes do, at every tile of every range."""
+    import ctypes
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(_native.__file__), "csrc")
+    (tmp_path / "pieces.cc").write_text("""
+#include "kv_pieces.h"
+extern "C" int ends(const uint32_t* tiles, uint32_t seq, uint32_t tile, uint32_t count, uint32_t i) {
+  const tcx::TileEnd e = tcx::tile_end(seq, tile, count, i, [&](uint32_t s) { return tiles[s]; });
+  return e.last + 2 * e.whole;
+}""")
+    so = str(tmp_path / "pieces.so")
+    subprocess.check_call(["g++", "-std=c++17", "-shared", "-fPIC", "-I", csrc, str(tmp_path / "pieces.cc"), "-o", so])
+    ends = ctypes.CDLL(so).ends
+    rng = np.random.default_rng(0)
+    for ranges in (1, 2, 3, 7, 20):
+        tiles = rng.choice([0, 0, 1, 1, 2, 3, 9], 25).astype(np.uint32)
+        tiles[-1] = 1
+        flat = [(s, t) for s, n in enumerate(tiles) for t in range(n)]
+        for r in range(ranges):
+            mine = flat[len(flat) * r // ranges: len(flat) * (r + 1) // ranges]
+            for i, (s, t) in enumerate(mine):
+                last = i + 1 == len(mine) or mine[i + 1][0] != s
+                whole = last and sum(x[0] == s for x in mine) == tiles[s]
+                got = ends(tiles.ctypes.data_as(ctypes.c_void_p), int(mine[0][0]), mine[0][1], len(mine), i)
+                assert got == last + 2 * whole, (ranges, r, i)
+
+
 def attention_args(**kw):
     """Arguments that pass the checks of the C entry, made-up pointers among them, with `kw` changed."""
     a = _native.KvAttentionArgs(
