@@ -78,12 +78,9 @@ AttnArgs device_args(const tcx_kv_attention_args& x) {
   a.pool_pages = x.pool_pages;
   a.row_bytes = x.head_dim * 2;
   a.token_bytes = x.kv_heads * a.row_bytes;
-  a.page_bytes = x.page_tokens * a.token_bytes;
   a.page_tokens = static_cast<uint32_t>(x.page_tokens);
   a.kv_heads = static_cast<uint32_t>(x.kv_heads);
   a.group = static_cast<uint32_t>(x.q_heads / x.kv_heads);
-  a.k_plane = x.k_plane;
-  a.v_plane = x.v_plane;
   a.page_table = x.d_page_table;
   a.page_offsets = x.d_page_offsets;
   a.seq_tokens = x.d_seq_tokens;

@@ -12,9 +12,8 @@ constexpr uint32_t kBadSlot = 1, kBadLength = 2;
 
 struct AttnArgs {
   const uint8_t* pool;
-  uint64_t pool_pages, page_bytes, token_bytes, row_bytes;  // row: one head of one token
+  uint64_t pool_pages, token_bytes, row_bytes;  // row: one head of one token
   uint32_t page_tokens, kv_heads, group;
-  uint64_t k_plane, v_plane;
   const uint32_t* page_table;
   const uint64_t* page_offsets;
   const uint32_t* seq_tokens;
@@ -102,47 +101,27 @@ __device__ __forceinline__ Finish finish_row(const AttnArgs& a, uint64_t row, fl
   return f;
 }
 
-// N values of a finished row from column e on, N a multiple of 4.
-template <typename T, int D, int N>
+// Four values of a finished row, from column e on.
+template <typename T, int D>
 __device__ __forceinline__ void store_row(const AttnArgs& a, uint32_t t, uint32_t h, uint32_t e, const Finish& f,
-                                          const float (&v)[N]) {
+                                          const float (&v)[4]) {
   const uint64_t row = static_cast<uint64_t>(t) * a.kv_heads * a.group + h;
-  float x[N];
+  float x[4];
 #pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = v[i] * f.own;
-  if (f.own == 0.f) {  // nothing seen here: 0, whatever the sums hold
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = 0.f;
-  }
+  for (int i = 0; i < 4; ++i) x[i] = f.own == 0.f ? 0.f : v[i] * f.own;  // nothing seen here: 0, whatever the sums hold
   if (f.prior != 0.f) {
-    const float4* p = reinterpret_cast<const float4*>(a.prior_o + row * D + e);
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const float4 y = p[i];
-      x[4 * i] += f.prior * y.x;
-      x[4 * i + 1] += f.prior * y.y;
-      x[4 * i + 2] += f.prior * y.z;
-      x[4 * i + 3] += f.prior * y.w;
-    }
+    const float4 y = *reinterpret_cast<const float4*>(a.prior_o + row * D + e);
+    x[0] += f.prior * y.x;
+    x[1] += f.prior * y.y;
+    x[2] += f.prior * y.z;
+    x[3] += f.prior * y.w;
   }
   if (a.part_o != nullptr) {
-    float4* p = reinterpret_cast<float4*>(a.part_o + row * D + e);
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) p[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+    *reinterpret_cast<float4*>(a.part_o + row * D + e) = make_float4(x[0], x[1], x[2], x[3]);
     return;
   }
   uint8_t* out = a.out + t * a.out_token_stride + h * a.out_head_stride + e * 2;
-  if constexpr (N % 8 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 8; ++i)
-      reinterpret_cast<uint4*>(out)[i] = make_uint4(pack2<T>(x[8 * i], x[8 * i + 1]), pack2<T>(x[8 * i + 2], x[8 * i + 3]),
-                                                    pack2<T>(x[8 * i + 4], x[8 * i + 5]),
-                                                    pack2<T>(x[8 * i + 6], x[8 * i + 7]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i)
-      reinterpret_cast<uint2*>(out)[i] = make_uint2(pack2<T>(x[4 * i], x[4 * i + 1]), pack2<T>(x[4 * i + 2], x[4 * i + 3]));
-  }
+  *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
 }
 
 __device__ __forceinline__ void store_lse(const AttnArgs& a, uint32_t t, uint32_t h, const Finish& f) {

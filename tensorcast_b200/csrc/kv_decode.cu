@@ -128,7 +128,7 @@ __device__ __forceinline__ void join_parts(const DecodeArgs& d, const TileInfo& 
     if (r0 + threadIdx.x / kLanes >= rows) continue;
     const uint32_t t = info.q_first + r / a.group, h = head * a.group + r % a.group;
     const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
-    store_row<T, D, 4>(a, t, h, e, f, x);
+    store_row<T, D>(a, t, h, e, f, x);
     if (e == 0) store_lse(a, t, h, f);
   }
   __syncwarp();
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(32 * (kWarps * G + 1), G == 1 ? 2 : 1)
           if (info.flags & kWhole) {
             const uint32_t t = info.q_first + r / a.group, h = head * a.group + r % a.group;
             const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
-            store_row<T, D, 4>(a, t, h, e, f, {v.x, v.y, v.z, v.w});
+            store_row<T, D>(a, t, h, e, f, {v.x, v.y, v.z, v.w});
             if (e == 0) store_lse(a, t, h, f);
           } else {
             const uint64_t row =

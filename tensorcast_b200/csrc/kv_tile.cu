@@ -21,8 +21,8 @@
 // Work: the visible (row tile, kv head, token tile) units laid end to end and cut
 // into equal ranges, one CTA on every SM, whatever the prompts' lengths and masks
 // are; row tiles cut by a border leave parts in the scratch, which are added up in the
-// ranges' order by tile_join_kernel, or where they are few by the CTA that comes
-// last. tile_plan_kernel lays prompts' units out from the device's lengths; over a
+// ranges' order by tile_join_kernel, or where a prefix has few rows in all by the CTA
+// that comes last. tile_plan_kernel lays prompts' units out from the device's lengths; over a
 // prefix all row tiles have the same ones.
 //
 // Bound by the softmax: a unit's products take 2560 cycles, its exponentials 1536 on
@@ -51,7 +51,7 @@ constexpr int kPlanCache = 2048;
 // scores, its output), in token tiles: counted when the work is cut into ranges.
 constexpr uint32_t kPieceCost = 3;
 
-// Up to so many rows the CTA that comes last adds their parts up, one warp to a row
+// Over a prefix: up to so many rows the CTA that comes last adds their parts up, one warp to a row
 // at a time: 256 rows took it 115 us over 18 ranges, a launch of its own takes 18.
 constexpr uint32_t kJoinHere = 32;
 
@@ -78,7 +78,7 @@ struct RangeEnd {
 struct TileArgs {
   AttnArgs a;
   uint32_t prefix;  // rows of all sequences over the shared prefix
-  uint32_t join_here;  // few rows: the CTA that comes last adds their parts up
+  uint32_t join_here;  // few rows over a prefix: the CTA that comes last adds their parts up
   uint32_t max_q, max_ranges;
   uint32_t* item_first;  // [n_seq + 1]
   Item* items;
@@ -243,50 +243,49 @@ __device__ __forceinline__ uint32_t finite_only(uint32_t pair) {
   return pair;
 }
 
-// The rows of an item and head that the ranges [from, to] hold parts of, one warp of
-// eight to a row, the parts in the ranges' order.
+// Row r of an item and head, of which the ranges [from, to] hold parts: a warp adds them
+// up in the ranges' order. The first of them is in place `first_slot` of its range.
 template <typename T, int D>
-__device__ __forceinline__ void join_rows(const TileArgs& d, const Item& it, uint32_t head, uint32_t from, uint32_t to,
-                                          uint32_t first_slot, uint32_t warp, uint32_t lane) {
+__device__ __forceinline__ void join_row(const TileArgs& d, const Item& it, uint32_t head, uint32_t from, uint32_t to,
+                                         uint32_t first_slot, uint32_t r, uint32_t lane) {
   constexpr int E = D / 32;
   const AttnArgs& a = d.a;
-  for (uint32_t r = warp; r < it.rows; r += 8) {
-    auto row_of = [&](uint32_t k) { return static_cast<uint64_t>(k * 2 + (k == from ? first_slot : 0)) * kRows + r; };
-    float top = -INFINITY, sum = 0.f, x[E] = {};
-    for (uint32_t k = from + lane; k <= to; k += 32) top = fmaxf(top, __ldcg(&d.part_ml[row_of(k)].x));
-    for (int i = 16; i; i /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
-    const float ref = top == -INFINITY ? 0.f : top;
+  auto row_of = [&](uint32_t k) { return static_cast<uint64_t>(k * 2 + (k == from ? first_slot : 0)) * kRows + r; };
+  float top = -INFINITY, sum = 0.f, x[E] = {};
+  for (uint32_t k = from + lane; k <= to; k += 32) top = fmaxf(top, __ldcg(&d.part_ml[row_of(k)].x));
+  for (int i = 16; i; i /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
+  const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll 4
-    for (uint32_t k = from; k <= to; ++k) {
-      const uint64_t row = row_of(k);
-      const float2 ml = __ldcg(&d.part_ml[row]);
-      const float f = exp2_approx(ml.x - ref);
-      sum += f * ml.y;
-      if constexpr (E == 4) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(d.part_o + row * D) + lane);
-        x[0] += f * v.x;
-        x[1] += f * v.y;
-        x[2] += f * v.z;
-        x[3] += f * v.w;
-      } else {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(d.part_o + row * D) + lane);
-        x[0] += f * v.x;
-        x[1] += f * v.y;
-      }
-    }
-    const uint32_t row = it.row0 + r, t = it.q_first + row / a.group, h = head * a.group + row % a.group;
-    const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
+  for (uint32_t k = from; k <= to; ++k) {
+    const uint64_t row = row_of(k);
+    const float2 ml = __ldcg(&d.part_ml[row]);
+    const float f = exp2_approx(ml.x - ref);
+    sum += f * ml.y;
     if constexpr (E == 4) {
-      store_row<T, D, 4>(a, t, h, lane * 4, f, x);
-    } else {  // two lanes' values in one
-      const float y[4] = {x[0], x[1], __shfl_down_sync(~0u, x[0], 1), __shfl_down_sync(~0u, x[1], 1)};
-      if (lane % 2 == 0) store_row<T, D, 4>(a, t, h, lane * 2, f, y);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(d.part_o + row * D) + lane);
+      x[0] += f * v.x;
+      x[1] += f * v.y;
+      x[2] += f * v.z;
+      x[3] += f * v.w;
+    } else {
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(d.part_o + row * D) + lane);
+      x[0] += f * v.x;
+      x[1] += f * v.y;
     }
-    if (lane == 0) store_lse(a, t, h, f);
-    __syncwarp();
   }
+  const uint32_t row = it.row0 + r, t = it.q_first + row / a.group, h = head * a.group + row % a.group;
+  const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
+  if constexpr (E == 4) {
+    store_row<T, D>(a, t, h, lane * 4, f, x);
+  } else {  // two lanes' values in one
+    const float y[4] = {x[0], x[1], __shfl_down_sync(~0u, x[0], 1), __shfl_down_sync(~0u, x[1], 1)};
+    if (lane % 2 == 0) store_row<T, D>(a, t, h, lane * 2, f, y);
+  }
+  if (lane == 0) store_lse(a, t, h, f);
+  __syncwarp();
 }
 
+// kPrefix: the rows of all sequences over the shared prefix.
 template <typename T, int D, bool kPrefix>
 __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant__ CUtensorMap map, TileArgs d) {
   using L = TileLayout<D>;
@@ -899,7 +898,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
         tmem_fence_before();
       }
-      if (d.join_here && (at != 0 || n != it.tiles)) {
+      if (kPrefix && d.join_here && (at != 0 || n != it.tiles)) {
         // Another range has parts of these rows too: whoever comes last adds them up.
         const uint64_t first = begin.unit + tiles_done - at, last = first + it.tiles - 1;
         uint32_t from = 0, to = 0;  // the last ranges that begin at the first and last tile, or before
@@ -914,7 +913,10 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         asm volatile("bar.sync 1, 256;" ::: "memory");
         if (threadIdx.x == 0) s_last = alive && last_to_arrive(a.counters + TCX_KV_COUNTERS / 2 + from, to - from + 1);
         asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (s_last) join_rows<T, D>(d, it, head, from, to, begin_of(from).unit != first, warp, lane);
+        if (s_last) {
+          const uint32_t first_slot = begin_of(from).unit != first;
+          for (uint32_t r = warp; r < it.rows; r += 8) join_row<T, D>(d, it, head, from, to, first_slot, r, lane);
+        }
       }
       left -= n;
       tiles_done += n;
@@ -937,7 +939,6 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
 // ones, in the ranges' order: one warp for each row.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) tile_join_kernel(TileArgs d) {
-  constexpr int E = D / 32;
   const AttnArgs& a = d.a;
   const uint32_t range = blockIdx.x, r = blockIdx.y * 8 + threadIdx.x / 32, lane = threadIdx.x % 32;
   next_may_start();
@@ -954,39 +955,7 @@ __global__ void __launch_bounds__(256) tile_join_kernel(TileArgs d) {
     end += __ffs(ends) - 1;
     break;
   }
-  auto row_of = [&](uint32_t k) { return static_cast<uint64_t>(k * 2 + (k == range ? own.slot : 0)) * kRows + r; };
-  float top = -INFINITY, sum = 0.f, x[E] = {};
-  for (uint32_t k = range + lane; k <= end; k += 32) top = fmaxf(top, d.part_ml[row_of(k)].x);
-  for (int i = 16; i; i /= 2) top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
-  const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll 4
-  for (uint32_t k = range; k <= end; ++k) {
-    const uint64_t row = row_of(k);
-    const float2 ml = d.part_ml[row];
-    const float f = exp2_approx(ml.x - ref);
-    sum += f * ml.y;
-    const float* o = d.part_o + row * D + lane * E;
-    if constexpr (E == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(o);
-      x[0] += f * v.x;
-      x[1] += f * v.y;
-      x[2] += f * v.z;
-      x[3] += f * v.w;
-    } else {
-      const float2 v = *reinterpret_cast<const float2*>(o);
-      x[0] += f * v.x;
-      x[1] += f * v.y;
-    }
-  }
-  const uint32_t row = it.row0 + r, t = it.q_first + row / a.group, h = own.head * a.group + row % a.group;
-  const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
-  if constexpr (E == 4) {
-    store_row<T, D, 4>(a, t, h, lane * 4, f, x);
-  } else {  // two lanes' values in one
-    const float y[4] = {x[0], x[1], __shfl_down_sync(~0u, x[0], 1), __shfl_down_sync(~0u, x[1], 1)};
-    if (lane % 2 == 0) store_row<T, D, 4>(a, t, h, lane * 2, f, y);
-  }
-  if (lane == 0) store_lse(a, t, h, f);
+  join_row<T, D>(d, it, own.head, range, end, own.slot, r, lane);
 }
 
 uint64_t max_items(const tcx_kv_attention_args& x, bool prefix) {
@@ -1071,7 +1040,7 @@ tcx_status launch_tile(const tcx_kv_attention_args& x, const AttnArgs& a, const 
   d.a = a;
   d.prefix = prefix;
   d.max_q = static_cast<uint32_t>(x.max_q);
-  d.join_here = (prefix ? x.q_tokens : x.max_q) * a.group <= kJoinHere;
+  d.join_here = prefix && x.q_tokens * a.group <= kJoinHere;
   d.max_ranges = max_ranges(x, prefix);
   d.item_first = reinterpret_cast<uint32_t*>(at + p.item_first);
   d.items = reinterpret_cast<Item*>(at + p.items);
