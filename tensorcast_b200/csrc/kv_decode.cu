@@ -306,23 +306,15 @@ __global__ void __launch_bounds__(32 * (kWarps * G + 1), G == 1 ? 2 : 1)
   // ---- the consumers: rows row0 + lane / 4 and 8 more, tokens 16 part .. 16 part + 15 of each tile
   const uint32_t part = warp % kWarps, row0 = warp / kWarps * kWarpRows;
   auto meet = [&] { asm volatile("bar.sync 1, %0;" ::"n"(128 * G) : "memory"); };
+  constexpr int kMeets = 2 * G + 1;  // at the end of a piece, and one more where its parts are joined
   uint32_t qf[D / 16][4];
   constexpr bool kIsHalf = std::is_same<T, __half>::value;
   float o[D / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, peak[2] = {-INFINITY, -INFINITY};
-  bool alive = true;
-  for (uint32_t i = 0; i < count; ++i) {
+  uint32_t i = 0;
+  for (; i < count; ++i) {
     const uint32_t stage = i % L::kStages, at = base + stage * L::kStage;
-    alive = alive && mbar_wait_warp(smem_addr(&s_full[stage]), i / L::kStages & 1, &s_gave_up, a.status);
-    TileInfo info{};
-    if (alive) {
-      info = s_info[stage];
-    } else {
-      // The notes may be another lap's, and the copies may still arrive for other warps: a
-      // warp whose wait ran out meets them as often as they do, by the lengths alone, and
-      // has no rows, so that it reads and stores nothing.
-      const TileEnd end = tile_end(s_begin[0], s_begin[1], count, i, [&](uint32_t s) { return seq_info(a, s, prefix).tiles; });
-      info.flags = (end.last ? kLast : 0u) | (end.whole ? kWhole : 0u);
-    }
+    if (!mbar_wait_warp(smem_addr(&s_full[stage]), i / L::kStages & 1, &s_gave_up, a.status)) break;
+    const TileInfo info = s_info[stage];
     if (info.flags & kFirst) {
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
@@ -398,7 +390,7 @@ __global__ void __launch_bounds__(32 * (kWarps * G + 1), G == 1 ? 2 : 1)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const uint32_t row = row0 + lane / 4 + 8 * r;
-        if (row < info.queries * a.group && row < d.score_rows && alive) {
+        if (row < info.queries * a.group && row < d.score_rows) {
           float* to = d.scores + (static_cast<uint64_t>(head) * d.score_rows + row) * d.columns + column;
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
@@ -494,7 +486,6 @@ __global__ void __launch_bounds__(32 * (kWarps * G + 1), G == 1 ? 2 : 1)
             v.z += f * x.z;
             v.w += f * x.w;
           }
-          if (!alive) continue;
           if (info.flags & kWhole) {
             const uint32_t t = info.q_first + r / a.group, h = head * a.group + r % a.group;
             const Finish f = finish_row(a, static_cast<uint64_t>(t) * a.kv_heads * a.group + h, top, sum);
@@ -511,13 +502,26 @@ __global__ void __launch_bounds__(32 * (kWarps * G + 1), G == 1 ? 2 : 1)
       meet();  // all have read s_ml: the next sequence's come there
       if (!(info.flags & kWhole)) {  // whoever comes last adds the parts up, in the ranges' order
         if (threadIdx.x == 0)
-          s_last = alive && last_to_arrive(a.counters + info.first_range * a.kv_heads + head, info.parts);
+          s_last = last_to_arrive(a.counters + info.first_range * a.kv_heads + head, info.parts);
         meet();
         if (s_last) join_parts<T, D, G>(d, info, head, rows);
       }
       proxy_fence_smem();  // these accesses come before the copies of the next tile here
     }
-    mbar_arrive_warp(smem_addr(&s_empty[stage]), lane, alive);
+    mbar_arrive_warp(smem_addr(&s_empty[stage]), lane, true);
+  }
+  // A wait of this warp ran out. The copies may still arrive for the other warps, which
+  // then meet it at the ends of their pieces: it comes there as often as they do, by the
+  // lengths alone (the notes may be another lap's), and neither reads nor stores.
+  if (i < count) wait_for_previous();
+  for (; i < count; ++i) {
+    const TileEnd end = tile_end(s_begin[0], s_begin[1], count, i, [&](uint32_t s) { return seq_info(a, s, prefix).tiles; });
+    if (!end.last) continue;
+    for (int k = 0; k < kMeets; ++k) meet();
+    if (!end.whole) {
+      if (threadIdx.x == 0) s_last = 0;
+      meet();
+    }
   }
 }
 
