@@ -588,7 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         any_hi = every_hi = it.limit - 1;
         any_lo = every_lo = it.low;
       }
-      // Does the tile hold tokens that not every row sees (every: of the item)?
+      const bool mixed = kPrefix && (every_hi != any_hi || every_lo != any_lo);
+      // Does the tile hold tokens that not every row of the item sees?
       auto partly_seen = [&](int token) {
         return token + kTokens - 1 > every_hi || (token < every_lo && token + kTokens > it.sinks);
       };
@@ -690,7 +691,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
             // half of the rows; both come here, and neither goes on alone. One that some
             // sequences' rows see must not reach the others': where it is not finite it is
             // kept from the product, and added to its rows' sums behind the last one.
-            if ((kPrefix || masked) && partly_seen(token)) {
+            if ((masked || mixed) && partly_seen(token)) {
               const uint32_t v = 2 * (tiles_done + j) + 1, of = r % kHalfRows, halves = it.rows > kHalfRows ? 2 : 1;
               wait(full((v + 1) / 2), full_phase((v + 1) / 2));
               const int mine = token + static_cast<int>(of);
@@ -702,7 +703,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
               };
               if (mine > any_hi || (mine < any_lo && mine >= it.sinks)) {
                 for (uint32_t c = h; c < D / 8; c += halves) put(place_of(c), {0, 0, 0, 0});
-              } else if (kPrefix && (mine > every_hi || (mine < every_lo && mine >= it.sinks))) {
+              } else if (mixed && (mine > every_hi || (mine < every_lo && mine >= it.sinks))) {
 #pragma unroll 1
                 for (uint32_t c = h; c < D / 8; c += halves) {
                   uint32_t x[4], y[4];
@@ -781,7 +782,7 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
         }
         wait(bar(kSummed, h), summed++);
         tmem_fence_after();
-        if (kPrefix && *static_cast<volatile uint32_t*>(&s_left_out[pieces & 1]) == pieces + 1) {
+        if (mixed && *static_cast<volatile uint32_t*>(&s_left_out[pieces & 1]) == pieces + 1) {
           // The values that were kept from this piece's products, read again: an infinity
           // or NaN is one whatever its weight.
 #pragma unroll 1
