@@ -607,12 +607,13 @@ uint64_t tcx_kv_attention_scratch_bytes(const tcx_kv_attention_args* args);
  * d_seq_tokens may change between calls (also between replays of a captured
  * one), up to the pages' capacity. Rows of out and lse from q_tokens on are not
  * touched. Table entries are checked on the device: a bad one leaves a non-zero
- * code in *d_status (1 slot out of the pool, 2 more tokens than the pages hold;
- * 4: a wait inside the kernel ran out) and nothing outside the pool is read; the rows of that sequence are then not
- * meaningful. Calls that may run at the same time need their own scratch and
- * counters. Values of tokens that
- * none of a sequence's queries sees are never used, whatever they hold; a
- * non-finite value of a token that some of them see may reach the others. */
+ * code in *d_status (1 slot out of the pool, 2 more tokens than the pages hold)
+ * and nothing outside the pool is read; the rows of that sequence are then not
+ * meaningful. Code 4: a wait inside the kernel ran out, and no row is. Calls that
+ * may run at the same time need their own scratch and counters. Values of tokens
+ * that none of a sequence's queries sees never reach it, whatever they hold (also
+ * those of a shared prefix that other sequences see); a non-finite value of a
+ * token that some of its queries see may reach its others. */
 tcx_status tcx_kv_attention(const tcx_kv_attention_args* args, void* d_scratch, uint64_t scratch_bytes, void* stream);
 
 /* Eviction: sequence s of n = d_seq_tokens[s] tokens keeps min(n, d_budgets[s])

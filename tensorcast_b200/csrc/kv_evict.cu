@@ -25,7 +25,7 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kBins = 2048;
 constexpr int kBatch = 8;                 // tokens of a thread in a round of the last pass
-constexpr uint32_t kHeldTokens = 14336;   // images that shared memory holds: 56 KiB, three CTAs on an SM
+constexpr uint32_t kHeldTokens = 14336;   // images that shared memory holds: 56 KiB (registers leave two CTAs on an SM)
 constexpr int kSelectShared = kHeldTokens * 4;
 
 struct EvictArgs {

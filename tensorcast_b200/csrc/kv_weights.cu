@@ -9,10 +9,10 @@
 // keeping them would take rows x tokens x 4 bytes. Two CTAs share an SM, so that one's
 // fetches run beside the other's exponentials. The exponential units bound it, at 0.45
 // of their rate while an SM has work (a fourth of the exponentials as polynomials
-// changed less than 1 %); over the whole call 0.34, because 657 CTAs are 2.2 rounds.
+// changed less than 1 %); over the whole call 0.36, because 657 CTAs are 2.2 rounds.
 // Measured on B200: 256 queries at the ends of two sequences of 5000-6100 tokens, 32 / 8
-// heads of 128, 65 us beside 75 us for their attention (69 us with one thread for all
-// 128 rows of a key).
+// heads of 128, 58 to 62 us beside 70 us for their attention (4 us more with one thread
+// for all 128 rows of a key).
 #include <algorithm>
 #include <type_traits>
 

@@ -14,7 +14,9 @@ Both work on the pool and the tables of ``kvcache.KvWorkload`` (a token row of a
 An object holds the tables of one batch on the device. ``seq_tokens`` (and ``prefix_tokens``) are
 read on the device by every call, so a program lets a sequence grow by writing them in place, up
 to the pages' capacity, also between the replays of a captured call; page tables may be written in
-place likewise. The object must live as long as a graph that captured its calls. Everything is
+place likewise. Every object has its own copy of the lengths, made from ``w.seq_tokens``: where one
+object's sequences have grown, another one (the eviction behind some steps of decode, say) is given
+them by ``other.seq_tokens.copy_(grown.seq_tokens)``. The object must live as long as a graph that captured its calls. Everything is
 inference: no gradients.
 """
 from __future__ import annotations
@@ -313,8 +315,9 @@ class KvEvict(_OnDevice):
 
     ``dst`` holds the pages that the kept rows are copied to, in their old order, and the budgets as
     its ``seq_tokens``; its pages must be distinct and none of ``w``'s. A budget must hold ``sinks +
-    recent`` tokens, or the whole sequence where that is shorter. The source pages are only
-    read: other sequences may share them. Rows are copied whole, so the element type does not matter.
+    recent`` tokens, or the whole sequence where that is shorter. Where a sequence outgrows such a
+    budget in place (``seq_tokens``), its first ``sinks`` tokens stay and as many of the newest as the
+    budget holds behind them. The source pages are only read: other sequences may share them. Rows are copied whole, so the element type does not matter.
     """
 
     def __init__(self, w: KvWorkload, dst: KvWorkload, kv_heads: int, *, sinks: int = 0, recent: int = 0,
