@@ -81,13 +81,18 @@ __device__ __forceinline__ uint64_t checked_slot(const AttnArgs& a, const uint32
 
 // A finished row: o = sum of 2^(z - m) v and l = sum of 2^(z - m) become
 //   o * own + prior_o * prior,  lse (in powers of two)
+// A part that the row sees counts even where its weight has become 0, so that infinities
+// and NaN show; one that it does not see is 0, whatever the sums hold.
 struct Finish {
   float own, prior, lse;
+  bool sees_own, sees_prior;
 };
 
 __device__ __forceinline__ Finish finish_row(const AttnArgs& a, uint64_t row, float m, float l) {
   Finish f;
-  f.own = l == 0.f ? 0.f : 1.f / l;
+  f.sees_own = l != 0.f;
+  f.sees_prior = false;
+  f.own = f.sees_own ? 1.f / l : 0.f;
   f.prior = 0.f;
   f.lse = m + log2f(l);  // l 0: m is -inf, and so is this
   if (a.prior_lse != nullptr) {
@@ -96,6 +101,7 @@ __device__ __forceinline__ Finish finish_row(const AttnArgs& a, uint64_t row, fl
     const float w = exp2f(f.lse - ref), wp = exp2f(p - ref), sum = w + wp;
     f.own = w == 0.f ? 0.f : f.own * w / sum;
     f.prior = wp == 0.f ? 0.f : wp / sum;
+    f.sees_prior = p != -INFINITY;
     f.lse = top + log2f(sum);
   }
   return f;
@@ -108,8 +114,8 @@ __device__ __forceinline__ void store_row(const AttnArgs& a, uint32_t t, uint32_
   const uint64_t row = static_cast<uint64_t>(t) * a.kv_heads * a.group + h;
   float x[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = f.own == 0.f ? 0.f : v[i] * f.own;  // nothing seen here: 0, whatever the sums hold
-  if (f.prior != 0.f) {
+  for (int i = 0; i < 4; ++i) x[i] = f.sees_own ? v[i] * f.own : 0.f;
+  if (f.sees_prior) {
     const float4 y = *reinterpret_cast<const float4*>(a.prior_o + row * D + e);
     x[0] += f.prior * y.x;
     x[1] += f.prior * y.y;

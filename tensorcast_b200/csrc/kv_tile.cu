@@ -846,8 +846,8 @@ __global__ void __launch_bounds__(kThreads, 1) tile_kernel(const __grid_constant
           for (int i = 0; i < 32; ++i) x[i] = __uint_as_float(o[i]);
           if (!whole) return;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) x[i] = f.own == 0.f ? 0.f : x[i] * f.own;  // nothing seen: 0
-          if (f.prior != 0.f) {
+          for (int i = 0; i < 32; ++i) x[i] = f.sees_own ? x[i] * f.own : 0.f;
+          if (f.sees_prior) {
             const float4* y = reinterpret_cast<const float4*>(a.prior_o + q_row * D + c);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {

@@ -781,6 +781,27 @@ def test_strides_of_single_tokens_and_heads_do_not_matter(cuda_device):
     assert (odd[0] == out).all() and (odd[1] == lse).all() and (got == want).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("count", [1, 40])
+@pytest.mark.parametrize("where", ["prefix", "own"])
+def test_non_finite_values_show_through_a_weight_of_zero(cuda_device, where, count):
+    """A row sees a prefix and its own tokens, one of which weighs nothing in 32 bits beside the other."""
+    prefix, n = 20, 60
+    w, free = kvtools.tables([n], taken=2, kv_heads=1)
+    pool = kvtools.make_pool(w, 1, 64, BF16)
+    rows = free[:2][np.arange(prefix) // 16].astype(np.int64) * 16 + np.arange(prefix) % 16
+    mine = kvtools.token_rows(w, 0)
+    pool[0, torch.from_numpy(rows), :, 0] = 30.0 if where == "own" else -30.0
+    pool[0, torch.from_numpy(mine), :, 0] = -30.0 if where == "own" else 30.0
+    at = int(rows[7] if where == "prefix" else mine[7])
+    pool[1, at, 0, 3], pool[1, at, 0, 4] = math.inf, math.nan
+    q = queries(count, 4, 64, BF16, 0)
+    q[:, :, 0] = 40.0
+    out, lse = KvAttention(w, 4, 1, query_tokens=[count], prefix_pages=free[:2], prefix_tokens=prefix).run(pool.cuda(), 0, q)
+    assert not torch.isfinite(out[..., 3:5]).any()
+    assert torch.isfinite(out[..., :3]).all() and torch.isfinite(out[..., 5:]).all() and torch.isfinite(lse).all()
+
+
 # ---------------------------------------------------------------- accumulated weights (GPU)
 
 @pytest.mark.gpu
