@@ -66,7 +66,10 @@ def _check_tables(w: KvWorkload, what: str) -> None:
     if int(offs[-1]) != np.asarray(w.page_table).size:
         _refuse(f"{what}: page_offsets end at {int(offs[-1])}, the page table has {np.asarray(w.page_table).size}")
     _slots(w.page_table, what)
-    if (np.asarray(w.seq_tokens).astype(np.int64) > np.diff(offs) * w.page_tokens).any():
+    tokens = np.asarray(w.seq_tokens).astype(np.int64)
+    if (tokens < 0).any():
+        _refuse(f"{what}: seq_tokens must not be negative")
+    if (tokens > np.diff(offs) * w.page_tokens).any():
         _refuse(f"{what}: a sequence has more tokens than its pages hold")
 
 

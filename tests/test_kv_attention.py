@@ -110,6 +110,15 @@ extern "C" int ends(const uint32_t* tiles, uint32_t seq, uint32_t tile, uint32_t
                 assert got == last + 2 * whole, (ranges, r, i)
 
 
+def test_negative_lengths_are_refused():
+    """They would count as more than 2^31 tokens, which the device cuts to the pages' capacity."""
+    w, free = kvtools.tables([5, 40], taken=3)
+    bad = KvWorkload(**{**w.__dict__, "seq_tokens": np.array([5, -1])})
+    refused("negative", lambda: KvAttention(bad, 4, 2, device="cpu"))
+    refused("negative", lambda: KvEvict(bad, w, 2, device="cpu"))
+    refused("negative", lambda: KvEvict(w, bad, 2, device="cpu"))
+
+
 def attention_args(**kw):
     """Arguments that pass the checks of the C entry, made-up pointers among them, with `kw` changed."""
     a = _native.KvAttentionArgs(
