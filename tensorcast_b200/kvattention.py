@@ -160,6 +160,8 @@ class KvAttention(_OnDevice):
             _refuse(f"planes must be layers x {{K, V}}, got {w.planes}")
         if window < 0 or sinks < 0:
             _refuse("window and sinks must not be negative")
+        if max(window, sinks) >= 1 << 30:
+            _refuse("window and sinks must be below 2^30")
         head_dim = w.token_bytes // (2 * kv_heads)
         scale = head_dim ** -0.5 if scale is None else float(scale)
         if not scale > 0 or not math.isfinite(scale):
@@ -359,7 +361,8 @@ class KvEvict(_OnDevice):
             d_page_offsets=t.page_offsets.data_ptr(), d_seq_tokens=t.seq_tokens.data_ptr(),
             d_dst_page_table=t.dst_page_table.data_ptr() or t.buffer.data_ptr(),
             d_dst_page_offsets=t.dst_page_offsets.data_ptr(), d_budgets=t.budgets.data_ptr(), n_seq=w.n_seq,
-            dst_total_pages=int(dst.page_offsets[-1]), sinks=sinks, recent=recent, d_status=t.status.data_ptr())
+            dst_total_pages=int(dst.page_offsets[-1]), sinks=min(sinks, 1 << 32), recent=min(recent, 1 << 32),
+            d_status=t.status.data_ptr())
         layers = w.planes // 2
         self._weights_shape = (layers, kv_heads, int(w.page_offsets[-1]) * w.page_tokens)
         shape = (layers, kv_heads, int(dst.page_offsets[-1]) * dst.page_tokens)

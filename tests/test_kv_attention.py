@@ -119,6 +119,14 @@ def test_negative_lengths_are_refused():
     refused("negative", lambda: KvEvict(w, bad, 2, device="cpu"))
 
 
+def test_windows_and_sinks_beyond_every_length_are_refused_at_once():
+    """2^64 + 3 must not become 3 on its way to the entry point."""
+    w, _ = kvtools.tables([5, 40])
+    for size in (1 << 30, (1 << 64) + 3):
+        refused("below 2\\^30", lambda: KvAttention(w, 4, 2, window=size, device="cpu"))
+        refused("below 2\\^30", lambda: KvAttention(w, 4, 2, sinks=size, device="cpu"))
+
+
 def attention_args(**kw):
     """Arguments that pass the checks of the C entry, made-up pointers among them, with `kw` changed."""
     a = _native.KvAttentionArgs(
@@ -969,6 +977,23 @@ def test_evict_reports_bad_tables(cuda_device):
     ev = KvEvict(w, dst, 2)
     refused("weights must be", lambda: ev.run(pool, weights[:, :1]))
     refused("weights must be", lambda: ev.run(pool, weights.half()))
+
+
+@pytest.mark.gpu
+def test_evict_with_more_sinks_than_64_bits_hold(cuda_device):
+    """Everything stays while the budget holds it; of a sequence that outgrows the budget, its first tokens."""
+    w, free = kvtools.tables([20], spare=2, taken=2)
+    pool = kvtools.make_pool(w, 2, 64, BF16).cuda()
+    dst = KvWorkload(w.planes, w.pool_pages, 16, w.token_bytes, np.array([25], np.uint32), np.array([0, 2], np.uint64),
+                     free[:2].copy())
+    weights = torch.rand((1, 2, int(w.page_offsets[-1]) * 16), device="cuda")
+    for sinks, recent, want in (((1 << 64) + 3, 0, np.arange(25)), (0, (1 << 64) + 3, np.arange(15, 40)),
+                                (7, 1 << 64, np.r_[:7, 22:40])):
+        ev = KvEvict(w, dst, 2, sinks=sinks, recent=recent)
+        assert (ev.run(pool, weights)[0][0, :, :20].cpu().numpy() == np.arange(20)).all()
+        ev.seq_tokens.fill_(40)
+        assert (ev.run(pool, weights)[0][0, :, :25].cpu().numpy() == want).all()
+        ev.check_status()
 
 
 # ---------------------------------------------------------------- together
